@@ -11,10 +11,13 @@
 #include <type_traits>
 
 #include "../../include/expert_cache.h"
+#include "adapters.h"
 #include "align.h"
+#include "experts.h"
 #include "gather.h"
 #include "manage.h"
 #include "refresh.h"
+#include "route.h"
 
 namespace ec {
 namespace {
@@ -139,6 +142,84 @@ ManageArgs make_args(const void* ids, int mk, int E, int S, int max_distinct, in
   a.decay = decay;
   a.out = out;
   return a;
+}
+
+// ---- operators over slots -----------------------------------------------------------------
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <class X, bool BIAS>
+void launch_route_of(const RouteArgs& a, hipStream_t stream) {
+  const dim3 grid((a.T - 1) / kRouteWaves + 1), block(kRouteWaves * kWave);
+  if (a.E <= 64)
+    hipLaunchKernelGGL((route_k<X, 1, BIAS>), grid, block, 0, stream, a);
+  else if (a.E <= 128)
+    hipLaunchKernelGGL((route_k<X, 2, BIAS>), grid, block, 0, stream, a);
+  else if (a.E <= 256)
+    hipLaunchKernelGGL((route_k<X, 4, BIAS>), grid, block, 0, stream, a);
+  else if (a.E <= 512)
+    hipLaunchKernelGGL((route_k<X, 8, BIAS>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((route_k<X, 16, BIAS>), grid, block, 0, stream, a);
+}
+
+template <class X>
+int launch_route(const RouteArgs& a, hipStream_t stream) {
+  if (a.bias)
+    launch_route_of<X, true>(a, stream);
+  else
+    launch_route_of<X, false>(a, stream);
+  return (int)hipGetLastError();
+}
+
+bool experts_bad(const expert_cache_experts* e, int T, int top_k) {
+  if (e == nullptr || e->S <= 0 || e->H <= 0 || e->I <= 0) return true;
+  if (e->type != EXPERT_CACHE_BF16 && e->type != EXPERT_CACHE_F16) return true;
+  const bool byte = e->weights == EXPERT_CACHE_INT8 || e->weights == EXPERT_CACHE_E4M3;
+  if (!byte && e->weights != e->type) return true;
+  if (e->H % (byte ? 16 : 8) || e->I % (byte ? 16 : 8)) return true;
+  if (T < 0 || top_k <= 0 || top_k > kExpertsMaxK) return true;
+  return (long long)T * top_k > kExpertsMaxPairs;
+}
+
+template <class X, class W>
+int launch_moe(const ExpertsArgs& a, int T, hipStream_t stream) {
+  const int groups = a.by_slot ? a.S : a.n;
+  hipLaunchKernelGGL((experts_up_k<X, W, 4, 2>), dim3((a.I - 1) / 16 + 1, groups), dim3(256), 0,
+                     stream, a);
+  int rc = (int)hipGetLastError();
+  if (rc) return rc;
+  hipLaunchKernelGGL((experts_down_k<W, 4, 2>), dim3((a.H - 1) / 16 + 1, groups), dim3(256), 0,
+                     stream, a);
+  rc = (int)hipGetLastError();
+  if (rc) return rc;
+  hipLaunchKernelGGL((experts_sum_k<X>), dim3((a.H - 1) / 1024 + 1, T), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+bool adapters_bad(const expert_cache_adapters* l, int T) {
+  if (l == nullptr || l->S <= 0 || l->O <= 0 || l->H <= 0 || l->R <= 0 || T < 0) return true;
+  if (l->type != EXPERT_CACHE_BF16 && l->type != EXPERT_CACHE_F16) return true;
+  return l->H % 8 || l->R % 8 || l->R > kAdapterMaxRank;
+}
+
+// Workgroups that share the hidden length of a tile's product.
+int adapter_splits(int T, int H) {
+  const int tiles = (T - 1) / kAdapterTile + 1, most = (H + 4 * kUnit - 1) / (4 * kUnit);
+  const int want = 256 / tiles;
+  return want < 1 ? 1 : want < most ? want : most;
+}
+
+template <class X>
+int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
+  const int tiles = (a.T - 1) / kAdapterTile + 1;
+  hipLaunchKernelGGL((adapters_shrink_k<X, 4>), dim3(tiles, kAdapterTile, a.splits), dim3(256),
+                     0, stream, a);
+  const int rc = (int)hipGetLastError();
+  if (rc) return rc;
+  hipLaunchKernelGGL((adapters_expand_k<X, 4>), dim3(tiles, (a.O - 1) / 64 + 1), dim3(256), 0,
+                     stream, a);
+  return (int)hipGetLastError();
 }
 
 }  // namespace
@@ -316,6 +397,121 @@ int expert_cache_gather_live(void* d0, const void* s0, long b0, void* d1, const 
   hipLaunchKernelGGL((gather_k<kGatherUnroll, true, false, true>), dim3(chunks, lanes),
                      dim3(kGatherThreads), 0, stream, g, miss, n_miss, slot_expert);
   return (int)hipGetLastError();
+}
+
+int expert_cache_route(const void* logits, int type, long row_stride, const float* bias, int T,
+                       int E, int top_k, int scoring, int groups, int topk_groups,
+                       int renormalize, float scale, float* weights, void* ids, int id_bytes,
+                       hipStream_t stream) {
+  if (T < 0 || E <= 0 || E > kRouteMaxExperts || (row_stride < E && T > 1)) return -1;
+  if (scoring < 0 || scoring > 1 || (id_bytes != 4 && id_bytes != 8)) return -1;
+  if (groups < 1 || groups > kRouteMaxGroups || E % groups) return -1;
+  if (topk_groups < 1 || topk_groups > groups) return -1;
+  if (top_k < 1 || top_k > kRouteMaxK || top_k > topk_groups * (E / groups)) return -1;
+  if (type < EXPERT_CACHE_F32 || type > EXPERT_CACHE_F16) return -1;
+  if (T == 0) return 0;
+  if (logits == nullptr || weights == nullptr || ids == nullptr) return -1;
+  const RouteArgs a = {logits,       row_stride,       bias,          T,     E,       top_k, groups,
+                       topk_groups,  scoring == 1,     renormalize != 0, id_bytes == 8, scale,
+                       weights,      ids};
+  if (type == EXPERT_CACHE_F32) return launch_route<float>(a, stream);
+  return type == EXPERT_CACHE_BF16 ? launch_route<Bf16>(a, stream) : launch_route<F16>(a, stream);
+}
+
+int expert_cache_moe_workspace(const expert_cache_experts* e, int T, int top_k, long* bytes) {
+  if (bytes == nullptr || experts_bad(e, T, top_k)) return -1;
+  *bytes = 4L * T * top_k * (e->I + e->H);
+  return 0;
+}
+
+int expert_cache_moe(const expert_cache_experts* e, const void* x, long x_stride,
+                     const float* topk_weights, const void* ids, int id_bytes, int T, int top_k,
+                     void* out, long out_stride, void* workspace, hipStream_t stream) {
+  if (experts_bad(e, T, top_k) || (id_bytes != 4 && id_bytes != 8)) return -1;
+  if (T == 0) return 0;
+  if (e->w13 == nullptr || e->w2 == nullptr || !aligned16(e->w13) || !aligned16(e->w2)) return -1;
+  if (e->weights >= EXPERT_CACHE_INT8 && (e->s13 == nullptr || e->s2 == nullptr)) return -1;
+  if (x == nullptr || !aligned16(x) || (T > 1 && (x_stride % 8 || x_stride < e->H))) return -1;
+  if (out == nullptr || (out_stride < e->H && T > 1)) return -1;
+  if (topk_weights == nullptr || ids == nullptr) return -1;
+  if (workspace == nullptr || !aligned16(workspace)) return -1;
+  if (ranges_meet(x, 2 * ((T - 1LL) * x_stride + e->H), out,
+                  2 * ((T - 1LL) * out_stride + e->H)))
+    return -1;
+  ExpertsArgs a;
+  a.x = x;
+  a.x_stride = x_stride;
+  a.w13 = e->w13;
+  a.w2 = e->w2;
+  a.s13 = e->s13;
+  a.s2 = e->s2;
+  a.probs = topk_weights;
+  a.ids = ids;
+  a.n = T * top_k;
+  a.k = top_k;
+  a.S = e->S;
+  a.H = e->H;
+  a.I = e->I;
+  a.wide = id_bytes == 8;
+  a.by_slot = a.n > a.S;
+  a.hi = static_cast<Bf16*>(workspace);
+  a.lo = a.hi + (long long)a.n * a.I;
+  a.part = reinterpret_cast<float*>(a.lo + (long long)a.n * a.I);
+  a.out = out;
+  a.out_stride = out_stride;
+  if (e->type == EXPERT_CACHE_BF16) {
+    if (e->weights == EXPERT_CACHE_INT8) return launch_moe<Bf16, int8_t>(a, T, stream);
+    if (e->weights == EXPERT_CACHE_E4M3) return launch_moe<Bf16, E4m3>(a, T, stream);
+    return launch_moe<Bf16, Bf16>(a, T, stream);
+  }
+  if (e->weights == EXPERT_CACHE_INT8) return launch_moe<F16, int8_t>(a, T, stream);
+  if (e->weights == EXPERT_CACHE_E4M3) return launch_moe<F16, E4m3>(a, T, stream);
+  return launch_moe<F16, F16>(a, T, stream);
+}
+
+int expert_cache_adapt_workspace(const expert_cache_adapters* l, int T, long* bytes) {
+  if (bytes == nullptr || adapters_bad(l, T)) return -1;
+  *bytes = T == 0 ? 0 : 4L * adapter_splits(T, l->H) * T * l->R;
+  return 0;
+}
+
+int expert_cache_adapt(const expert_cache_adapters* l, const void* x, long x_stride,
+                       const void* ids, int id_bytes, int T, const void* base,
+                       long base_stride, void* out, long out_stride, void* workspace,
+                       hipStream_t stream) {
+  if (adapters_bad(l, T) || (id_bytes != 4 && id_bytes != 8)) return -1;
+  if (T == 0) return 0;
+  if (l->a == nullptr || l->b == nullptr || !aligned16(l->a) || !aligned16(l->b)) return -1;
+  if (x == nullptr || !aligned16(x) || (T > 1 && (x_stride % 8 || x_stride < l->H))) return -1;
+  if (base == nullptr || out == nullptr || ids == nullptr) return -1;
+  if ((base_stride < l->O || out_stride < l->O) && T > 1) return -1;
+  if (workspace == nullptr || !aligned16(workspace)) return -1;
+  const long long out_bytes = 2 * ((T - 1LL) * out_stride + l->O);
+  const bool in_place = out == base && (out_stride == base_stride || T == 1);
+  if (!in_place && ranges_meet(base, 2 * ((T - 1LL) * base_stride + l->O), out, out_bytes))
+    return -1;
+  if (ranges_meet(x, 2 * ((T - 1LL) * x_stride + l->H), out, out_bytes)) return -1;
+  AdaptersArgs a;
+  a.x = x;
+  a.x_stride = x_stride;
+  a.a = l->a;
+  a.b = l->b;
+  a.scales = l->scales;
+  a.ids = ids;
+  a.base = base;
+  a.base_stride = base_stride;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.T = T;
+  a.S = l->S;
+  a.H = l->H;
+  a.O = l->O;
+  a.R = l->R;
+  a.splits = adapter_splits(T, l->H);
+  a.wide = id_bytes == 8;
+  a.v = static_cast<float*>(workspace);
+  return l->type == EXPERT_CACHE_BF16 ? launch_adapt<Bf16>(a, stream)
+                                      : launch_adapt<F16>(a, stream);
 }
 
 }  // extern "C"

@@ -6,9 +6,9 @@ Same search order and same argument lists for the reference's two bound entry po
 points that replace the reference's torch remap, `expert_cache_prefetch`,
 `expert_cache_manage_remap_prefetch` (one layer's policy step with another's prefetch step
 in one launch), `expert_cache_gather_live` (the prefetch copy that stops for dropped
-predictions), and `expert_cache_refresh` (policy step, remap and gather in one call). Every
-call is asynchronous on the caller's stream and never reads a device value back, so the whole
-path is HIP-graph capturable.
+predictions), and `expert_cache_refresh` (policy step, remap and gather in one call); and the
+operators of ops.py with the workspace sizes of two of them. Every call is asynchronous on the
+caller's stream and never reads a device value back, so the whole path is HIP-graph capturable.
 
 There is no fallback: if the library or one of its symbols is missing, loading fails with
 an error that says so.
@@ -58,6 +58,19 @@ SIGNATURES = {
                                            + [_P, _I, _I] + [_P] * 7 + [_P]),
     # refresh(layer, ids, id_bytes, mk, out, stream)
     "expert_cache_refresh": [_P, _P, _I, _I, _P, _P],
+    # route(logits, type, row_stride, bias, T, E, top_k, scoring, groups, topk_groups,
+    #       renormalize, scale, weights, ids, id_bytes, stream)
+    "expert_cache_route": ([_P, _I, _L, _P] + [_I] * 7 + [ctypes.c_float, _P, _P, _I, _P]),
+    # moe_workspace(experts, T, top_k, bytes)
+    "expert_cache_moe_workspace": [_P, _I, _I, _P],
+    # moe(experts, x, x_stride, topk_weights, ids, id_bytes, T, top_k, out, out_stride,
+    #     workspace, stream)
+    "expert_cache_moe": [_P, _P, _L, _P, _P, _I, _I, _I, _P, _L, _P, _P],
+    # adapt_workspace(adapters, T, bytes)
+    "expert_cache_adapt_workspace": [_P, _I, _P],
+    # adapt(adapters, x, x_stride, ids, id_bytes, T, base, base_stride, out, out_stride,
+    #       workspace, stream)
+    "expert_cache_adapt": [_P, _P, _L, _P, _I, _I, _P, _L, _P, _L, _P, _P],
 }
 
 
@@ -68,6 +81,20 @@ class Layer(ctypes.Structure):
                 + [(n, _P) for n in ("table", "map_cold", "slot_expert", "slot_stamp",
                                      "routed", "step", "miss", "n_miss", "arrived")]
                 + [("dst", _P * 6), ("src", _P * 6), ("bytes", _L * 6)])
+
+
+class Experts(ctypes.Structure):
+    """expert_cache_experts: the weights of one layer's experts."""
+
+    _fields_ = ([(n, _I) for n in ("S", "H", "I", "type", "weights")]
+                + [(n, _P) for n in ("w13", "w2", "s13", "s2")])
+
+
+class Adapters(ctypes.Structure):
+    """expert_cache_adapters: the low-rank adapters of one projection."""
+
+    _fields_ = ([(n, _I) for n in ("S", "H", "O", "R", "type")]
+                + [(n, _P) for n in ("a", "b", "scales")])
 
 
 def library_path() -> str:

@@ -1,0 +1,301 @@
+"""Operators around the slot cache: the routing that makes its ids, and the products over what
+its slots hold.
+
+    weights, ids = route(logits, top_k)               # expert ids from the gate's logits
+    slots = cache.refresh(ids)                        # experts into slots (cache.py)
+    y = Experts(w13_slots, w2_slots)(x, weights, slots)
+
+    slots = adapter_cache.refresh(adapter_ids)        # the same for adapters of requests
+    y = Adapters(a_slots, b_slots)(x, projected, slots)
+
+`Experts` and `Adapters` check their weights once and are kept like the weights themselves; a
+cache's slot tensors never move, so a handle over them stays good. Weights are used as they lie,
+without another layout. Calls run on the current stream of the tensors' device, allocate only
+their result and a workspace through torch, and read nothing back, so they can be captured.
+
+ValueError names an argument that an operator does not take; nothing has run then.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_TOKENS = {torch.bfloat16: 1, torch.float16: 2}
+_LOGITS = {torch.float32: 0, **_TOKENS}
+_BYTES = {torch.int8: 3, torch.float8_e4m3fn: 4}
+_SCORING = {"softmax": 0, "sigmoid": 1}
+_BLOCK = 128  # rows and columns of e4m3 weights that share a scale
+
+MAX_PAIRS = 1024    # tokens x top_k of one Experts call
+MAX_TOP_K = 64
+MAX_EXPERTS = 1024  # of one routing
+MAX_RANK = 256
+
+
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` as rows that the kernels can load 16 bytes at a time: itself, or a copy."""
+    if t.stride(1) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and
+                                                 (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _ids(ids: torch.Tensor, device) -> tuple[torch.Tensor, int]:
+    _need(ids.dtype in (torch.int32, torch.int64), f"ids must be int32 or int64, not {ids.dtype}")
+    _need(ids.device == device, f"ids are on {ids.device}, not {device}")
+    return ids.contiguous(), ids.element_size()
+
+
+class _On:
+    """The current stream of `device`, with that device current."""
+
+    __slots__ = ("device", "guard")
+
+    def __init__(self, device):
+        self.device = device
+        self.guard = None
+
+    def __enter__(self) -> int:
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _check(rc: int, name: str) -> None:
+    if rc != 0:
+        raise RuntimeError(f"{name} failed rc={rc}")
+
+
+def _on_gpu(*tensors) -> torch.device:
+    device = tensors[0].device
+    _need(device.type == "cuda", f"tensors must be on a GPU, not on {device}")
+    for t in tensors[1:]:
+        _need(t is None or t.device == device, "tensors are on different devices")
+    return device
+
+
+def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
+          bias: torch.Tensor | None = None, groups: int = 1, topk_groups: int = 1,
+          renormalize: bool = True, scale: float = 1.0,
+          id_dtype: torch.dtype = torch.int32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The `top_k` experts of every token: (weights float32 [T, top_k], ids [T, top_k]).
+
+    logits  [T, E] float32, bfloat16 or float16; E up to 1024
+    scoring "softmax" of a row, or "sigmoid" of each logit
+    bias    float32 [E] added to the scores for the selection alone
+    groups  select from the best `topk_groups` of this many equal groups (up to 64). A group
+            counts as its best expert, with a bias as the sum of its two best.
+    renormalize  divide the selected scores by their sum
+    scale   factor on the weights
+
+    Among equals the lowest id comes first. Experts whose logit is NaN or -inf are never
+    selected; where too few are left the id is -1 and the weight 0."""
+    _need(logits.dim() == 2, f"logits must be [T, E], not {tuple(logits.shape)}")
+    _need(logits.dtype in _LOGITS, f"logits must be float32, bfloat16 or float16, not {logits.dtype}")
+    _need(scoring in _SCORING, f"scoring must be softmax or sigmoid, not {scoring!r}")
+    _need(id_dtype in (torch.int32, torch.int64), f"ids are int32 or int64, not {id_dtype}")
+    T, E = logits.shape
+    _need(0 < E <= MAX_EXPERTS, f"{E} experts (1 to {MAX_EXPERTS})")
+    _need(1 <= groups <= 64 and E % groups == 0, f"{groups} groups of {E} experts")
+    _need(1 <= topk_groups <= groups, f"{topk_groups} of {groups} groups")
+    _need(1 <= top_k <= min(MAX_TOP_K, topk_groups * (E // groups)),
+          f"top_k {top_k} of {topk_groups} x {E // groups} experts (at most {MAX_TOP_K})")
+    if bias is not None:
+        _need(bias.dtype == torch.float32 and bias.shape == (E,) and bias.is_contiguous(),
+              f"bias must be contiguous float32 [{E}], not {bias.dtype} {tuple(bias.shape)}")
+    device = _on_gpu(logits, bias)
+    if logits.stride(1) != 1 or logits.stride(0) < E:
+        logits = logits.contiguous()
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
+    ids = torch.empty((T, top_k), dtype=id_dtype, device=device)
+    with _On(device) as stream:
+        _check(_lib.lib().expert_cache_route(
+            logits.data_ptr(), _LOGITS[logits.dtype], logits.stride(0),
+            bias.data_ptr() if bias is not None else None, T, E, top_k, _SCORING[scoring],
+            groups, topk_groups, bool(renormalize), scale, weights.data_ptr(), ids.data_ptr(),
+            ids.element_size(), stream), "expert_cache_route")
+    return weights, ids
+
+
+def _scales(s, shape, name: str, device):
+    _need(s is not None and s.dtype == torch.float32 and s.is_contiguous(),
+          f"{name} must be contiguous float32")
+    _need(tuple(s.shape) == shape or tuple(s.shape) == shape + (1,),
+          f"{name} must be {list(shape)}, not {list(s.shape)}")
+    _need(s.device == device, f"{name} is on {s.device}, not {device}")
+
+
+class Experts:
+    """The experts of one layer, in slots or all of them: a whole MoE layer for a few tokens.
+
+    w13  [S, 2*I, H]: gate rows, then up rows        w2  [S, H, I]
+    in bfloat16 or float16 (the tokens' type); int8 with float32 scales a row, w13_scale
+    [S, 2*I] or [S, 2*I, 1] and w2_scale [S, H] or [S, H, 1]; or float8_e4m3fn with float32
+    scales a 128 x 128 block, [S, ceil(2*I/128), ceil(H/128)] and [S, ceil(H/128), ceil(I/128)].
+    H and I are multiples of 8, with one-byte weights of 16.
+
+    Activations are not quantised: one-byte weights are widened to the tokens' type, sums are
+    32-bit, and only the result is rounded."""
+
+    def __init__(self, w13: torch.Tensor, w2: torch.Tensor, w13_scale: torch.Tensor | None = None,
+                 w2_scale: torch.Tensor | None = None):
+        _need(w13.dim() == 3 and w2.dim() == 3 and w13.dtype == w2.dtype,
+              "w13 and w2 must be [S, 2*I, H] and [S, H, I] of one type")
+        S, two, H = w13.shape
+        _need(two % 2 == 0 and tuple(w2.shape) == (S, H, two // 2) and min(S, two, H) > 0,
+              f"w13 {list(w13.shape)} does not go with w2 {list(w2.shape)}")
+        dtype = w13.dtype
+        _need(dtype in _TOKENS or dtype in _BYTES, f"weights of {dtype} are not supported")
+        least = 16 if dtype in _BYTES else 8
+        _need(H % least == 0 and (two // 2) % least == 0,
+              f"H {H} and I {two // 2} must be multiples of {least}")
+        for name, w in (("w13", w13), ("w2", w2)):
+            _need(w.is_contiguous() and w.data_ptr() % 16 == 0,
+                  f"{name} must be contiguous and 16-byte aligned")
+        device = _on_gpu(w13, w2)
+        if dtype == torch.int8:
+            _scales(w13_scale, (S, two), "w13_scale", device)
+            _scales(w2_scale, (S, H), "w2_scale", device)
+        elif dtype == torch.float8_e4m3fn:
+            _scales(w13_scale, (S, -(-two // _BLOCK), -(-H // _BLOCK)), "w13_scale", device)
+            _scales(w2_scale, (S, -(-H // _BLOCK), -(-two // 2 // _BLOCK)), "w2_scale", device)
+        else:
+            _need(w13_scale is None and w2_scale is None, f"weights of {dtype} have no scales")
+        self.w13, self.w2, self.w13_scale, self.w2_scale = w13, w2, w13_scale, w2_scale
+        self.S, self.H, self.I, self.device = S, H, two // 2, device
+        self.dtypes = (dtype,) if dtype in _TOKENS else tuple(_TOKENS)
+        self._structs = {}
+        for t in self.dtypes:
+            e = _lib.Experts(S, H, two // 2, _TOKENS[t], _BYTES.get(dtype, _TOKENS[t]),
+                             w13.data_ptr(), w2.data_ptr(),
+                             *[s.data_ptr() if s is not None else None
+                               for s in (w13_scale, w2_scale)])
+            self._structs[t] = (e, ctypes.addressof(e))
+        self._bytes: dict = {}
+
+    def __call__(self, x: torch.Tensor, topk_weights: torch.Tensor, slot_ids: torch.Tensor,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+        """The layer's output [T, H] for tokens x [T, H]: the sum over their slots of the routing
+        weight (float32 [T, top_k]) times the expert. slot_ids [T, top_k] are int32 or int64;
+        T x top_k is at most 1024. A pair whose id is outside [0, S) or whose weight is 0 adds
+        nothing (and an infinity in that expert does not show); a token without any other
+        pair gets zeros. `out`, if given, has contiguous rows and does not overlap x."""
+        _need(x.dim() == 2 and x.shape[1] == self.H, f"x must be [T, {self.H}], not {list(x.shape)}")
+        _need(x.dtype in self.dtypes, f"tokens of {x.dtype} do not go with {self.w13.dtype} weights")
+        _need(x.device == self.device, f"x is on {x.device}, not {self.device}")
+        T = x.shape[0]
+        _need(slot_ids.dim() == 2 and slot_ids.shape[0] == T and
+              topk_weights.shape == slot_ids.shape,
+              f"topk_weights {list(topk_weights.shape)} and slot_ids {list(slot_ids.shape)} must "
+              f"be [{T}, top_k]")
+        k = slot_ids.shape[1]
+        _need(1 <= k <= MAX_TOP_K and T * k <= MAX_PAIRS,
+              f"{T} tokens x top_k {k} (top_k at most {MAX_TOP_K}, {MAX_PAIRS} in all)")
+        _need(topk_weights.dtype == torch.float32 and topk_weights.device == self.device,
+              f"topk_weights must be float32 on {self.device}")
+        ids, nbytes = _ids(slot_ids, self.device)
+        topk_weights, x = topk_weights.contiguous(), _rows(x)
+        if out is None:
+            out = torch.empty((T, self.H), dtype=x.dtype, device=self.device)
+        else:
+            _out(out, x.dtype, (T, self.H), self.device)
+        struct = self._structs[x.dtype][1]
+        h = _lib.lib()
+        size = self._bytes.get((T, k))
+        if size is None:
+            size = self._bytes[T, k] = _workspace(h.expert_cache_moe_workspace, struct, T, k)
+        with _On(self.device) as stream:
+            work = torch.empty(size, dtype=torch.uint8, device=self.device)
+            _check(h.expert_cache_moe(struct, x.data_ptr(), x.stride(0), topk_weights.data_ptr(),
+                                      ids.data_ptr(), nbytes, T, k, out.data_ptr(),
+                                      out.stride(0), work.data_ptr(), stream), "expert_cache_moe")
+        return out
+
+
+def _workspace(entry, struct, *sizes) -> int:
+    size = ctypes.c_long()
+    _check(entry(struct, *sizes, ctypes.addressof(size)), entry.__name__)
+    return max(16, size.value)
+
+
+def _out(out, dtype, shape, device) -> None:
+    _need(out.dtype == dtype and tuple(out.shape) == shape and out.device == device and
+          out.stride(1) == 1 and (shape[0] < 2 or out.stride(0) >= shape[1]),
+          f"out must be {dtype} {list(shape)} on {device} with contiguous rows")
+
+
+class Adapters:
+    """Low-rank adapters in slots, added for every token to a projection that all share.
+
+    a  [S, R, H], b  [S, O, R] in bfloat16 or float16; scales float32 [S] or None (1).
+    H and R are multiples of 8, R at most 256."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None):
+        _need(a.dim() == 3 and b.dim() == 3 and a.dtype == b.dtype and a.dtype in _TOKENS,
+              "a and b must be [S, R, H] and [S, O, R] in bfloat16 or float16")
+        S, R, H = a.shape
+        _need(b.shape[0] == S and b.shape[2] == R and min(*a.shape, *b.shape) > 0,
+              f"a {list(a.shape)} does not go with b {list(b.shape)}")
+        _need(H % 8 == 0 and R % 8 == 0 and R <= MAX_RANK,
+              f"H {H} and R {R} must be multiples of 8, R at most {MAX_RANK}")
+        for name, w in (("a", a), ("b", b)):
+            _need(w.is_contiguous() and w.data_ptr() % 16 == 0,
+                  f"{name} must be contiguous and 16-byte aligned")
+        self.device = _on_gpu(a, b, scales)
+        if scales is not None:
+            _scales(scales, (S,), "scales", self.device)
+        self.a, self.b, self.scales = a, b, scales
+        self.S, self.R, self.H, self.O, self.dtype = S, R, H, b.shape[1], a.dtype
+        self._struct = _lib.Adapters(S, H, b.shape[1], R, _TOKENS[a.dtype], a.data_ptr(),
+                                     b.data_ptr(), scales.data_ptr() if scales is not None
+                                     else None)
+        self._at = ctypes.addressof(self._struct)
+        self._bytes: dict = {}
+
+    def __call__(self, x: torch.Tensor, base: torch.Tensor, slot_ids: torch.Tensor,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+        """base + scale * b[s] (a[s] x) for every token, s its slot id ([T], int32 or int64);
+        x [T, H], base [T, O]. A token whose id is outside [0, S) has no adapter: its row is
+        base's. `out` may be base, whose rows without an adapter are then not written; any
+        other `out` does not overlap base or x."""
+        _need(x.dim() == 2 and x.shape[1] == self.H, f"x must be [T, {self.H}], not {list(x.shape)}")
+        T = x.shape[0]
+        _need(tuple(base.shape) == (T, self.O), f"base must be [{T}, {self.O}], not {list(base.shape)}")
+        _need(x.dtype == self.dtype and base.dtype == self.dtype,
+              f"x and base must be {self.dtype}, not {x.dtype} and {base.dtype}")
+        _need(x.device == self.device and base.device == self.device,
+              f"x and base must be on {self.device}")
+        _need(slot_ids.dim() == 1 and slot_ids.shape[0] == T,
+              f"slot_ids must be [{T}], not {list(slot_ids.shape)}")
+        ids, nbytes = _ids(slot_ids, self.device)
+        x = _rows(x)
+        if out is None:
+            out = torch.empty((T, self.O), dtype=self.dtype, device=self.device)
+        else:
+            _out(out, self.dtype, (T, self.O), self.device)
+        if base.stride(1) != 1 or (T > 1 and base.stride(0) < self.O):
+            base = base.contiguous()
+        h = _lib.lib()
+        size = self._bytes.get(T)
+        if size is None:
+            size = self._bytes[T] = _workspace(h.expert_cache_adapt_workspace, self._at, T)
+        with _On(self.device) as stream:
+            work = torch.empty(size, dtype=torch.uint8, device=self.device)
+            _check(h.expert_cache_adapt(self._at, x.data_ptr(), x.stride(0), ids.data_ptr(),
+                                        nbytes, T, base.data_ptr(), base.stride(0),
+                                        out.data_ptr(), out.stride(0), work.data_ptr(), stream),
+                   "expert_cache_adapt")
+        return out
