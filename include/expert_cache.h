@@ -253,7 +253,7 @@ int expert_cache_route(const void* logits, int type, long row_stride, const floa
  * The experts of one layer as expert_cache_moe takes them: S slots (or experts) of
  *   w13  [S, 2*I, H]  gate rows, then up rows
  *   w2   [S, H, I]
- * contiguous and 16-byte aligned. `weights` is `type` itself, or INT8 with a float a row
+ * contiguous and 16-byte aligned, like the scales. `weights` is `type` itself, or INT8 with a float a row
  * (s13 [S, 2*I], s2 [S, H]), or E4M3 with a float for every 128 x 128 block
  * (s13 [S, ceil(2*I/128), ceil(H/128)], s2 [S, ceil(H/128), ceil(I/128)]). `type` is that of
  * the tokens: BF16 or F16.

@@ -178,18 +178,20 @@ def test_experts_numbers_that_are_none_stay_where_they_belong(kind, T):
     assert torch.equal(e(x, probs, ids), clean)
     ids2, probs2 = ids.clone(), probs.clone()
     ids2[0, 0], probs2[0, 0] = 5, 0.0                # weight 0: left out, whatever it holds
-    want = e(x[:1], probs[:1, 1:].contiguous(), ids[:1, 1:].contiguous())
-    assert torch.equal(e(x, probs2, ids2)[:1], want)
+    want, bound = _moe(e, x, probs2, ids2)
+    _close(e(x, probs2, ids2), want, bound)
     ids2[1, 0] = 5
     got = e(x, probs2, ids2)
     assert not torch.isfinite(got[1]).any()
-    assert torch.equal(got[2:], clean[2:])
+    # the other tokens' sums may have another order: the formula's bound holds for any
+    _close(got[2:], want[2:], bound[2:])
     x2 = x.clone()
     x2[2, 7] = float("nan")
     got = e(x2, probs, ids)
     assert torch.isnan(got[2]).all()
     rest = [t for t in range(T) if t != 2]
-    assert torch.equal(got[rest], clean[rest])
+    want, bound = _moe(e, x, probs, ids)
+    _close(got[rest], want[rest], bound[rest])
 
 
 def test_experts_hidden_values_past_float16():

@@ -67,7 +67,8 @@ BAD_LAYER = [dict(S=0), dict(H=0), dict(I=0), dict(H=-8), dict(type=0), dict(typ
 
 @pytest.mark.parametrize("over", BAD_LAYER + [
     dict(w13=None), dict(w2=None), dict(w13=0x10008), dict(w2=0x20004),
-    dict(weights=3), dict(weights=4, s13=16), dict(weights=3, s2=16), dict(x=None),
+    dict(weights=3), dict(weights=4, s13=16), dict(weights=3, s2=16),
+    dict(weights=3, s13=16, s2=20), dict(weights=4, s13=8, s2=16), dict(x=None),
     dict(x=0x30002), dict(xs=36), dict(xs=24), dict(out=None), dict(os=24), dict(probs=None),
     dict(ids=None), dict(id_bytes=2), dict(work=None), dict(work=0x70008),
     dict(out=0x30000), dict(out=0x30000 + 64), dict(out=0x30000 - 100)], ids=str)

@@ -53,19 +53,40 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a
   const unsigned own = (unsigned)ballot(id == slot) & 0xFFFFu;
   if (slot < 0 || __builtin_ctz(own) != which) return;
   const int token = min(t0 + (lane & 15), a.T - 1);
-  const void* const cols[1] = {static_cast<const X*>(a.x) + token * a.x_stride};
-  const float* const none[1] = {nullptr};
-  const int units = (a.H + kUnit - 1) / kUnit;
+  const unsigned short* x = static_cast<const unsigned short*>(a.x) + token * a.x_stride;
+  const int units = (a.H + kUnit - 1) / kUnit, quarter = lane >> 4;
   const int per = (units + a.splits - 1) / a.splits;
   const int first = blockIdx.z * per, last = min(units, first + per);
   for (int r0 = 0; r0 < a.R; r0 += 16) {
-    const X* const rows[1] = {static_cast<const X*>(a.a) +
-                              ((long long)slot * a.R + min(r0 + (lane & 15), a.R - 1)) * a.H};
-    f32x4 acc[1] = {};
-    if (first + wave < last)
-      product<X, X, 1, 1, 2>(rows, cols, none, first + wave, WAVES, min(a.H, last * kUnit), acc);
+    const X* from = static_cast<const X*>(a.a) + ((long long)slot * a.R + r0) * a.H;
+    const unsigned row = row_bytes<X>(r0 + (lane & 15), r0, a.R, a.H);
+    f32x4 acc = {0, 0, 0, 0};
+    constexpr int D = 2;
+    Rows<X> w[D];
+    u32x4 b[D][4];
+    pipeline<D>(
+        (last - first - wave + WAVES - 1) / WAVES,
+        [&](auto d, int i) EC_INLINE {
+          const int u = first + wave + i * WAVES;
+          w[d].load(from, row, nullptr, u, a.H, quarter);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[wave][i][lane] = acc[0][i];
+          for (int f = 0; f < 4; ++f) {
+            const int k = u * kUnit + operand_at<X>(f, quarter);
+            b[d][f] = load16(x + (k < a.H ? k : 0));
+          }
+        },
+        [&](auto d, int i) EC_INLINE {
+          const int u = first + wave + i * WAVES;
+          if ((u + 1) * kUnit > a.H) {
+            w[d].cut(u, a.H, quarter);
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+              b[d][f] = keep(u * kUnit + operand_at<X>(f, quarter) < a.H, b[d][f]);
+          }
+          add_whole<X, X>(w[d], b[d], acc);
+        });
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[wave][i][lane] = acc[i];
     lds_sync();
     for (int j = threadIdx.x; j < 256; j += WAVES * kWave) {
       const int row = r0 + (j & 15), col = j >> 4;

@@ -172,35 +172,88 @@ int launch_route(const RouteArgs& a, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
+// Longest rows of weights: the bytes of 64 of them are counted in 32 bits.
+constexpr int kMaxLength = 1 << 24;
+
 bool experts_bad(const expert_cache_experts* e, int T, int top_k) {
   if (e == nullptr || e->S <= 0 || e->H <= 0 || e->I <= 0) return true;
   if (e->type != EXPERT_CACHE_BF16 && e->type != EXPERT_CACHE_F16) return true;
   const bool byte = e->weights == EXPERT_CACHE_INT8 || e->weights == EXPERT_CACHE_E4M3;
   if (!byte && e->weights != e->type) return true;
   if (e->H % (byte ? 16 : 8) || e->I % (byte ? 16 : 8)) return true;
+  if (e->H > kMaxLength || e->I > kMaxLength) return true;
   if (T < 0 || top_k <= 0 || top_k > kExpertsMaxK) return true;
   return (long long)T * top_k > kExpertsMaxPairs;
 }
 
-template <class X, class W>
-int launch_moe(const ExpertsArgs& a, int T, hipStream_t stream) {
-  const int groups = a.by_slot ? a.S : a.n;
-  hipLaunchKernelGGL((experts_up_k<X, W, 4, 2>), dim3((a.I - 1) / 16 + 1, groups), dim3(256), 0,
-                     stream, a);
+constexpr int kUpWaves = 4, kDownWaves = 8;
+constexpr int kDirectTokens = 64;
+constexpr int kPairTiles = 4;
+
+// How a call of expert_cache_moe is split up, and where things are in its workspace.
+struct MoePlan {
+  bool few, direct;
+  int groups, down_groups, splits;
+  long lo, part, meta, arrived, bytes;
+};
+MoePlan moe_plan(int H, int I, int T, int top_k) {
+  const long n = (long)T * top_k;
+  MoePlan p;
+  p.few = T <= kFewTokens / 2;
+  p.direct = T <= kDirectTokens;
+  p.groups = p.few ? (H <= 16 * 255 ? 1 : 2) : 2 * kPairTiles;
+  p.down_groups = (H - 1) / (8 * p.groups) + 1;
+  p.splits = 1;
+  if (p.few) {  // workgroups that share their rows: as fill the device, a unit a wave at least
+    const int want = 256 / p.down_groups, most = (int)n * ((I - 1) / kUnit + 1) / kDownWaves;
+    p.splits = want < 2 || most < 2 ? 1 : want < most ? want : most;
+  }
+  p.lo = 2 * n * I;
+  p.part = 4 * n * I;
+  p.meta = p.part + (p.few ? 32L * p.down_groups * p.splits * p.groups * kFewTokens : 4 * n * H);
+  p.arrived = p.meta + (p.few ? n * (long)sizeof(ExpertsMeta) : 0);
+  p.bytes = p.arrived + 4L * p.down_groups;
+  return p;
+}
+
+template <class X, class W, bool ONCE>
+int launch_moe_of(const ExpertsArgs& a, int T, int groups, hipStream_t stream) {
+  const int all = a.by_slot ? a.S : a.n;
+  hipLaunchKernelGGL((experts_up_k<X, W, ONCE, kUpWaves, 2>), dim3((a.I - 1) / kTile + 1, all),
+                     dim3(kUpWaves * kWave), 0, stream, a);
   int rc = (int)hipGetLastError();
   if (rc) return rc;
-  hipLaunchKernelGGL((experts_down_k<W, 4, 2>), dim3((a.H - 1) / 16 + 1, groups), dim3(256), 0,
+  const dim3 down(a.down_groups, a.few ? a.splits : all);
+  if (a.few) {
+    if (groups == 1)
+      hipLaunchKernelGGL((experts_down_k<X, W, ONCE, 1, kDownWaves, 3>), down,
+                         dim3(kDownWaves * kWave), 0, stream, a);
+    else
+      hipLaunchKernelGGL((experts_down_k<X, W, ONCE, 2, kDownWaves, 3>), down,
+                         dim3(kDownWaves * kWave), 0, stream, a);
+    return (int)hipGetLastError();
+  }
+  hipLaunchKernelGGL((experts_pairs_k<X, W, ONCE, 4, kPairTiles, 1>), down, dim3(4 * kWave), 0,
                      stream, a);
   rc = (int)hipGetLastError();
-  if (rc) return rc;
+  if (rc || a.direct) return rc;
   hipLaunchKernelGGL((experts_sum_k<X>), dim3((a.H - 1) / 1024 + 1, T), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
+}
+
+// Weights whose rows are whole lines of 128 bytes are read past the caches.
+template <class X, class W>
+int launch_moe(const ExpertsArgs& a, int T, int groups, hipStream_t stream) {
+  const uintptr_t lines = reinterpret_cast<uintptr_t>(a.w13) | reinterpret_cast<uintptr_t>(a.w2) |
+                          (uintptr_t)a.H * sizeof(W) | (uintptr_t)a.I * sizeof(W);
+  return lines % 128 ? launch_moe_of<X, W, false>(a, T, groups, stream)
+                     : launch_moe_of<X, W, true>(a, T, groups, stream);
 }
 
 bool adapters_bad(const expert_cache_adapters* l, int T) {
   if (l == nullptr || l->S <= 0 || l->O <= 0 || l->H <= 0 || l->R <= 0 || T < 0) return true;
   if (l->type != EXPERT_CACHE_BF16 && l->type != EXPERT_CACHE_F16) return true;
-  return l->H % 8 || l->R % 8 || l->R > kAdapterMaxRank;
+  return l->H % 8 || l->R % 8 || l->R > kAdapterMaxRank || l->H > kMaxLength;
 }
 
 // Workgroups that share the hidden length of a tile's product.
@@ -420,7 +473,7 @@ int expert_cache_route(const void* logits, int type, long row_stride, const floa
 
 int expert_cache_moe_workspace(const expert_cache_experts* e, int T, int top_k, long* bytes) {
   if (bytes == nullptr || experts_bad(e, T, top_k)) return -1;
-  *bytes = 4L * T * top_k * (e->I + e->H);
+  *bytes = moe_plan(e->H, e->I, T, top_k).bytes;
   return 0;
 }
 
@@ -430,7 +483,9 @@ int expert_cache_moe(const expert_cache_experts* e, const void* x, long x_stride
   if (experts_bad(e, T, top_k) || (id_bytes != 4 && id_bytes != 8)) return -1;
   if (T == 0) return 0;
   if (e->w13 == nullptr || e->w2 == nullptr || !aligned16(e->w13) || !aligned16(e->w2)) return -1;
-  if (e->weights >= EXPERT_CACHE_INT8 && (e->s13 == nullptr || e->s2 == nullptr)) return -1;
+  if (e->weights >= EXPERT_CACHE_INT8 &&
+      (e->s13 == nullptr || e->s2 == nullptr || !aligned16(e->s13) || !aligned16(e->s2)))
+    return -1;
   if (x == nullptr || !aligned16(x) || (T > 1 && (x_stride % 8 || x_stride < e->H))) return -1;
   if (out == nullptr || (out_stride < e->H && T > 1)) return -1;
   if (topk_weights == nullptr || ids == nullptr) return -1;
@@ -454,19 +509,27 @@ int expert_cache_moe(const expert_cache_experts* e, const void* x, long x_stride
   a.I = e->I;
   a.wide = id_bytes == 8;
   a.by_slot = a.n > a.S;
-  a.hi = static_cast<Bf16*>(workspace);
-  a.lo = a.hi + (long long)a.n * a.I;
-  a.part = reinterpret_cast<float*>(a.lo + (long long)a.n * a.I);
+  const MoePlan plan = moe_plan(e->H, e->I, T, top_k);
+  a.few = plan.few;
+  a.direct = plan.direct;
+  a.down_groups = plan.down_groups;
+  a.splits = plan.splits;
+  char* const at = static_cast<char*>(workspace);
+  a.hi = reinterpret_cast<Bf16*>(at);
+  a.lo = reinterpret_cast<Bf16*>(at + plan.lo);
+  a.part = reinterpret_cast<float*>(at + plan.part);
+  a.meta = reinterpret_cast<ExpertsMeta*>(at + plan.meta);
+  a.arrived = reinterpret_cast<int*>(at + plan.arrived);
   a.out = out;
   a.out_stride = out_stride;
   if (e->type == EXPERT_CACHE_BF16) {
-    if (e->weights == EXPERT_CACHE_INT8) return launch_moe<Bf16, int8_t>(a, T, stream);
-    if (e->weights == EXPERT_CACHE_E4M3) return launch_moe<Bf16, E4m3>(a, T, stream);
-    return launch_moe<Bf16, Bf16>(a, T, stream);
+    if (e->weights == EXPERT_CACHE_INT8) return launch_moe<Bf16, int8_t>(a, T, plan.groups, stream);
+    if (e->weights == EXPERT_CACHE_E4M3) return launch_moe<Bf16, E4m3>(a, T, plan.groups, stream);
+    return launch_moe<Bf16, Bf16>(a, T, plan.groups, stream);
   }
-  if (e->weights == EXPERT_CACHE_INT8) return launch_moe<F16, int8_t>(a, T, stream);
-  if (e->weights == EXPERT_CACHE_E4M3) return launch_moe<F16, E4m3>(a, T, stream);
-  return launch_moe<F16, F16>(a, T, stream);
+  if (e->weights == EXPERT_CACHE_INT8) return launch_moe<F16, int8_t>(a, T, plan.groups, stream);
+  if (e->weights == EXPERT_CACHE_E4M3) return launch_moe<F16, E4m3>(a, T, plan.groups, stream);
+  return launch_moe<F16, F16>(a, T, plan.groups, stream);
 }
 
 int expert_cache_adapt_workspace(const expert_cache_adapters* l, int T, long* bytes) {

@@ -184,14 +184,44 @@ __device__ __forceinline__ u32x4 load16(const void* p) {
   return *static_cast<const u32x4*>(p);
 }
 
-// A routing or slot id, whatever its width; out of [0, n) becomes -1.
+// The same for what is read once: it need not stay in the caches.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load16_of(const void* p) {
+  if constexpr (ONCE)
+    return __builtin_nontemporal_load(static_cast<const u32x4*>(p));
+  else
+    return load16(p);
+}
+
+// What a kernel reads at an address that is the same in all lanes and that nothing writes while
+// it runs: a scalar load, beside the vector loads and not in line with them.
+template <class T>
+__device__ __forceinline__ T load_uniform(const T* p) {
+  using Constant = const __attribute__((address_space(4))) T;
+  return *(Constant*)(reinterpret_cast<uintptr_t>(p));
+}
+
+// A routing or slot id of 4 or 8 bytes; out of [0, n) becomes -1. Both widths take the same two
+// loads, so that nothing waits in a branch.
+struct RawId {
+  unsigned low, high;
+};
+__device__ __forceinline__ RawId raw_id(const void* ids, long long i, bool wide) {
+  const unsigned* p = static_cast<const unsigned*>(ids) + (i << wide);
+  return RawId{p[0], p[wide]};
+}
+__device__ __forceinline__ int id_of(RawId r, bool wide, int n) {
+  const bool in = (r.low < (unsigned)n) & (!wide | (r.high == 0));
+  return in ? (int)r.low : -1;
+}
 __device__ __forceinline__ int load_id(const void* ids, long long i, bool wide, int n) {
-  if (wide) {
-    const long long v = static_cast<const long long*>(ids)[i];
-    return v < 0 || v >= n ? -1 : (int)v;
-  }
-  const int v = static_cast<const int*>(ids)[i];
-  return v < 0 || v >= n ? -1 : v;
+  return id_of(raw_id(ids, i, wide), wide, n);
+}
+
+// Two ids and a weight that were loaded before this point, all under way at once: without it
+// the compiler moves a load to its first use, behind another one's wait.
+__device__ __forceinline__ void together(RawId& a, RawId& b, float& w) {
+  asm volatile("" : "+v"(a.low), "+v"(a.high), "+v"(b.low), "+v"(b.high), "+v"(w));
 }
 
 }  // namespace ec

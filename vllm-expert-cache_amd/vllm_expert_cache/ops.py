@@ -27,51 +27,14 @@ _TOKENS = {torch.bfloat16: 1, torch.float16: 2}
 _LOGITS = {torch.float32: 0, **_TOKENS}
 _BYTES = {torch.int8: 3, torch.float8_e4m3fn: 4}
 _SCORING = {"softmax": 0, "sigmoid": 1}
+_ID_BYTES = {torch.int32: 4, torch.int64: 8}
 _BLOCK = 128  # rows and columns of e4m3 weights that share a scale
 
 MAX_PAIRS = 1024    # tokens x top_k of one Experts call
 MAX_TOP_K = 64
 MAX_EXPERTS = 1024  # of one routing
+MAX_GROUPS = 64
 MAX_RANK = 256
-
-
-def _need(ok, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` as rows that the kernels can load 16 bytes at a time: itself, or a copy."""
-    if t.stride(1) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and
-                                                 (t.stride(0) % 8 or t.stride(0) < t.shape[1])):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _ids(ids: torch.Tensor, device) -> tuple[torch.Tensor, int]:
-    _need(ids.dtype in (torch.int32, torch.int64), f"ids must be int32 or int64, not {ids.dtype}")
-    _need(ids.device == device, f"ids are on {ids.device}, not {device}")
-    return ids.contiguous(), ids.element_size()
-
-
-class _On:
-    """The current stream of `device`, with that device current."""
-
-    __slots__ = ("device", "guard")
-
-    def __init__(self, device):
-        self.device = device
-        self.guard = None
-
-    def __enter__(self) -> int:
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
 
 
 def _check(rc: int, name: str) -> None:
@@ -79,11 +42,43 @@ def _check(rc: int, name: str) -> None:
         raise RuntimeError(f"{name} failed rc={rc}")
 
 
+# The current stream's handle without building a torch.cuda.Stream around it (a microsecond of
+# each call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on_device(device: torch.device, call, *args):
+    """call(*args, stream) on the current stream of `device`, with that device current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        return call(*args, _raw_stream(index))
+    with torch.cuda.device(device):
+        return call(*args, _raw_stream(index))
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` as rows that the kernels can load 16 bytes at a time: itself, or a copy."""
+    n, step = t.shape[0], t.stride()
+    if step[1] != 1 or t.data_ptr() % 16 or (n > 1 and (step[0] % 8 or step[0] < t.shape[1])):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _ids(ids: torch.Tensor, device) -> tuple[torch.Tensor, int]:
+    nbytes = _ID_BYTES.get(ids.dtype)
+    if nbytes is None or ids.device != device:
+        raise ValueError(f"ids must be int32 or int64 on {device}, not {ids.dtype} on {ids.device}")
+    return ids if ids.is_contiguous() else ids.contiguous(), nbytes
+
+
 def _on_gpu(*tensors) -> torch.device:
     device = tensors[0].device
-    _need(device.type == "cuda", f"tensors must be on a GPU, not on {device}")
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a GPU, not on {device}")
     for t in tensors[1:]:
-        _need(t is None or t.device == device, "tensors are on different devices")
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors are on {device} and on {t.device}")
     return device
 
 
@@ -103,36 +98,48 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
 
     Among equals the lowest id comes first. Experts whose logit is NaN or -inf are never
     selected; where too few are left the id is -1 and the weight 0."""
-    _need(logits.dim() == 2, f"logits must be [T, E], not {tuple(logits.shape)}")
-    _need(logits.dtype in _LOGITS, f"logits must be float32, bfloat16 or float16, not {logits.dtype}")
-    _need(scoring in _SCORING, f"scoring must be softmax or sigmoid, not {scoring!r}")
-    _need(id_dtype in (torch.int32, torch.int64), f"ids are int32 or int64, not {id_dtype}")
+    kind = _LOGITS.get(logits.dtype)
+    if kind is None or logits.dim() != 2:
+        raise ValueError(f"logits must be float32, bfloat16 or float16 [T, E], not {logits.dtype} "
+                         f"{list(logits.shape)}")
+    code, nbytes = _SCORING.get(scoring), _ID_BYTES.get(id_dtype)
+    if code is None or nbytes is None:
+        raise ValueError(f"scoring {scoring!r} (softmax or sigmoid), ids of {id_dtype} (int32 or "
+                         f"int64)")
     T, E = logits.shape
-    _need(0 < E <= MAX_EXPERTS, f"{E} experts (1 to {MAX_EXPERTS})")
-    _need(1 <= groups <= 64 and E % groups == 0, f"{groups} groups of {E} experts")
-    _need(1 <= topk_groups <= groups, f"{topk_groups} of {groups} groups")
-    _need(1 <= top_k <= min(MAX_TOP_K, topk_groups * (E // groups)),
-          f"top_k {top_k} of {topk_groups} x {E // groups} experts (at most {MAX_TOP_K})")
-    if bias is not None:
-        _need(bias.dtype == torch.float32 and bias.shape == (E,) and bias.is_contiguous(),
-              f"bias must be contiguous float32 [{E}], not {bias.dtype} {tuple(bias.shape)}")
+    if not 0 < E <= MAX_EXPERTS:
+        raise ValueError(f"{E} experts (1 to {MAX_EXPERTS})")
+    if not 1 <= groups <= MAX_GROUPS or E % groups or not 1 <= topk_groups <= groups:
+        raise ValueError(f"{topk_groups} of {groups} groups of {E} experts (at most {MAX_GROUPS} "
+                         f"equal groups)")
+    if not 1 <= top_k <= min(MAX_TOP_K, topk_groups * (E // groups)):
+        raise ValueError(f"top_k {top_k} of {topk_groups} x {E // groups} experts (at most "
+                         f"{MAX_TOP_K})")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,) or
+                             not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous float32 [{E}], not {bias.dtype} "
+                         f"{list(bias.shape)}")
     device = _on_gpu(logits, bias)
-    if logits.stride(1) != 1 or logits.stride(0) < E:
-        logits = logits.contiguous()
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
-    ids = torch.empty((T, top_k), dtype=id_dtype, device=device)
-    with _On(device) as stream:
-        _check(_lib.lib().expert_cache_route(
-            logits.data_ptr(), _LOGITS[logits.dtype], logits.stride(0),
-            bias.data_ptr() if bias is not None else None, T, E, top_k, _SCORING[scoring],
-            groups, topk_groups, bool(renormalize), scale, weights.data_ptr(), ids.data_ptr(),
-            ids.element_size(), stream), "expert_cache_route")
+    step = logits.stride()
+    if step[1] != 1 or step[0] < E:
+        logits, step = logits.contiguous(), (E, 1)
+    weights = logits.new_empty((T, top_k), dtype=torch.float32)
+    ids = logits.new_empty((T, top_k), dtype=id_dtype)
+    _check(_on_device(device, _lib.lib().expert_cache_route, logits.data_ptr(), kind, step[0],
+                      None if bias is None else bias.data_ptr(), T, E, top_k, code, groups,
+                      topk_groups, 1 if renormalize else 0, scale, weights.data_ptr(),
+                      ids.data_ptr(), nbytes), "expert_cache_route")
     return weights, ids
 
 
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
 def _scales(s, shape, name: str, device):
-    _need(s is not None and s.dtype == torch.float32 and s.is_contiguous(),
-          f"{name} must be contiguous float32")
+    _need(s is not None and s.dtype == torch.float32 and s.is_contiguous() and
+          s.data_ptr() % 16 == 0, f"{name} must be contiguous, 16-byte aligned float32")
     _need(tuple(s.shape) == shape or tuple(s.shape) == shape + (1,),
           f"{name} must be {list(shape)}, not {list(s.shape)}")
     _need(s.device == device, f"{name} is on {s.device}, not {device}")
@@ -193,35 +200,36 @@ class Experts:
         T x top_k is at most 1024. A pair whose id is outside [0, S) or whose weight is 0 adds
         nothing (and an infinity in that expert does not show); a token without any other
         pair gets zeros. `out`, if given, has contiguous rows and does not overlap x."""
-        _need(x.dim() == 2 and x.shape[1] == self.H, f"x must be [T, {self.H}], not {list(x.shape)}")
-        _need(x.dtype in self.dtypes, f"tokens of {x.dtype} do not go with {self.w13.dtype} weights")
-        _need(x.device == self.device, f"x is on {x.device}, not {self.device}")
-        T = x.shape[0]
-        _need(slot_ids.dim() == 2 and slot_ids.shape[0] == T and
-              topk_weights.shape == slot_ids.shape,
-              f"topk_weights {list(topk_weights.shape)} and slot_ids {list(slot_ids.shape)} must "
-              f"be [{T}, top_k]")
-        k = slot_ids.shape[1]
-        _need(1 <= k <= MAX_TOP_K and T * k <= MAX_PAIRS,
-              f"{T} tokens x top_k {k} (top_k at most {MAX_TOP_K}, {MAX_PAIRS} in all)")
-        _need(topk_weights.dtype == torch.float32 and topk_weights.device == self.device,
-              f"topk_weights must be float32 on {self.device}")
+        struct = self._structs.get(x.dtype)
+        if struct is None or x.dim() != 2 or x.shape[1] != self.H or x.device != self.device:
+            raise ValueError(f"x must be [T, {self.H}] on {self.device} of {self.dtypes}, not "
+                             f"{list(x.shape)} on {x.device} of {x.dtype}")
+        T, shape = x.shape[0], slot_ids.shape
+        if len(shape) != 2 or shape[0] != T or topk_weights.shape != shape or \
+                topk_weights.dtype != torch.float32 or topk_weights.device != self.device:
+            raise ValueError(f"slot_ids {list(shape)} and float32 topk_weights must be [{T}, top_k] "
+                             f"on {self.device}, not {topk_weights.dtype} "
+                             f"{list(topk_weights.shape)} on {topk_weights.device}")
+        k = shape[1]
+        if not 1 <= k <= MAX_TOP_K or T * k > MAX_PAIRS:
+            raise ValueError(f"{T} tokens x top_k {k} (top_k at most {MAX_TOP_K}, {MAX_PAIRS} in "
+                             f"all)")
         ids, nbytes = _ids(slot_ids, self.device)
-        topk_weights, x = topk_weights.contiguous(), _rows(x)
+        if not topk_weights.is_contiguous():
+            topk_weights = topk_weights.contiguous()
+        x = _rows(x)
         if out is None:
-            out = torch.empty((T, self.H), dtype=x.dtype, device=self.device)
+            out = x.new_empty((T, self.H))
         else:
             _out(out, x.dtype, (T, self.H), self.device)
-        struct = self._structs[x.dtype][1]
-        h = _lib.lib()
+        h, at = _lib.lib(), struct[1]
         size = self._bytes.get((T, k))
         if size is None:
-            size = self._bytes[T, k] = _workspace(h.expert_cache_moe_workspace, struct, T, k)
-        with _On(self.device) as stream:
-            work = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _check(h.expert_cache_moe(struct, x.data_ptr(), x.stride(0), topk_weights.data_ptr(),
-                                      ids.data_ptr(), nbytes, T, k, out.data_ptr(),
-                                      out.stride(0), work.data_ptr(), stream), "expert_cache_moe")
+            size = self._bytes[T, k] = _workspace(h.expert_cache_moe_workspace, at, T, k)
+        work = x.new_empty(size, dtype=torch.uint8)
+        _check(_on_device(self.device, h.expert_cache_moe, at, x.data_ptr(), x.stride(0),
+                          topk_weights.data_ptr(), ids.data_ptr(), nbytes, T, k, out.data_ptr(),
+                          out.stride(0), work.data_ptr()), "expert_cache_moe")
         return out
 
 
@@ -271,31 +279,30 @@ class Adapters:
         x [T, H], base [T, O]. A token whose id is outside [0, S) has no adapter: its row is
         base's. `out` may be base, whose rows without an adapter are then not written; any
         other `out` does not overlap base or x."""
-        _need(x.dim() == 2 and x.shape[1] == self.H, f"x must be [T, {self.H}], not {list(x.shape)}")
+        dtype, device = self.dtype, self.device
+        if x.dim() != 2 or x.shape[1] != self.H or x.dtype != dtype or x.device != device:
+            raise ValueError(f"x must be {dtype} [T, {self.H}] on {device}, not {x.dtype} "
+                             f"{list(x.shape)} on {x.device}")
         T = x.shape[0]
-        _need(tuple(base.shape) == (T, self.O), f"base must be [{T}, {self.O}], not {list(base.shape)}")
-        _need(x.dtype == self.dtype and base.dtype == self.dtype,
-              f"x and base must be {self.dtype}, not {x.dtype} and {base.dtype}")
-        _need(x.device == self.device and base.device == self.device,
-              f"x and base must be on {self.device}")
-        _need(slot_ids.dim() == 1 and slot_ids.shape[0] == T,
-              f"slot_ids must be [{T}], not {list(slot_ids.shape)}")
-        ids, nbytes = _ids(slot_ids, self.device)
+        if base.shape != (T, self.O) or base.dtype != dtype or base.device != device:
+            raise ValueError(f"base must be {dtype} [{T}, {self.O}] on {device}, not {base.dtype} "
+                             f"{list(base.shape)} on {base.device}")
+        if slot_ids.shape != (T,):
+            raise ValueError(f"slot_ids must be [{T}], not {list(slot_ids.shape)}")
+        ids, nbytes = _ids(slot_ids, device)
         x = _rows(x)
         if out is None:
-            out = torch.empty((T, self.O), dtype=self.dtype, device=self.device)
+            out = x.new_empty((T, self.O))
         else:
-            _out(out, self.dtype, (T, self.O), self.device)
+            _out(out, dtype, (T, self.O), device)
         if base.stride(1) != 1 or (T > 1 and base.stride(0) < self.O):
             base = base.contiguous()
         h = _lib.lib()
         size = self._bytes.get(T)
         if size is None:
             size = self._bytes[T] = _workspace(h.expert_cache_adapt_workspace, self._at, T)
-        with _On(self.device) as stream:
-            work = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _check(h.expert_cache_adapt(self._at, x.data_ptr(), x.stride(0), ids.data_ptr(),
-                                        nbytes, T, base.data_ptr(), base.stride(0),
-                                        out.data_ptr(), out.stride(0), work.data_ptr(), stream),
-                   "expert_cache_adapt")
+        work = x.new_empty(size, dtype=torch.uint8)
+        _check(_on_device(device, h.expert_cache_adapt, self._at, x.data_ptr(), x.stride(0),
+                          ids.data_ptr(), nbytes, T, base.data_ptr(), base.stride(0),
+                          out.data_ptr(), out.stride(0), work.data_ptr()), "expert_cache_adapt")
         return out
