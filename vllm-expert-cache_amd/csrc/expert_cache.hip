@@ -256,22 +256,53 @@ bool adapters_bad(const expert_cache_adapters* l, int T) {
   return l->H % 8 || l->R % 8 || l->R > kAdapterMaxRank || l->H > kMaxLength;
 }
 
-// Workgroups that share the hidden length of a tile's product.
+constexpr int kAdapterWaves = 4;
+#ifndef EC_AT
+#define EC_AT 128
+#define EC_AM 256
+#define EC_SW 8
+#endif
+constexpr int kShrinkManyWaves = EC_SW;
+// Up to this many tokens every adapter of a tile has workgroups of its own.
+constexpr int kAdapterFewTokens = EC_AT;
+
+// Workgroups that share the hidden length of a tile's product: as fill the device, a unit a wave
+// at least.
 int adapter_splits(int T, int H) {
-  const int tiles = (T - 1) / kAdapterTile + 1, most = (H + 4 * kUnit - 1) / (4 * kUnit);
-  const int want = 256 / tiles;
+  const bool few = T <= kAdapterFewTokens;
+  const int tiles = (T - 1) / (few ? kTile : kManyTokens) + 1;
+  const int units = (H - 1) / kUnit + 1, waves = few ? kAdapterWaves : kShrinkManyWaves;
+  const int most = (units - 1) / waves + 1, want = (few ? 512 : EC_AM) / tiles;
   return want < 1 ? 1 : want < most ? want : most;
 }
 
 template <class X>
 int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
-  const int tiles = (a.T - 1) / kAdapterTile + 1;
-  hipLaunchKernelGGL((adapters_shrink_k<X, 4>), dim3(tiles, kAdapterTile, a.splits), dim3(256),
-                     0, stream, a);
+  constexpr int W = kAdapterWaves;
+  const bool few = a.T <= kAdapterFewTokens;
+  const dim3 block(W * kWave);
+  if (few) {
+    const int tiles = (a.T - 1) / kTile + 1;
+    const dim3 shrink(tiles, kTile, a.splits);
+    if (a.R <= 16)
+      hipLaunchKernelGGL((adapters_shrink_k<X, W, 1>), shrink, block, 0, stream, a);
+    else if (a.R <= 32)
+      hipLaunchKernelGGL((adapters_shrink_k<X, W, 2>), shrink, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((adapters_shrink_k<X, W, 4>), shrink, block, 0, stream, a);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+    hipLaunchKernelGGL((adapters_expand_k<X, W, 1, 4>), dim3(tiles, (a.O - 1) / (16 * W) + 1),
+                       block, 0, stream, a);
+    return (int)hipGetLastError();
+  }
+  const int tiles = (a.T - 1) / kManyTokens + 1;
+  hipLaunchKernelGGL((adapters_shrink_many_k<X, kShrinkManyWaves>), dim3(tiles, a.splits),
+                     dim3(kShrinkManyWaves * kWave), 0, stream, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
-  hipLaunchKernelGGL((adapters_expand_k<X, 4>), dim3(tiles, (a.O - 1) / 64 + 1), dim3(256), 0,
-                     stream, a);
+  hipLaunchKernelGGL((adapters_expand_many_k<X, W>), dim3(tiles, (a.O - 1) / (64 * W) + 1), block,
+                     0, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -572,6 +603,8 @@ int expert_cache_adapt(const expert_cache_adapters* l, const void* x, long x_str
   a.R = l->R;
   a.splits = adapter_splits(T, l->H);
   a.wide = id_bytes == 8;
+  a.aligned = aligned16(base) && aligned16(out) &&
+              (T == 1 || (base_stride % 8 == 0 && out_stride % 8 == 0));
   a.v = static_cast<float*>(workspace);
   return l->type == EXPERT_CACHE_BF16 ? launch_adapt<Bf16>(a, stream)
                                       : launch_adapt<F16>(a, stream);
