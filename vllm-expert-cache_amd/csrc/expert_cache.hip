@@ -187,32 +187,39 @@ bool experts_bad(const expert_cache_experts* e, int T, int top_k) {
 }
 
 constexpr int kUpWaves = 4, kDownWaves = 8;
-constexpr int kDirectTokens = 64;
 constexpr int kPairTiles = 4;
+// Above 8 tokens, experts of this many weights in w2 at most take the down projection of few
+// tokens. It reads an expert once for every two of its tokens (from the L2 after the first), which
+// costs more than the other's third launch once the experts are large. Measured on MI355X, us a
+// call, few / not: 16 tokens, top-7 of 30 slots, 480 x 80 fp8 12.8 / 26.9; 9 tokens, top-6 of 186,
+// 448 x 1152 float16 57.4 / 63.3; 14 tokens, top-10 of 24, 6240 x 1920 int8 301 / 221; 16 tokens,
+// top-8 of 128, 7168 x 2048 fp8 472 / 444.
+constexpr long kFewWeights = 1 << 21;
 
 // How a call of expert_cache_moe is split up, and where things are in its workspace.
 struct MoePlan {
-  bool few, direct;
-  int groups, down_groups, splits;
+  bool few;
+  int groups, down_groups, splits, k_waves;
   long lo, part, meta, arrived, bytes;
 };
 MoePlan moe_plan(int H, int I, int T, int top_k) {
   const long n = (long)T * top_k;
   MoePlan p;
-  p.few = T <= kFewTokens / 2;
-  p.direct = T <= kDirectTokens;
-  p.groups = p.few ? (H <= 16 * 255 ? 1 : 2) : 2 * kPairTiles;
+  p.few = T <= 8 || (T <= kFewTokens && (long)H * I <= kFewWeights);
+  const int units = (I - 1) / kUnit + 1;
+  p.k_waves = units >= 4 ? 4 : units >= 2 ? 2 : 1;
+  p.groups = p.few ? (H <= 16 * 255 ? 1 : 2) : 2 * kPairTiles * (4 / p.k_waves);
   p.down_groups = (H - 1) / (8 * p.groups) + 1;
   p.splits = 1;
   if (p.few) {  // workgroups that share their rows: as fill the device, a unit a wave at least
-    const int want = 256 / p.down_groups, most = (int)n * ((I - 1) / kUnit + 1) / kDownWaves;
+    const int want = 256 / p.down_groups, most = (int)n * units / kDownWaves;
     p.splits = want < 2 || most < 2 ? 1 : want < most ? want : most;
   }
   p.lo = 2 * n * I;
   p.part = 4 * n * I;
   p.meta = p.part + (p.few ? 32L * p.down_groups * p.splits * p.groups * kFewTokens : 4 * n * H);
   p.arrived = p.meta + (p.few ? n * (long)sizeof(ExpertsMeta) : 0);
-  p.bytes = p.arrived + 4L * p.down_groups;
+  p.bytes = p.arrived + (p.few ? 4L * p.down_groups : 0);
   return p;
 }
 
@@ -233,10 +240,10 @@ int launch_moe_of(const ExpertsArgs& a, int T, int groups, hipStream_t stream) {
                          dim3(kDownWaves * kWave), 0, stream, a);
     return (int)hipGetLastError();
   }
-  hipLaunchKernelGGL((experts_pairs_k<X, W, ONCE, 4, kPairTiles, 1>), down, dim3(4 * kWave), 0,
+  hipLaunchKernelGGL((experts_pairs_k<W, ONCE, 4, kPairTiles, 1>), down, dim3(4 * kWave), 0,
                      stream, a);
   rc = (int)hipGetLastError();
-  if (rc || a.direct) return rc;
+  if (rc) return rc;
   hipLaunchKernelGGL((experts_sum_k<X>), dim3((a.H - 1) / 1024 + 1, T), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
@@ -542,9 +549,9 @@ int expert_cache_moe(const expert_cache_experts* e, const void* x, long x_stride
   a.by_slot = a.n > a.S;
   const MoePlan plan = moe_plan(e->H, e->I, T, top_k);
   a.few = plan.few;
-  a.direct = plan.direct;
   a.down_groups = plan.down_groups;
   a.splits = plan.splits;
+  a.k_waves = plan.k_waves;
   char* const at = static_cast<char*>(workspace);
   a.hi = reinterpret_cast<Bf16*>(at);
   a.lo = reinterpret_cast<Bf16*>(at + plan.lo);

@@ -46,13 +46,13 @@ struct ExpertsArgs {
   int n, k, S, H, I;
   bool wide, by_slot;
   bool few;     // experts_down_k makes the down projection
-  bool direct;  // the down projection adds up as well (not experts_sum_k)
   Bf16* hi;  // [n][I] hidden values times routing weight, as two bfloat16
   Bf16* lo;
   float* part;        // [n][H]; few: [tiles of H][splits][16][16], where splits > 1
   ExpertsMeta* meta;  // few: [n or S]
-  int* arrived;       // direct: [down_groups] workgroups that have left their part
+  int* arrived;       // few: [down_groups] workgroups that have left their part
   int down_groups, splits;
+  int k_waves;  // not few: waves that share a row's length
   void* out;
   long long out_stride;  // elements
 };
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_up_k(ExpertsArgs a) {
   } red;
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (a.direct && blockIdx.y == 0)
+  if (a.few && blockIdx.y == 0)
     for (int i = blockIdx.x * WAVES * kWave + threadIdx.x; i < a.down_groups;
          i += gridDim.x * WAVES * kWave)
       a.arrived[i] = 0;
@@ -556,7 +556,6 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_down_k(ExpertsArgs a) {
     }
     live += __builtin_amdgcn_readlane(upto, 63);
   }
-#pragma unroll
   for (int i = lane; i < kFewTokens * kRows; i += kWave) sums[wave][i / kRows][i % kRows] = 0.f;
   lds_sync();
 
@@ -648,28 +647,26 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_down_k(ExpertsArgs a) {
   if (one) static_cast<X*>(a.out)[t * a.out_stride + r] = from_f32<X>(y);
 }
 
-// More tokens: 16 * TILES rows of one expert for its pairs, the tiles of a wave sharing what it
-// loads of the columns. The last workgroup of the rows adds up every token's pairs in order.
-template <class X, class W, bool ONCE, int WAVES, int TILES, int D>
+// More tokens: down projection of one expert for its pairs, 16 * TILES rows a wave, which share
+// what it loads of the columns. a.k_waves of the waves split the length of the same rows.
+template <class W, bool ONCE, int WAVES, int TILES, int D>
 __global__ __launch_bounds__(WAVES* kWave, sizeof(W) == 1 ? 3 : 2) void experts_pairs_k(ExpertsArgs a) {
-  constexpr int kThreads = WAVES * kWave, kRows = TILES * kTile;
+  constexpr int kThreads = WAVES * kWave, kRows = TILES * kTile;  // rows of a wave
+  __shared__ Pairs list;
   __shared__ __attribute__((aligned(16))) union {
-    struct {
-      Pairs list;
-      union {
-        float packed[WAVES][2][kRows];  // token, row
-        float whole[WAVES][TILES][4][kWave];
-      } red;
-    } s;
-    unsigned char used[kExpertsMaxPairs];
-  } lds;
-  __shared__ int last;
+    float packed[WAVES][2][kRows];  // token, row
+    float whole[WAVES][TILES][4][kWave];
+  } red;
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int slot;
-  const int count = list_pairs(a, blockIdx.y, slot, lds.s.list);
-  const int row0 = blockIdx.x * kRows;
-  const int units = (a.I + kUnit - 1) / kUnit, mine = (units - wave + WAVES - 1) / WAVES;
+  const int count = list_pairs(a, blockIdx.y, slot, list);
+  const int k_wave = wave % a.k_waves, group = wave / a.k_waves;
+  const int all_rows = WAVES / a.k_waves * kRows;
+  const int first_row = blockIdx.x * all_rows;
+  const int row0 = min(first_row + group * kRows, (a.H - 1) / kRows * kRows);
+  const int units = (a.I + kUnit - 1) / kUnit;
+  const int mine = (units - k_wave + a.k_waves - 1) / a.k_waves;
   lds_sync();
   if (count > 0) {
     const W* base = static_cast<const W*>(a.w2) + ((long long)slot * a.H + row0) * a.I;
@@ -680,12 +677,12 @@ __global__ __launch_bounds__(WAVES* kWave, sizeof(W) == 1 ? 3 : 2) void experts_
       scale = a.s2 + ((long long)slot * rb + row0 / kUnit) * units;
     }
     const int start = first_unit(blockIdx.y * gridDim.x + blockIdx.x, units);
-    const auto unit = [&](int i) EC_INLINE { return wrap(wave + i * WAVES + start, units); };
+    const auto unit = [&](int i) EC_INLINE { return wrap(k_wave + i * a.k_waves + start, units); };
     const bool packed = count <= 2;
     for (int c0 = 0; c0 < count; c0 += kTile) {
       if (packed) {
         const Bf16* cols = (column & 4 ? a.lo : a.hi) +
-                           (long long)lds.s.list.pair[min(column >> 3, count - 1)] * a.I;
+                           (long long)list.pair[min(column >> 3, count - 1)] * a.I;
         unsigned rows[TILES][2];
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
@@ -718,7 +715,7 @@ __global__ __launch_bounds__(WAVES* kWave, sizeof(W) == 1 ? 3 : 2) void experts_
             const f32x4 v = acc[t].template total<8>(g);
             if ((column & 7) == 0 && quarter < 2)
               *reinterpret_cast<f32x4*>(
-                  &lds.s.red.packed[wave][column >> 3][t * kTile + g * 8 + quarter * 4]) = v;
+                  &red.packed[wave][column >> 3][t * kTile + g * 8 + quarter * 4]) = v;
           }
         });
       } else {
@@ -728,7 +725,7 @@ __global__ __launch_bounds__(WAVES* kWave, sizeof(W) == 1 ? 3 : 2) void experts_
         for (int t = 0; t < TILES; ++t)
           rows[t] = row_bytes<W>(row0 + t * kTile + column, row0, a.H, a.I);
         Rows<W> w[1][TILES];
-        const long long at = (long long)lds.s.list.pair[min(c0 + column, count - 1)] * a.I;
+        const long long at = (long long)list.pair[min(c0 + column, count - 1)] * a.I;
         u32x4 b[1][8];
         each<TILES>([&](auto t) EC_INLINE { v[t] = f32x4{0, 0, 0, 0}; });
         pipeline<1>(
@@ -757,46 +754,25 @@ __global__ __launch_bounds__(WAVES* kWave, sizeof(W) == 1 ? 3 : 2) void experts_
             });
         each<TILES>([&](auto t) EC_INLINE {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) lds.s.red.whole[wave][t][i][lane] = v[t][i];
+          for (int i = 0; i < 4; ++i) red.whole[wave][t][i][lane] = v[t][i];
         });
       }
       lds_sync();
       const int here = min(count - c0, kTile);
-      for (int j = threadIdx.x; j < kRows * here; j += kThreads) {
-        const int r = j % kRows, col = j / kRows, row = row0 + r;
+      for (int j = threadIdx.x; j < all_rows * here; j += kThreads) {
+        const int r = j % all_rows, col = j / all_rows, row = first_row + r;
         if (row >= a.H) continue;
+        const int wave0 = r / kRows * a.k_waves, tile = r % kRows / kTile;
         const int from = r % kTile / 4 * 16 + col;
         float y = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w)
-          y += packed ? lds.s.red.packed[w][col & 1][r] : lds.s.red.whole[w][r / kTile][r & 3][from];
+        for (int w = wave0; w < wave0 + a.k_waves; ++w)
+          y += packed ? red.packed[w][col & 1][r % kRows]
+                      : red.whole[w][tile][r & 3][from];
         if constexpr (__is_same(W, int8_t)) y *= a.s2[(long long)slot * a.H + row];
-        store_part(a.part + (long long)lds.s.list.pair[c0 + col] * a.H + row, y);
+        a.part[(long long)list.pair[c0 + col] * a.H + row] = y;
       }
       lds_sync();
     }
-  }
-  if (!a.direct || !arrive(a.arrived + blockIdx.x, gridDim.y, &last)) return;
-  // which pairs have a part: as list_pairs lists them
-  for (int j = threadIdx.x; j < a.n; j += kThreads) {
-    const int id = load_id(a.ids, j, a.wide, a.S);
-    bool used = id >= 0 && a.probs[j] != 0.f;
-    for (int i = j / a.k * a.k; i < j; ++i)
-      used = used && !(load_id(a.ids, i, a.wide, a.S) == id && a.probs[i] != 0.f);
-    lds.used[j] = used;
-  }
-  lds_sync();
-  const int tokens = a.n / a.k;
-  for (int j = threadIdx.x; j < kRows * tokens; j += kThreads) {
-    const int row = row0 + j % kRows, t = j / kRows;
-    if (row >= a.H) continue;
-    float y = 0;
-#pragma unroll 8
-    for (int i = t * a.k; i < (t + 1) * a.k; ++i) {
-      const float v = load_part(a.part + (long long)i * a.H + row);
-      y += lds.used[i] ? v : 0.f;
-    }
-    static_cast<X*>(a.out)[t * a.out_stride + row] = from_f32<X>(y);
   }
 }
 
