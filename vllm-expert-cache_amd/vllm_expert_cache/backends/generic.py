@@ -24,6 +24,9 @@ Arming is a plan that either completes or stops with a reason (`_Declined`):
 
 A served step applies one `_Patch` (slot tensors, slot config, slot count) around the stock
 `apply` and undoes it in reverse order, also when `apply` raises.
+
+With EXPERT_CACHE_MOE=1 a served step of a layer whose weights ops.Experts takes (`_experts`) is
+refresh and that operator over the slots, without the stock `apply`.
 """
 from __future__ import annotations
 
@@ -35,6 +38,7 @@ import torch
 
 from ..cache import ExpertSlotCache
 from ..config import settings
+from ..ops import MAX_PAIRS, MAX_TOP_K, Experts
 
 # The two expert weight matrices, in the spellings vLLM schemes register: the plain one,
 # and the packed compressed-tensors one (wNa16 int4, w4a4 nvfp4 / mxfp4).
@@ -182,6 +186,31 @@ def _bindings(layer, mirrors: list[_Mirror], slots: dict) -> dict:
     return bound
 
 
+def _experts(layer, cache: ExpertSlotCache, slot_cfg) -> Experts:
+    """The layer's experts over its slots, computed as `apply` computes them but without
+    quantising activations. ValueError says why ops.Experts cannot stand in for it."""
+    w13, w2 = _WEIGHT_PAIRS[0]
+    if not (w13 in cache.bound and w2 in cache.bound):
+        raise ValueError("packed expert weights")
+    weights = [cache.bound[name].data for name in (w13, w2)]
+    if any(getattr(getattr(layer, name), "is_shuffled", False) for name in (w13, w2)):
+        raise ValueError("expert weights in another kernel's layout")
+    activation = getattr(layer, "activation", "silu")
+    activation = getattr(activation, "value", activation)
+    if activation != "silu":
+        raise ValueError(f"activation {activation!r}")
+    if getattr(layer, "apply_router_weight_on_input", False):
+        raise ValueError("routing weights applied to the input")
+    scales = []
+    for dname in ("_w1", "_w2"):
+        desc = getattr(slot_cfg, dname, None)
+        for fname in _DESC_TENSORS[1:]:
+            if getattr(desc, fname, None) is not None:
+                raise ValueError(f"{dname}.{fname} in the quant config")
+        scales.append(getattr(desc, "scale", None))
+    return Experts(*weights, *scales)
+
+
 def _plan(layer, method, logger):
     """Steps 1-4 of arming. Returns (cache, config built against the slots)."""
     w13, w2 = _weight_pair(layer)
@@ -226,7 +255,16 @@ def _plan(layer, method, logger):
     return cache, slot_cfg
 
 
-def _serve_from_slots(layer, method, cache: ExpertSlotCache, slot_cfg) -> None:
+def _takes(experts: Experts | None, x, topk_weights, topk_ids, shared_experts) -> bool:
+    """Whether a served step's arguments are ones that `experts` computes."""
+    return (experts is not None and shared_experts is None and x.dim() == 2
+            and x.dtype in experts.dtypes and topk_weights.dtype == torch.float32
+            and topk_ids.dim() == 2 and topk_ids.dtype in (torch.int32, torch.int64)
+            and topk_ids.shape[1] <= MAX_TOP_K and topk_ids.numel() <= MAX_PAIRS)
+
+
+def _serve_from_slots(layer, method, cache: ExpertSlotCache, slot_cfg,
+                      experts: Experts | None = None) -> None:
     """Step 5: wrap this method instance's apply."""
     stock_apply = method.apply
 
@@ -240,6 +278,8 @@ def _serve_from_slots(layer, method, cache: ExpertSlotCache, slot_cfg) -> None:
             return stock_apply(layer, x, topk_weights, topk_ids, shared_experts,
                                shared_experts_input)
         slot_ids = cache.refresh(topk_ids)
+        if _takes(experts, x, topk_weights, topk_ids, shared_experts):
+            return experts(x, topk_weights, slot_ids)
         patch = _Patch()
         try:
             patch.set(method.moe_kernel.fused_experts, "quant_config", slot_cfg)
@@ -264,7 +304,14 @@ def arm(layer, method, logger) -> bool:
             logger.warning("expert-cache: not caching %s -- %s", type(method).__name__,
                            d.reason)
         return False
-    _serve_from_slots(layer, method, cache, slot_cfg)
+    experts = None
+    if settings.moe:
+        try:
+            experts = _experts(layer, cache, slot_cfg)
+        except ValueError as e:
+            logger.warning("expert-cache: %s computes its own served steps -- %s",
+                           type(method).__name__, e)
+    _serve_from_slots(layer, method, cache, slot_cfg, experts)
     return True
 
 

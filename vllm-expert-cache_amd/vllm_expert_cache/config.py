@@ -12,6 +12,8 @@ deployment configured for it behaves the same here:
 EXPERT_CACHE_CHUNKS / EXPERT_CACHE_LANES (gather grid) are read by cache.py and
 EXPERT_CACHE_LIB (library path) by _lib.py, as in the reference. EXPERT_CACHE_PREFETCH_CHUNKS
 (workgroups of a prefetch copy, default 16) is this package's own, read by cache.py.
+EXPERT_CACHE_MOE is this package's own as well: "1" has armed layers compute their served steps
+with ops.Experts where it takes the layer's weights, instead of vLLM's kernel.
 """
 from __future__ import annotations
 
@@ -24,6 +26,10 @@ class _Settings:
     @property
     def disabled(self) -> bool:
         return os.environ.get("EXPERT_CACHE_DISABLE", "0") == "1"
+
+    @property
+    def moe(self) -> bool:
+        return os.environ.get("EXPERT_CACHE_MOE", "0") == "1"
 
     @property
     def slots(self) -> int | None:
