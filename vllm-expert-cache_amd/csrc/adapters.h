@@ -216,105 +216,135 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
 constexpr int kManyTokens = 64;  // of a workgroup of the kernels below: a lane each
 constexpr int kManyTiles = kManyTokens / kTile;
 
-// A's product for 64 tokens over one split of the hidden length, 64 ranks at a time.
-template <class X, int WAVES>
-__global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_many_k(AdaptersArgs a) {
-  constexpr int T = kManyTiles, N = 4, kRows = N * kTile;
-  __shared__ float red[WAVES][N][4][kWave];
+// A's product for 64 tokens over one split of the hidden length, 32 * ROWS ranks at a time. A unit
+// of the tokens and of A goes through LDS: from the L1 each wave would take the rows it shares
+// with the others for itself, and what a compute unit gets from its L1 (56 bytes/ns) is the
+// bound then. A wave has 32 of the ranks, 32 of the tokens and a part of each unit.
+template <class X, int ROWS>
+__global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersArgs a) {
+  constexpr int kRows = 32 * ROWS, kParts = 4 / ROWS, D = 4;
+  constexpr int kPitch = 2 * kUnit + 16;  // bytes of a row: 16 rows start in different banks
+  constexpr int kLine = 2 * kUnit / 16;   // lanes that read a row's unit
+  constexpr int kEach = 8 * kWave / kLine;  // rows that the workgroup reads at once
+  __shared__ __attribute__((aligned(16))) union {
+    char unit[2][kRows + kManyTokens][kPitch];
+    f32x4 parts[kParts - 1][2 * ROWS][2][2][kWave];
+  } lds;
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int half = wave & 1, group = wave / 2 % ROWS, part = wave / (2 * ROWS);
   const int t0 = blockIdx.x * kManyTokens;
   int id = load_id(a.ids, min(t0 + lane, a.T - 1), a.wide, a.S);
   if (t0 + lane >= a.T) id = -1;
-  const int units = (a.H + kUnit - 1) / kUnit, per = (units + a.splits - 1) / a.splits;
-  const int first = blockIdx.y * per, count = min(units - first, per);
+  // a split has every a.splits-th unit, and each workgroup starts at another of them
+  const int units = (a.H + kUnit - 1) / kUnit;
+  const int count = (units - (int)blockIdx.y + a.splits - 1) / a.splits;
+  const int start = first_unit(blockIdx.x, count);
+  const int my_row = threadIdx.x / kLine, my_k = threadIdx.x % kLine * 8;
   for (unsigned long long left = ballot(id >= 0); left;) {
     const int slot = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
     const unsigned long long own = ballot(id == slot);
     left &= ~own;
-    // columns of other adapters read what this one's first token has
-    const unsigned short* x[T];
+    const bool any = (unsigned)(own >> half * 32) != 0;
+    // tokens of other adapters read what this one's first token has
+    const unsigned short* x[2];
 #pragma unroll
-    for (int c = 0; c < T; ++c) {
-      const int t = c * kTile + column;
-      x[c] = static_cast<const unsigned short*>(a.x) +
+    for (int j = 0; j < 2; ++j) {
+      const int t = my_row + j * kEach;
+      x[j] = static_cast<const unsigned short*>(a.x) +
              (t0 + (own >> t & 1 ? t : __builtin_ctzll(own))) * a.x_stride;
     }
-    const auto has = [&](int c) EC_INLINE { return (own >> c * kTile & 0xFFFF) != 0; };
     for (int r0 = 0; r0 < a.R; r0 += kRows) {
-      const X* from = static_cast<const X*>(a.a) + ((long long)slot * a.R + r0) * a.H;
-      unsigned rows[N];
+      const char* from = static_cast<const char*>(a.a) + ((long long)slot * a.R + r0) * (2LL * a.H);
+      unsigned rows[ROWS];
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        rows[n] = row_bytes<X>(r0 + n * kTile + column, r0, a.R, a.H);
-      f32x4 acc[T][N];
-#pragma unroll
-      for (int c = 0; c < T; ++c)
-#pragma unroll
-        for (int n = 0; n < N; ++n) acc[c][n] = f32x4{0, 0, 0, 0};
-      for (int i = wave; i < count; i += WAVES) {
-        const int u = first + i;
-        Rows<X> w[N];
-        u32x4 b[T][4];
-        each<N>([&](auto n) EC_INLINE { w[n].load(from, rows[n], nullptr, u, a.H, quarter); });
-        each<T>([&](auto c) EC_INLINE {
-          if (has(c)) {
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              const int k = u * kUnit + operand_at<X>(f, quarter);
-              b[c][f] = load16(x[c] + (k < a.H ? k : 0));
-            }
-          }
-        });
-        if ((u + 1) * kUnit > a.H) {
-          each<N>([&](auto n) EC_INLINE { w[n].cut(u, a.H, quarter); });
-          each<T>([&](auto c) EC_INLINE {
-#pragma unroll
-            for (int f = 0; f < 4; ++f)
-              b[c][f] = keep(u * kUnit + operand_at<X>(f, quarter) < a.H, b[c][f]);
+      for (int j = 0; j < ROWS; ++j) rows[j] = row_bytes<X>(r0 + my_row + j * kEach, r0, a.R, a.H);
+      f32x4 acc[2][2];
+      each<2>([&](auto r) EC_INLINE {
+        each<2>([&](auto c) EC_INLINE { acc[r][c] = f32x4{0, 0, 0, 0}; });
+      });
+      u32x4 w[D][ROWS], b[D][2];
+      const auto unit = [&](int i) EC_INLINE {
+        return (int)blockIdx.y + a.splits * wrap(i + start, count);
+      };
+      lds_sync();  // the parts of the ranks before have been read
+      pipeline<D>(
+          count,
+          [&](auto d, int i) EC_INLINE {
+            const int k = unit(i) * kUnit + my_k;
+            const unsigned at = k < a.H ? 2u * k : 0u;
+            each<ROWS>([&](auto j) EC_INLINE { w[d][j] = load16(from + (rows[j] + at)); });
+            each<2>([&](auto j) EC_INLINE { b[d][j] = load16(x[j] + at / 2); });
+          },
+          [&](auto d, int i) EC_INLINE {
+            char(*to)[kPitch] = lds.unit[i & 1];
+            const bool in = unit(i) * kUnit + my_k < a.H;
+            each<ROWS>([&](auto j) EC_INLINE {
+              *reinterpret_cast<u32x4*>(&to[my_row + j * kEach][2 * my_k]) = keep(in, w[d][j]);
+            });
+            each<2>([&](auto j) EC_INLINE {
+              *reinterpret_cast<u32x4*>(&to[kRows + my_row + j * kEach][2 * my_k]) =
+                  keep(in, b[d][j]);
+            });
+            lds_sync();  // two units in turn: the other is free once all have come here
+            if (!any) return;
+            each<ROWS>([&](auto s) EC_INLINE {  // 32 values of k at a time, of the unit's four
+              const int k = (part * ROWS + s) * 64 + quarter * 16;
+              u32x4 rw[2], cl[2];
+              each<2>([&](auto n) EC_INLINE {
+                rw[n] = load16(&to[group * 32 + n * 16 + column][k]);
+                cl[n] = load16(&to[kRows + half * 32 + n * 16 + column][k]);
+              });
+              each<2>([&](auto r) EC_INLINE {
+                each<2>([&](auto c) EC_INLINE {
+                  acc[r][c] = Frag<X>::mfma(rw[r], cl[c], acc[r][c]);
+                });
+              });
+            });
           });
-        }
-        each<T>([&](auto c) EC_INLINE {
-          if (has(c))
-            each<N>([&](auto n) EC_INLINE { add_whole<X, X>(w[n], b[c], acc[c][n]); });
+      lds_sync();
+      if (part) {
+        each<2>([&](auto r) EC_INLINE {
+          each<2>([&](auto c) EC_INLINE {
+            lds.parts[part - 1][wave % (2 * ROWS)][r][c][lane] = acc[r][c];
+          });
         });
       }
-      each<T>([&](auto c) EC_INLINE {
-        if (!has(c)) return;
-        lds_sync();
-        each<N>([&](auto n) EC_INLINE {
+      lds_sync();
+      if (!part) {
+        each<2>([&](auto r) EC_INLINE {
+          each<2>([&](auto c) EC_INLINE {
+            const int t = half * 32 + c * 16 + column;
+            const int row = r0 + group * 32 + r * 16 + quarter * 4;
+            f32x4 y = acc[r][c];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) red[wave][n][i][lane] = acc[c][n][i];
+            for (int p = 0; p < kParts - 1; ++p) y += lds.parts[p][wave][r][c][lane];
+            if (own >> t & 1 && row < a.R)
+              *reinterpret_cast<f32x4*>(
+                  a.v + ((long long)blockIdx.y * a.T + t0 + t) * a.R + row) = y;
+          });
         });
-        lds_sync();
-        for (int j = threadIdx.x; j < kRows * kTile; j += WAVES * kWave) {
-          const int r = j % kRows, t = c * kTile + j / kRows;
-          if (r0 + r < a.R && own >> t & 1) {
-            float y = 0;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w)
-              y += red[w][r / kTile][r & 3][r % kTile / 4 * 16 + j / kRows];
-            a.v[((long long)blockIdx.y * a.T + t0 + t) * a.R + r0 + r] = y;
-          }
-        }
-      });
+      }
     }
   }
 }
 
-// B's product and the sum with the base for 64 tokens, 64 outputs a wave: the tokens' low-rank
-// values are joined, scaled and split into two bfloat16 once for the workgroup, in LDS.
+// B's product and the sum with the base for 64 tokens: the tokens' low-rank values are joined,
+// scaled and split into two bfloat16 once for the workgroup, in LDS. A wave has 64 outputs; the
+// rows of its instructions are interleaved so that a lane ends with two runs of eight neighbouring
+// outputs and the wave reads and writes 64 bytes of a token at a time.
 template <class X, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersArgs a) {
-  constexpr int T = kManyTiles, N = 4, kRun = 4 * N, kRanks = 64;
+  constexpr int T = kManyTiles, N = 4, kRanks = 64;
   __shared__ __attribute__((aligned(16))) Bf16 low[2][kManyTokens][kRanks + 8];
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int t0 = blockIdx.x * kManyTokens;
-  const int row0 = (blockIdx.y * WAVES + wave) * (16 * N);
+  const int t0 = blockIdx.y * kManyTokens;
+  const int row0 = (blockIdx.x * WAVES + wave) * (16 * N);
   const bool some = row0 < a.O;
-  const int o0 = row0 + quarter * kRun;
+  const int o0 = row0 + quarter * 8;  // eight outputs from here, and eight from 32 after it
   const bool fast = a.aligned && row0 + 16 * N <= a.O;
+  int id = load_id(a.ids, min(t0 + lane, a.T - 1), a.wide, a.S);
   u32x4 in[T][2];
 #pragma unroll
   for (int c = 0; c < T; ++c) {
@@ -323,19 +353,20 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersA
         static_cast<const unsigned short*>(a.base) + token * a.base_stride + o0;
     if (fast) {
       in[c][0] = load16(base);
-      in[c][1] = load16(base + 8);
+      in[c][1] = load16(base + 32);
     } else {
 #pragma unroll
-      for (int i = 0; i < kRun / 2; ++i) {
-        const unsigned lo = o0 + 2 * i < a.O ? base[2 * i] : 0;
-        const unsigned hi = o0 + 2 * i + 1 < a.O ? base[2 * i + 1] : 0;
+      for (int i = 0; i < 8; ++i) {
+        const int at = i / 4 * 32 + i % 4 * 2;
+        const unsigned lo = o0 + at < a.O ? base[at] : 0;
+        const unsigned hi = o0 + at + 1 < a.O ? base[at + 1] : 0;
         in[c][i / 4][i % 4] = lo | hi << 16;
       }
     }
   }
-  int id = load_id(a.ids, min(t0 + lane, a.T - 1), a.wide, a.S);
   if (t0 + lane >= a.T) id = -1;
   const unsigned long long with = ballot(id >= 0);
+  const float scale = id < 0 ? 0.f : a.scales ? a.scales[id] : 1.f;
   f32x4 total[T][N];
 #pragma unroll
   for (int c = 0; c < T; ++c)
@@ -344,38 +375,54 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersA
   unsigned rows[N];
 #pragma unroll
   for (int n = 0; n < N; ++n)
-    rows[n] = row_bytes<X>(min(row0, a.O - 1) + (column >> 2) * kRun + n * 4 + (column & 3),
+    rows[n] = row_bytes<X>(min(row0, a.O - 1) + n / 2 * 32 + (column >> 2) * 8 + n % 2 * 4 + (column & 3),
                            min(row0, a.O - 1), a.O, a.R);
+  u32x4 w[2][N];
+  // 64 ranks of an adapter's rows
+  const auto load_rows = [&](int slot, int r0) EC_INLINE {
+    const char* from = static_cast<const char*>(a.b) +
+                       ((long long)slot * a.O + min(row0, a.O - 1)) * (2LL * a.R);
+    each<2>([&](auto h) EC_INLINE {
+      const int k = r0 + h * 32 + quarter * 8;
+      each<N>([&](auto n) EC_INLINE {
+        w[h][n] = load16(from + (rows[n] + (k < a.R ? k : 0) * 2u));
+      });
+    });
+  };
   for (int r0 = 0; with && r0 < a.R; r0 += kRanks) {
+    // the first adapter's rows come while the tokens' values are joined
+    load_rows(__builtin_amdgcn_readlane(id, __builtin_ctzll(with)), r0);
     lds_sync();
-    for (int j = threadIdx.x; j < kManyTokens * (kRanks / 4); j += WAVES * kWave) {
-      const int t = j / (kRanks / 4), r = j % (kRanks / 4) * 4;
-      const int slot = __shfl(id, t);
-      f32x4 v = {0, 0, 0, 0};
-      if (slot >= 0 && r0 + r < a.R) {
-        const float* from = a.v + (long long)(t0 + t) * a.R + r0 + r;
-#pragma unroll 4
-        for (int s = 0; s < a.splits; ++s)
-          v += *reinterpret_cast<const f32x4*>(from + (long long)s * a.T * a.R);
-        v *= a.scales ? a.scales[slot] : 1.f;
-      }
+    constexpr int kEach = kManyTokens * (kRanks / 4) / (WAVES * kWave);
+    const int t = threadIdx.x / (kRanks / 4), r = threadIdx.x % (kRanks / 4) * 4;
+    constexpr int kStep = kManyTokens / kEach;  // tokens between a thread's values
+    f32x4 v[kEach];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split_f32(v[i], low[0][t][r + i], low[1][t][r + i]);
+    for (int j = 0; j < kEach; ++j) v[j] = f32x4{0, 0, 0, 0};
+#pragma unroll 2
+    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        v[j] += *reinterpret_cast<const f32x4*>(
+            a.v + ((long long)s * a.T + min(t0 + t + j * kStep, a.T - 1)) * a.R +
+            min(r0 + r, a.R - 4));
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int at = t + j * kStep;
+      v[j] *= __shfl(scale, at);
+      const bool live = r0 + r < a.R && (with >> at & 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        split_f32(live ? v[j][i] : 0.f, low[0][at][r + i], low[1][at][r + i]);
     }
     lds_sync();
+    bool loaded = true;
     for (unsigned long long left = some ? with : 0; left;) {
       const int slot = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
       const unsigned long long own = ballot(id == slot);
       left &= ~own;
-      const char* from =
-          static_cast<const char*>(a.b) + ((long long)slot * a.O + row0) * (2LL * a.R);
-      u32x4 w[2][N];
-      each<2>([&](auto h) EC_INLINE {
-        const int k = r0 + h * 32 + quarter * 8;
-        each<N>([&](auto n) EC_INLINE {
-          w[h][n] = load16(from + (rows[n] + (k < a.R ? k : 0) * 2u));
-        });
-      });
+      if (!loaded) load_rows(slot, r0);
+      loaded = false;
       if (r0 + kRanks > a.R) {
         each<2>([&](auto h) EC_INLINE {
           const bool live = r0 + h * 32 + quarter * 8 < a.R;
@@ -407,7 +454,7 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersA
     unsigned short* out = static_cast<unsigned short*>(a.out) + (t0 + t) * a.out_stride + o0;
     if (adapted) {
 #pragma unroll
-      for (int i = 0; i < kRun / 2; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const unsigned v = in[c][i / 4][i % 4];
         const X lo{(unsigned short)v}, hi{(unsigned short)(v >> 16)};
         in[c][i / 4][i % 4] =
@@ -417,11 +464,13 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersA
     }
     if (fast) {
       *reinterpret_cast<u32x4*>(out) = in[c][0];
-      *reinterpret_cast<u32x4*>(out + 8) = in[c][1];
+      *reinterpret_cast<u32x4*>(out + 32) = in[c][1];
     } else {
 #pragma unroll
-      for (int i = 0; i < kRun; ++i)
-        if (o0 + i < a.O) out[i] = (unsigned short)(in[c][i / 8][i / 2 % 4] >> (i & 1) * 16);
+      for (int i = 0; i < 16; ++i) {
+        const int at = i / 8 * 32 + i % 8;
+        if (o0 + at < a.O) out[at] = (unsigned short)(in[c][i / 8][i / 2 % 4] >> (i & 1) * 16);
+      }
     }
   });
 }

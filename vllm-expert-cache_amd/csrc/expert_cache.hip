@@ -264,22 +264,16 @@ bool adapters_bad(const expert_cache_adapters* l, int T) {
 }
 
 constexpr int kAdapterWaves = 4;
-#ifndef EC_AT
-#define EC_AT 128
-#define EC_AM 256
-#define EC_SW 8
-#endif
-constexpr int kShrinkManyWaves = EC_SW;
 // Up to this many tokens every adapter of a tile has workgroups of its own.
-constexpr int kAdapterFewTokens = EC_AT;
+constexpr int kAdapterFewTokens = 128;
 
 // Workgroups that share the hidden length of a tile's product: as fill the device, a unit a wave
 // at least.
 int adapter_splits(int T, int H) {
   const bool few = T <= kAdapterFewTokens;
   const int tiles = (T - 1) / (few ? kTile : kManyTokens) + 1;
-  const int units = (H - 1) / kUnit + 1, waves = few ? kAdapterWaves : kShrinkManyWaves;
-  const int most = (units - 1) / waves + 1, want = (few ? 512 : EC_AM) / tiles;
+  const int units = (H - 1) / kUnit + 1, waves = few ? kAdapterWaves : 2;
+  const int most = (units - 1) / waves + 1, want = (few ? 512 : 256) / tiles;
   return want < 1 ? 1 : want < most ? want : most;
 }
 
@@ -304,12 +298,14 @@ int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
     return (int)hipGetLastError();
   }
   const int tiles = (a.T - 1) / kManyTokens + 1;
-  hipLaunchKernelGGL((adapters_shrink_many_k<X, kShrinkManyWaves>), dim3(tiles, a.splits),
-                     dim3(kShrinkManyWaves * kWave), 0, stream, a);
+  const dim3 grid(tiles, a.splits), wide(8 * kWave);
+  if (a.R <= 32)
+    hipLaunchKernelGGL((adapters_shrink_many_k<X, 1>), grid, wide, 0, stream, a);
+  else
+    hipLaunchKernelGGL((adapters_shrink_many_k<X, 2>), grid, wide, 0, stream, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
-  hipLaunchKernelGGL((adapters_expand_many_k<X, W>), dim3(tiles, (a.O - 1) / (64 * W) + 1), block,
-                     0, stream, a);
+  hipLaunchKernelGGL((adapters_expand_many_k<X, 8>), dim3((a.O - 1) / (64 * 8) + 1, tiles), wide, 0, stream, a);
   return (int)hipGetLastError();
 }
 

@@ -40,6 +40,14 @@ struct LogitKey {
     return ~(b & 0x80000000u ? ~b : b | 0x80000000u);
   }
   static __device__ __forceinline__ Key min_of(Key v) { return wave_min_u32(v); }
+  // of lane (own lane xor X), of lane l
+  template <int X>
+  static __device__ __forceinline__ Key from(Key v) {
+    return lane_xor<X>(v);
+  }
+  static __device__ __forceinline__ Key at(Key v, int l) {
+    return (Key)__builtin_amdgcn_readlane((int)v, l);
+  }
 };
 struct ScoreKey {
   using Key = unsigned long long;
@@ -57,17 +65,41 @@ struct ScoreKey {
     const unsigned lo = wave_min_u32((unsigned)(v >> 32) == hi ? (unsigned)v : 0xFFFFFFFFu);
     return (Key)hi << 32 | lo;
   }
+  template <int X>
+  static __device__ __forceinline__ Key from(Key v) {
+    return (Key)lane_xor<X>((unsigned)(v >> 32)) << 32 | lane_xor<X>((unsigned)v);
+  }
+  static __device__ __forceinline__ Key at(Key v, int l) {
+    return (Key)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+           (unsigned)__builtin_amdgcn_readlane((int)v, l);
+  }
 };
 
 __device__ __forceinline__ bool is_candidate(float x) { return x > -__builtin_inff(); }
 
 __device__ __forceinline__ float wave_max_f32(float v) {
-  for (int d = 1; d < kWave; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
+  const auto step = [&](unsigned o) { v = fmaxf(v, bits_as<float>(o)); };
+  step(lane_xor<1>(bits_as<unsigned>(v)));
+  step(lane_xor<2>(bits_as<unsigned>(v)));
+  step(lane_xor<4>(bits_as<unsigned>(v)));
+  step(lane_xor<8>(bits_as<unsigned>(v)));
+  step(lane_xor<16>(bits_as<unsigned>(v)));
+  step(lane_xor<32>(bits_as<unsigned>(v)));
   return v;
 }
+template <int X, class T>
+__device__ __forceinline__ T lane_xor_64(T v) {
+  const unsigned long long b = bits_as<unsigned long long>(v);
+  return bits_as<T>((unsigned long long)lane_xor<X>((unsigned)(b >> 32)) << 32 |
+                    lane_xor<X>((unsigned)b));
+}
 __device__ __forceinline__ double wave_sum_f64(double v) {
-  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
-  return v;
+  v += lane_xor_64<1>(v);
+  v += lane_xor_64<2>(v);
+  v += lane_xor_64<4>(v);
+  v += lane_xor_64<8>(v);
+  v += lane_xor_64<16>(v);
+  return v + lane_xor_64<32>(v);
 }
 
 // exp(x - m) with m the largest: where that is +infinity its holders share the whole weight.
@@ -93,17 +125,21 @@ __device__ unsigned long long keep_groups(const typename K::Key* keys, const Rou
       b0 = min(b0, v);
     }
   }
-  for (int d = 1; d < P; d *= 2) {
-    const Key o0 = __shfl_xor(b0, d), o1 = __shfl_xor(b1, d);
+  const auto join = [&](Key o0, Key o1) {
     b1 = min(max(b0, o0), min(b1, o1));
     b0 = min(b0, o0);
-  }
+  };
+  if (P > 1) join(K::template from<1>(b0), K::template from<1>(b1));
+  if (P > 2) join(K::template from<2>(b0), K::template from<2>(b1));
+  if (P > 4) join(K::template from<4>(b0), K::template from<4>(b1));
+  if (P > 8) join(K::template from<8>(b0), K::template from<8>(b1));
+  if (P > 16) join(K::template from<16>(b0), K::template from<16>(b1));
   if constexpr (BIAS) {
     if (b1 != K::kNone) b0 = K::of(K::value(b0) + K::value(b1));
   }
   int better = 0;
   for (int o = 0; o < a.groups; ++o) {
-    const Key v = __shfl(b0, o * P);
+    const Key v = K::at(b0, o * P);
     better += v < b0 || (v == b0 && o < g);
   }
   const bool keep = g < a.groups && (lane & (P - 1)) == 0 && better < a.topk_groups;
@@ -136,10 +172,12 @@ __global__ __launch_bounds__(kRouteWaves* kWave) void route_k(RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
     top = wave_max_f32(top);
+    if (BIAS || !a.renormalize) {  // otherwise the scores' sum cancels
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (is_candidate(x[i])) total += softmax_term(x[i], top);
-    total = wave_sum_f64(total);
+      for (int i = 0; i < V; ++i)
+        if (is_candidate(x[i])) total += softmax_term(x[i], top);
+      total = wave_sum_f64(total);
+    }
   }
   const auto score = [&](float v) {
     return a.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : softmax_term(v, top) / total;
