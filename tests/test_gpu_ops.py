@@ -136,6 +136,17 @@ def test_experts_rows_that_end_inside_a_tile(dtype, H, I):
     _close(e(x, probs, ids), *_moe(e, x, probs, ids))
 
 
+@pytest.mark.parametrize("kind", [I8, E4, BF16, F16])
+@pytest.mark.parametrize("T,k,S,H,I", [(17, 2, 40, 256, 512), (20, 2, 60, 192, 784),
+                                       (33, 1, 30, 64, 144)])
+def test_experts_of_one_or_two_tokens_among_many(T, k, S, H, I, kind):
+    """Many tokens over more slots: each expert has a token or two, and lengths of several units
+    that end whole or inside one."""
+    e = _experts(T + I, S, H, I, kind)
+    x, probs, ids = _tokens(T + H, T, k, S, H, F16 if kind == F16 else BF16)
+    _close(e(x, probs, ids), *_moe(e, x, probs, ids))
+
+
 @pytest.mark.parametrize("T,k,S", [(16, 64, 70), (64, 16, 9), (1024, 1, 3), (1, 64, 64)])
 def test_experts_largest_calls(T, k, S):
     e = _experts(T, S, 48, 32, BF16)
@@ -319,6 +330,47 @@ def test_adapters(dtype, T, run, S, R, H, O):
     _close(y, *_adapt(l, x, base, ids))
     assert l(x, base, ids, out=base) is base   # in place
     assert torch.equal(base, y)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,run,S,R,H,O", [
+    (129, 200, 2, 8, 8, 1), (150, 1, 70, 24, 136, 33), (193, 30, 4, 64, 392, 514),
+    (300, 100, 3, 72, 1032, 127), (257, 60, 5, 256, 264, 65), (1000, 300, 2, 16, 2056, 72)])
+def test_adapters_of_many_tokens(dtype, T, run, S, R, H, O):
+    """Past 128 tokens: long runs of an adapter and tokens that all differ, ranks of one, two and
+    more tiles, ends inside tiles, odd addresses, in place, rows without an adapter."""
+    l = _adapters(T + R, S, R, H, O, dtype, scaled=T % 2 == 1)
+    x, base, ids = _adapter_tokens(T + 1, T, S, H, O, dtype, run,
+                                   torch.int64 if S % 2 else torch.int32)
+    ids[T // 2], ids[T - 1] = -1, S            # none, in the middle of a run and at the end
+    y = l(x, base, ids)
+    _close(y, *_adapt(l, x, base, ids))
+    for t in (T // 2, T - 1):
+        assert torch.equal(y[t], base[t])
+    wx = torch.full((T, H + 5), float("nan"), dtype=dtype, device=DEV)
+    wb = torch.full((T, O + 3), 5.0, dtype=dtype, device=DEV)
+    wx[:, 3:H + 3], wb[:, 1:O + 1] = x, base
+    view = wb[:, 1:O + 1]
+    assert l(wx[:, 3:H + 3], view, ids, out=view) is view
+    assert torch.equal(view, y)
+    assert (wb[:, :1] == 5).all() and (wb[:, O + 1:] == 5).all()
+
+
+def test_adapters_of_many_tokens_keep_what_is_no_number_apart():
+    l = _adapters(11, 5, 40, 200, 70, BF16)
+    x, base, ids = _adapter_tokens(11, 260, 4, 200, 70, BF16, 25)
+    clean = l(x, base, ids)
+    l.a[4], l.b[4] = float("inf"), float("nan")     # nobody's
+    assert torch.equal(l(x, base, ids), clean)
+    ids[7], ids[130] = 4, -1
+    x[9, 3] = x[130, 5] = float("nan")
+    ids[9] = 1
+    base[200, 4] = float("inf")
+    got = l(x, base, ids)
+    assert torch.isnan(got[7]).all() and torch.isnan(got[9]).all()
+    assert torch.equal(got[130], base[130]) and got[200, 4] == float("inf")
+    rest = [t for t in range(260) if t not in (7, 9, 130, 200)]
+    _close(got[rest], *(v[rest] for v in _adapt(l, torch.nan_to_num(x), base, ids.clamp(max=3))))
 
 
 def test_adapters_rows_without_one_stay_as_they_are():

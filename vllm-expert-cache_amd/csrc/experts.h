@@ -703,11 +703,12 @@ __global__ __launch_bounds__(WAVES* kWave, sizeof(W) == 1 ? 3 : 2) void experts_
             },
             [&](auto d, int i) EC_INLINE {
               const int u = unit(i);
-              each<TILES>([&](auto t) EC_INLINE {
-                w[d][t].b = w[d][0].b;
-                if ((u + 1) * kUnit > a.I) w[d][t].cut(u, a.I);
-                acc[t].template add<Bf16>(w[d][t]);
-              });
+              each<TILES>([&](auto t) EC_INLINE { w[d][t].b = w[d][0].b; });
+              // all cuts before the first sum: with a branch between two tiles' sums, the block
+              // after it read the first one's result sooner than the matrix unit wrote it
+              if ((u + 1) * kUnit > a.I)
+                each<TILES>([&](auto t) EC_INLINE { w[d][t].cut(u, a.I); });
+              each<TILES>([&](auto t) EC_INLINE { acc[t].template add<Bf16>(w[d][t]); });
             });
         each<TILES>([&](auto t) EC_INLINE {
 #pragma unroll
