@@ -239,10 +239,10 @@ enum {
  * An expert whose logit or bias is NaN or -infinity is never selected and takes no part in
  * the softmax; places that no expert is left for get id -1 and weight 0. Where logits are
  * +infinity, they share the softmax.
- * Fails with -1 unless T >= 0, 0 < E <= 1024, row_stride >= E or T <= 1, type in 0-2,
+ * Fails with -1 unless 0 <= T <= 2^21, 0 < E <= 1024, row_stride >= E or T <= 1, type in 0-2,
  * scoring in {0, 1}, groups in 1..64 divides E, 0 < topk_groups <= groups,
  * 0 < top_k <= min(64, topk_groups * E / groups), id_bytes is 4 or 8, and no array but
- * `bias` is null (unless T is 0).
+ * `bias` is null (unless T is 0). weights and ids must not meet logits, bias or each other.
  */
 int expert_cache_route(const void* logits, int type, long row_stride, const float* bias, int T,
                        int E, int top_k, int scoring, int groups, int topk_groups,
@@ -253,10 +253,10 @@ int expert_cache_route(const void* logits, int type, long row_stride, const floa
  * The experts of one layer as expert_cache_moe takes them: S slots (or experts) of
  *   w13  [S, 2*I, H]  gate rows, then up rows
  *   w2   [S, H, I]
- * contiguous and 16-byte aligned, like the scales. `weights` is `type` itself, or INT8 with a float a row
- * (s13 [S, 2*I], s2 [S, H]), or E4M3 with a float for every 128 x 128 block
- * (s13 [S, ceil(2*I/128), ceil(H/128)], s2 [S, ceil(H/128), ceil(I/128)]). `type` is that of
- * the tokens: BF16 or F16.
+ * contiguous and 16-byte aligned, like the scales. `weights` is `type` itself, or INT8 with a
+ * float a row (s13 [S, 2*I], s2 [S, H]), or E4M3 with a float for every 128 x 128 block (s13
+ * [S, ceil(2*I/128), ceil(H/128)], s2 [S, ceil(H/128), ceil(I/128)]). `type` is that of the
+ * tokens: BF16 or F16.
  */
 typedef struct expert_cache_experts {
   int S, H, I, type, weights;
@@ -273,14 +273,15 @@ int expert_cache_moe_workspace(const expert_cache_experts* e, int T, int top_k, 
  * A mixture-of-experts layer for a few tokens, over slots:
  *   out_t = sum_j topk_weights[t, j] * w2[s] (silu(gate_s x_t) * (up_s x_t)), s = ids[t, j]
  * x [T, H] and out [T, H] are of the layer's type, rows x_stride and out_stride elements apart,
- * x 16-byte aligned with x_stride a multiple of 8; out must not overlap x. ids (int32 or int64
- * by id_bytes) are slot ids as expert_cache_refresh hands them out. A pair whose id is outside
+ * x 16-byte aligned with x_stride a multiple of 8; the memory from out's first to its last
+ * element must not meet that of x, ids or topk_weights. ids (int32 or int64 by id_bytes) are
+ * slot ids as expert_cache_refresh hands them out. A pair whose id is outside
  * [0, S) or whose weight is 0 adds nothing and reads no weights; a token without any other
  * pair gets zeros. All sums are in 32 bits, and only `out` is rounded to `type`. `workspace`
  * (16-byte aligned, expert_cache_moe_workspace bytes) is the call's own until it has run.
  * Fails with -1 unless the layer is as above, H and I are multiples of 8 (of 16 with one-byte
- * weights), 0 <= T, 0 < top_k <= 64, T * top_k <= 1024, id_bytes is 4 or 8, and no array is
- * null (unless T is 0).
+ * weights) and at most 2^24, 0 <= T, 0 < top_k <= 64, T * top_k <= 1024, id_bytes is 4 or 8,
+ * and no array is null (unless T is 0).
  */
 int expert_cache_moe(const expert_cache_experts* e, const void* x, long x_stride,
                      const float* topk_weights, const void* ids, int id_bytes, int T, int top_k,
@@ -305,11 +306,11 @@ int expert_cache_adapt_workspace(const expert_cache_adapters* l, int T, long* by
  *   out_t = base_t + scales[s] * b[s] (a[s] x_t),  s = ids[t]
  * x [T, H], base [T, O] and out [T, O] are of the adapters' type, rows x_stride, base_stride
  * and out_stride elements apart, x 16-byte aligned with x_stride a multiple of 8. out is base
- * itself (same address and stride) or overlaps neither base nor x. A token whose id is outside
- * [0, S) has no adapter: its row is base's, and is not written where out is base. All sums are
- * in 32 bits, and only `out` is rounded to `type`. `workspace` as for expert_cache_moe.
- * Fails with -1 unless S, O > 0, H and R are positive multiples of 8, R <= 256, T >= 0,
- * id_bytes is 4 or 8, and no array but `scales` is null (unless T is 0).
+ * itself (same address and stride) or meets neither base nor x, and never ids. A token whose id
+ * is outside [0, S) has no adapter: its row is base's, and is not written where out is base. All
+ * sums are in 32 bits, and only `out` is rounded to `type`. `workspace` as for expert_cache_moe.
+ * Fails with -1 unless S > 0, 0 < O <= 2^21, H and R are positive multiples of 8, H <= 2^24,
+ * R <= 256, 0 <= T <= 2^21, id_bytes is 4 or 8, and no array but `scales` is null (unless T is 0).
  */
 int expert_cache_adapt(const expert_cache_adapters* l, const void* x, long x_stride,
                        const void* ids, int id_bytes, int T, const void* base,

@@ -335,9 +335,10 @@ def test_adapters(dtype, T, run, S, R, H, O):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("T,run,S,R,H,O", [
     (129, 200, 2, 8, 8, 1), (150, 1, 70, 24, 136, 33), (193, 30, 4, 64, 392, 514),
-    (300, 100, 3, 72, 1032, 127), (257, 60, 5, 256, 264, 65), (1000, 300, 2, 16, 2056, 72)])
+    (300, 100, 3, 72, 1032, 127), (257, 60, 5, 256, 264, 65), (1000, 300, 2, 16, 2056, 72),
+    (280, 1, 70, 24, 136, 33), (257, 30, 4, 8, 8, 1), (321, 30, 4, 64, 392, 514)])
 def test_adapters_of_many_tokens(dtype, T, run, S, R, H, O):
-    """Past 128 tokens: long runs of an adapter and tokens that all differ, ranks of one, two and
+    """Many tokens: long runs of an adapter and tokens that all differ, ranks of one, two and
     more tiles, ends inside tiles, odd addresses, in place, rows without an adapter."""
     l = _adapters(T + R, S, R, H, O, dtype, scaled=T % 2 == 1)
     x, base, ids = _adapter_tokens(T + 1, T, S, H, O, dtype, run,

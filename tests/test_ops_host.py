@@ -39,6 +39,25 @@ def test_route_rejects(lib, over):
     assert _route(lib, **over) == -1
 
 
+@pytest.mark.parametrize("over", [
+    dict(T=2 ** 21 + 1), dict(T=2 ** 31 - 1, E=1, stride=1, k=1),
+    dict(weights=0x1020), dict(ids=0x1038), dict(ids=0x2008), dict(bias=0x2008),
+    dict(bias=0x2FF0), dict(type=1, weights=0x101C)], ids=str)
+def test_route_rejects_what_meets_or_is_too_long(lib, over):
+    assert _route(lib, **over) == -1
+
+
+@pytest.mark.parametrize("over", [dict(out=0x40008), dict(out=0x50000), dict(ids=0x60030)],
+                         ids=str)
+def test_results_over_ids_and_weights_are_refused(lib, over):
+    assert _moe(lib, **over) == -1
+
+
+def test_adapters_past_what_a_grid_holds_are_refused(lib):
+    assert _adapt(lib, T=2 ** 21 + 1) == -1
+    assert _adapt(lib, O=2 ** 21 + 1, bs=2 ** 21 + 1, os=2 ** 21 + 1) == -1
+
+
 def test_nothing_to_do_is_no_call(lib):
     assert _route(lib, T=0, logits=None, weights=None, ids=None) == 0
     assert _moe(lib, T=0, x=None, out=None, ids=None, work=None) == 0
@@ -269,3 +288,21 @@ def _rows(T=3, H=32, O=24, dtype=BF16, ids=torch.int32):
 def test_adapters_arguments(anywhere, x, base, ids, out):
     with pytest.raises(ValueError):
         ops.Adapters(*_ab())(x, base, ids, out)
+
+
+def test_what_is_too_long_is_refused(anywhere):
+    with pytest.raises(ValueError):
+        ops.route(torch.empty(ops.MAX_TOKENS + 1, 1), 1)
+    with pytest.raises(ValueError):
+        ops.Adapters(torch.empty(1, 8, 8, dtype=BF16),
+                     torch.empty(1, ops.MAX_OUTPUTS + 1, 8, dtype=BF16))
+    with pytest.raises(ValueError):
+        ops.Adapters(torch.empty(1, 8, ops.MAX_LENGTH + 8, dtype=BF16),
+                     torch.empty(1, 8, 8, dtype=BF16))
+    with pytest.raises(ValueError):
+        ops.Experts(torch.empty(1, 32, ops.MAX_LENGTH + 16, dtype=I8),
+                    torch.empty(1, ops.MAX_LENGTH + 16, 16, dtype=I8))
+    T = ops.MAX_TOKENS + 1
+    with pytest.raises(ValueError):
+        ops.Adapters(*_ab(H=8, O=1))(torch.empty(T, 8, dtype=BF16), torch.empty(T, 1, dtype=BF16),
+                                     torch.empty(T, dtype=torch.int32))

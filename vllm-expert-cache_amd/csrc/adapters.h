@@ -116,38 +116,32 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a
   }
 }
 
-// B's product and the sum with the base for one tile, 16 * TILES outputs a wave. The rows of
-// the TILES instructions are interleaved so that a lane ends with 4 * TILES neighbouring ones.
-// AHEAD adapters of a tile are loaded at a time.
-template <class X, int WAVES, int TILES, int AHEAD>
+// B's product and the sum with the base for one tile, 16 outputs a wave: few, so that a tile has
+// many waves. AHEAD adapters of a tile are loaded at a time: 33 tokens, rank 64, H and O 4096,
+// an adapter each take 27.1 us one by one and 23.4 us four by four.
+template <class X, int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a) {
-  constexpr int kRun = 4 * TILES;
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int t0 = blockIdx.x * kTile, token = t0 + column;
-  const int row0 = (blockIdx.y * WAVES + wave) * (16 * TILES);
+  const int row0 = (blockIdx.y * WAVES + wave) * kTile;
   if (row0 >= a.O) return;
   const int id = tile_slot(a, t0);
-  const bool fast = a.aligned && row0 + 16 * TILES <= a.O;
+  const bool fast = a.aligned && row0 + kTile <= a.O;
   const bool write = token < a.T && !(id < 0 && a.base == a.out);
-  const int o0 = row0 + quarter * kRun;
+  const int o0 = row0 + quarter * 4;
   const unsigned short* base = static_cast<const unsigned short*>(a.base) +
                                min(token, a.T - 1) * a.base_stride + o0;
-  unsigned short in[kRun];
+  unsigned short in[4];
   if (fast) {
-    __builtin_memcpy(in, __builtin_assume_aligned(base, 8 * (TILES > 1 ? 2 : 1)), sizeof in);
+    __builtin_memcpy(in, __builtin_assume_aligned(base, 8), sizeof in);
   } else {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) in[i] = o0 + i < a.O ? base[i] : 0;
+    for (int i = 0; i < 4; ++i) in[i] = o0 + i < a.O ? base[i] : 0;
   }
-  f32x4 total[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) total[t] = f32x4{0, 0, 0, 0};
+  f32x4 total = {0, 0, 0, 0};
   if (ballot(id >= 0)) {
-    unsigned rows[TILES];
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-      rows[t] = row_bytes<X>(row0 + (column >> 2) * kRun + t * 4 + (column & 3), row0, a.O, a.R);
+    const unsigned row = row_bytes<X>(row0 + column, row0, a.O, a.R);
     const float scale = id < 0 ? 0.f : a.scales ? a.scales[id] : 1.f;
     for (int k0 = 0; k0 < a.R; k0 += 32) {
       const int k = k0 + quarter * 8;
@@ -174,7 +168,7 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
       unsigned long long left = ballot(id >= 0) & 0xFFFFu;
       while (left) {
         int slot[AHEAD];
-        u32x4 w[AHEAD][TILES];
+        u32x4 w[AHEAD];
         each<AHEAD>([&](auto n) EC_INLINE {
           // (past the last adapter: the one before once more, for no column)
           const bool more = n == 0 || left != 0;
@@ -183,16 +177,13 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
           const int read = s < 0 ? 0 : s;
           left &= ~ballot(id == s);
           slot[n] = more ? s : -2;
-          const char* from = static_cast<const char*>(a.b) +
-                             ((long long)read * a.O + row0) * (2LL * a.R);
-          each<TILES>([&](auto t) EC_INLINE { w[n][t] = load16(from + (rows[t] + at)); });
+          w[n] = load16(static_cast<const char*>(a.b) +
+                        ((long long)read * a.O + row0) * (2LL * a.R) + (row + at));
         });
         each<AHEAD>([&](auto n) EC_INLINE {
-          each<TILES>([&](auto t) EC_INLINE {
-            const f32x4 c = mfma_split<X>(keep(k < a.R, w[n][t]), 0, hi, lo, f32x4{0, 0, 0, 0});
+          const f32x4 c = mfma_split<X>(keep(k < a.R, w[n]), 0, hi, lo, f32x4{0, 0, 0, 0});
 #pragma unroll
-            for (int i = 0; i < 4; ++i) total[t][i] += id == slot[n] ? c[i] : 0.f;
-          });
+          for (int i = 0; i < 4; ++i) total[i] += id == slot[n] ? c[i] : 0.f;
         });
       }
     }
@@ -201,14 +192,13 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
   unsigned short* out = static_cast<unsigned short*>(a.out) + token * a.out_stride + o0;
   if (id >= 0) {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i)
-      in[i] = from_f32<X>(to_f32(X{in[i]}) + total[i / 4][i & 3]).v;
+    for (int i = 0; i < 4; ++i) in[i] = from_f32<X>(to_f32(X{in[i]}) + total[i]).v;
   }
   if (fast) {
-    __builtin_memcpy(__builtin_assume_aligned(out, 8 * (TILES > 1 ? 2 : 1)), in, sizeof in);
+    __builtin_memcpy(__builtin_assume_aligned(out, 8), in, sizeof in);
   } else {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i)
+    for (int i = 0; i < 4; ++i)
       if (o0 + i < a.O) out[i] = in[i];
   }
 }
@@ -216,23 +206,23 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
 constexpr int kManyTokens = 64;  // of a workgroup of the kernels below: a lane each
 constexpr int kManyTiles = kManyTokens / kTile;
 
-// A's product for 64 tokens over one split of the hidden length, 32 * ROWS ranks at a time. A unit
+// A's product for 64 tokens over one split of the hidden length, 64 ranks at a time. A unit
 // of the tokens and of A goes through LDS: from the L1 each wave would take the rows it shares
 // with the others for itself, and what a compute unit gets from its L1 (56 bytes/ns) is the
 // bound then. A wave has 32 of the ranks, 32 of the tokens and a part of each unit.
-template <class X, int ROWS>
+template <class X>
 __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersArgs a) {
-  constexpr int kRows = 32 * ROWS, kParts = 4 / ROWS, D = 4;
+  constexpr int kRows = 64, D = 4;
   constexpr int kPitch = 2 * kUnit + 16;  // bytes of a row: 16 rows start in different banks
   constexpr int kLine = 2 * kUnit / 16;   // lanes that read a row's unit
   constexpr int kEach = 8 * kWave / kLine;  // rows that the workgroup reads at once
   __shared__ __attribute__((aligned(16))) union {
     char unit[2][kRows + kManyTokens][kPitch];
-    f32x4 parts[kParts - 1][2 * ROWS][2][2][kWave];
+    f32x4 parts[4][2][2][kWave];
   } lds;
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int half = wave & 1, group = wave / 2 % ROWS, part = wave / (2 * ROWS);
+  const int half = wave & 1, group = wave / 2 % 2, part = wave / 4;
   const int t0 = blockIdx.x * kManyTokens;
   int id = load_id(a.ids, min(t0 + lane, a.T - 1), a.wide, a.S);
   if (t0 + lane >= a.T) id = -1;
@@ -256,14 +246,14 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
     }
     for (int r0 = 0; r0 < a.R; r0 += kRows) {
       const char* from = static_cast<const char*>(a.a) + ((long long)slot * a.R + r0) * (2LL * a.H);
-      unsigned rows[ROWS];
+      unsigned rows[2];
 #pragma unroll
-      for (int j = 0; j < ROWS; ++j) rows[j] = row_bytes<X>(r0 + my_row + j * kEach, r0, a.R, a.H);
+      for (int j = 0; j < 2; ++j) rows[j] = row_bytes<X>(r0 + my_row + j * kEach, r0, a.R, a.H);
       f32x4 acc[2][2];
       each<2>([&](auto r) EC_INLINE {
         each<2>([&](auto c) EC_INLINE { acc[r][c] = f32x4{0, 0, 0, 0}; });
       });
-      u32x4 w[D][ROWS], b[D][2];
+      u32x4 w[D][2], b[D][2];
       const auto unit = [&](int i) EC_INLINE {
         return (int)blockIdx.y + a.splits * wrap(i + start, count);
       };
@@ -273,13 +263,13 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
           [&](auto d, int i) EC_INLINE {
             const int k = unit(i) * kUnit + my_k;
             const unsigned at = k < a.H ? 2u * k : 0u;
-            each<ROWS>([&](auto j) EC_INLINE { w[d][j] = load16(from + (rows[j] + at)); });
+            each<2>([&](auto j) EC_INLINE { w[d][j] = load16(from + (rows[j] + at)); });
             each<2>([&](auto j) EC_INLINE { b[d][j] = load16(x[j] + at / 2); });
           },
           [&](auto d, int i) EC_INLINE {
             char(*to)[kPitch] = lds.unit[i & 1];
             const bool in = unit(i) * kUnit + my_k < a.H;
-            each<ROWS>([&](auto j) EC_INLINE {
+            each<2>([&](auto j) EC_INLINE {
               *reinterpret_cast<u32x4*>(&to[my_row + j * kEach][2 * my_k]) = keep(in, w[d][j]);
             });
             each<2>([&](auto j) EC_INLINE {
@@ -288,8 +278,8 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
             });
             lds_sync();  // two units in turn: the other is free once all have come here
             if (!any) return;
-            each<ROWS>([&](auto s) EC_INLINE {  // 32 values of k at a time, of the unit's four
-              const int k = (part * ROWS + s) * 64 + quarter * 16;
+            each<2>([&](auto s) EC_INLINE {  // 32 values of k at a time, of the unit's four
+              const int k = (part * 2 + s) * 64 + quarter * 16;
               u32x4 rw[2], cl[2];
               each<2>([&](auto n) EC_INLINE {
                 rw[n] = load16(&to[group * 32 + n * 16 + column][k]);
@@ -306,7 +296,7 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
       if (part) {
         each<2>([&](auto r) EC_INLINE {
           each<2>([&](auto c) EC_INLINE {
-            lds.parts[part - 1][wave % (2 * ROWS)][r][c][lane] = acc[r][c];
+            lds.parts[wave - 4][r][c][lane] = acc[r][c];
           });
         });
       }
@@ -316,9 +306,7 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
           each<2>([&](auto c) EC_INLINE {
             const int t = half * 32 + c * 16 + column;
             const int row = r0 + group * 32 + r * 16 + quarter * 4;
-            f32x4 y = acc[r][c];
-#pragma unroll
-            for (int p = 0; p < kParts - 1; ++p) y += lds.parts[p][wave][r][c][lane];
+            const f32x4 y = acc[r][c] + lds.parts[wave][r][c][lane];
             if (own >> t & 1 && row < a.R)
               *reinterpret_cast<f32x4*>(
                   a.v + ((long long)blockIdx.y * a.T + t0 + t) * a.R + row) = y;
@@ -373,15 +361,16 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersA
 #pragma unroll
     for (int n = 0; n < N; ++n) total[c][n] = f32x4{0, 0, 0, 0};
   unsigned rows[N];
+  const int from0 = min(row0, a.O - 1);
 #pragma unroll
   for (int n = 0; n < N; ++n)
-    rows[n] = row_bytes<X>(min(row0, a.O - 1) + n / 2 * 32 + (column >> 2) * 8 + n % 2 * 4 + (column & 3),
-                           min(row0, a.O - 1), a.O, a.R);
+    rows[n] = row_bytes<X>(from0 + n / 2 * 32 + (column >> 2) * 8 + n % 2 * 4 + (column & 3),
+                           from0, a.O, a.R);
   u32x4 w[2][N];
   // 64 ranks of an adapter's rows
   const auto load_rows = [&](int slot, int r0) EC_INLINE {
     const char* from = static_cast<const char*>(a.b) +
-                       ((long long)slot * a.O + min(row0, a.O - 1)) * (2LL * a.R);
+                       ((long long)slot * a.O + from0) * (2LL * a.R);
     each<2>([&](auto h) EC_INLINE {
       const int k = r0 + h * 32 + quarter * 8;
       each<N>([&](auto n) EC_INLINE {

@@ -174,6 +174,9 @@ int launch_route(const RouteArgs& a, hipStream_t stream) {
 
 // Longest rows of weights: the bytes of 64 of them are counted in 32 bits.
 constexpr int kMaxLength = 1 << 24;
+// Most tokens of a call of expert_cache_route and expert_cache_adapt, and most outputs of an
+// adapter: what a grid's second dimension (65535 workgroups) holds, with room.
+constexpr int kMaxTokens = 1 << 21, kMaxOutputs = 1 << 21;
 
 bool experts_bad(const expert_cache_experts* e, int T, int top_k) {
   if (e == nullptr || e->S <= 0 || e->H <= 0 || e->I <= 0) return true;
@@ -187,14 +190,30 @@ bool experts_bad(const expert_cache_experts* e, int T, int top_k) {
 }
 
 constexpr int kUpWaves = 4, kDownWaves = 8;
-constexpr int kPairTiles = 4;
+constexpr int kPairTiles = 4, kPairRows = kPairTiles * kTile;
+
+// All figures below are us a call in a graph on MI355X.
+
 // Above 8 tokens, experts of this many weights in w2 at most take the down projection of few
 // tokens. It reads an expert once for every two of its tokens (from the L2 after the first), which
-// costs more than the other's third launch once the experts are large. Measured on MI355X, us a
-// call, few / not: 16 tokens, top-7 of 30 slots, 480 x 80 fp8 12.8 / 26.9; 9 tokens, top-6 of 186,
-// 448 x 1152 float16 57.4 / 63.3; 14 tokens, top-10 of 24, 6240 x 1920 int8 301 / 221; 16 tokens,
-// top-8 of 128, 7168 x 2048 fp8 472 / 444.
-constexpr long kFewWeights = 1 << 21;
+// costs more than the other's third launch once the experts are large. Few / not: 16 tokens,
+// top-7 of 30 slots, 480 x 80 fp8 11.8 / 14.7; 9 tokens, top-6 of 186, 448 x 1152 float16 53 / 60;
+// 16 tokens, top-8 of 128, 2048 x 1408 bf16 221 / 242; 14 tokens, top-10 of 24, 6240 x 1920 int8
+// 301 / 221; 16 tokens, top-2 of 8, 4096 x 7168 bf16 304 / 236.
+constexpr long kFewWeights = 1 << 22;
+// Up to 8 tokens few is the better one or close: 8 tokens, few / not: top-8 of 64, 2048 x 768 int8
+// 46 / 51; 2048 x 1408 bf16 124 / 139; top-2 of 8, 4096 x 7168 bf16 216 / 201.
+constexpr int kAlwaysFew = 8;
+// A workgroup of experts_down_k takes 8 rows where that makes 512 workgroups at most, else 16:
+// 8 / 16 rows: one token on 8 int8 experts, H 2048 14.1 / 15.6; on 8 fp8 experts, H 7168 62.1 /
+// 59.8.
+constexpr int kRowGroups = 510;
+// Down projection of more tokens: the waves of a workgroup share a row's length only as far as
+// rows alone do not make this many workgroups. Each for itself / four together: 32 tokens, top-8
+// of 64, 2048 x 512 int8 (512 workgroups) 56 / 64; 2048 x 1408 bf16 184 / 192; but 64 tokens, top-4
+// of 32, 2048 x 256 bf16 (256) 36.7 / 33.6; 24 tokens, top-2 of 8, 4096 x 7168 bf16 (128) 302 /
+// 249.
+constexpr int kPairGroups = 512;
 
 // How a call of expert_cache_moe is split up, and where things are in its workspace.
 struct MoePlan {
@@ -202,16 +221,23 @@ struct MoePlan {
   int groups, down_groups, splits, k_waves;
   long lo, part, meta, arrived, bytes;
 };
-MoePlan moe_plan(int H, int I, int T, int top_k) {
+MoePlan moe_plan(int S, int H, int I, int T, int top_k) {
   const long n = (long)T * top_k;
   MoePlan p;
-  p.few = T <= 8 || (T <= kFewTokens && (long)H * I <= kFewWeights);
+  p.few = T <= kAlwaysFew || (T <= kFewTokens && (long)H * I <= kFewWeights);
   const int units = (I - 1) / kUnit + 1;
-  p.k_waves = units >= 4 ? 4 : units >= 2 ? 2 : 1;
-  p.groups = p.few ? (H <= 16 * 255 ? 1 : 2) : 2 * kPairTiles * (4 / p.k_waves);
+  const long all = n < S ? n : S;
+  p.k_waves = 1;
+  while (p.k_waves < 4 && 2 * p.k_waves <= units &&
+         all * ((H - 1) / (kPairRows * (4 / p.k_waves)) + 1) < kPairGroups)
+    p.k_waves *= 2;
+  p.groups = p.few ? (H <= 8 * kRowGroups ? 1 : 2) : 2 * kPairTiles * (4 / p.k_waves);
   p.down_groups = (H - 1) / (8 * p.groups) + 1;
   p.splits = 1;
-  if (p.few) {  // workgroups that share their rows: as fill the device, a unit a wave at least
+  // Workgroups that share their rows: as fill the device, a unit a wave at least. Shared / not: 16
+  // tokens, top-8 of 64, 512 x 2048 bf16 113 / 174; one token on 2 experts, 1024 x 4096 bf16 15.8 /
+  // 16.4; on 8, 1024 x 512 13.0 / 12.3.
+  if (p.few) {
     const int want = 256 / p.down_groups, most = (int)n * units / kDownWaves;
     p.splits = want < 2 || most < 2 ? 1 : want < most ? want : most;
   }
@@ -248,7 +274,9 @@ int launch_moe_of(const ExpertsArgs& a, int T, int groups, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
-// Weights whose rows are whole lines of 128 bytes are read past the caches.
+// Weights whose rows are whole lines of 128 bytes are read past the caches: us past / through
+// them: one token on 2 bf16 experts of 176 MB 62.8 / 67.0, on 8 fp8 experts of 44 MB 59.8 / 65.7;
+// where a load's lines are shared with another one it costs: 5 tokens, H 1048, float16 23.7 / 21.1.
 template <class X, class W>
 int launch_moe(const ExpertsArgs& a, int T, int groups, hipStream_t stream) {
   const uintptr_t lines = reinterpret_cast<uintptr_t>(a.w13) | reinterpret_cast<uintptr_t>(a.w2) |
@@ -258,17 +286,19 @@ int launch_moe(const ExpertsArgs& a, int T, int groups, hipStream_t stream) {
 }
 
 bool adapters_bad(const expert_cache_adapters* l, int T) {
-  if (l == nullptr || l->S <= 0 || l->O <= 0 || l->H <= 0 || l->R <= 0 || T < 0) return true;
+  if (l == nullptr || l->S <= 0 || l->O <= 0 || l->H <= 0 || l->R <= 0) return true;
+  if (T < 0 || T > kMaxTokens || l->O > kMaxOutputs) return true;
   if (l->type != EXPERT_CACHE_BF16 && l->type != EXPERT_CACHE_F16) return true;
   return l->H % 8 || l->R % 8 || l->R > kAdapterMaxRank || l->H > kMaxLength;
 }
 
 constexpr int kAdapterWaves = 4;
 // Up to this many tokens every adapter of a tile has workgroups of its own.
-constexpr int kAdapterFewTokens = 128;
+constexpr int kAdapterFewTokens = 256;
 
 // Workgroups that share the hidden length of a tile's product: as fill the device, a unit a wave
-// at least.
+// at least. Half as many for many tokens: 4096 tokens, rank 64 39.3 and not 37.7 us with one
+// adapter, 1024 tokens 21.1 and not 23.4, with 64 adapters 242 and not 200.
 int adapter_splits(int T, int H) {
   const bool few = T <= kAdapterFewTokens;
   const int tiles = (T - 1) / (few ? kTile : kManyTokens) + 1;
@@ -285,6 +315,8 @@ int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
   if (few) {
     const int tiles = (a.T - 1) / kTile + 1;
     const dim3 shrink(tiles, kTile, a.splits);
+    // as many ranks at a time as there are: 16 tokens, rank 16 one tile at a time 8.6 us, four 9.5;
+    // rank 64 21.0 and 19.3; rank 32, two 11.8, one 13.0, four 12.7
     if (a.R <= 16)
       hipLaunchKernelGGL((adapters_shrink_k<X, W, 1>), shrink, block, 0, stream, a);
     else if (a.R <= 32)
@@ -293,19 +325,17 @@ int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
       hipLaunchKernelGGL((adapters_shrink_k<X, W, 4>), shrink, block, 0, stream, a);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    hipLaunchKernelGGL((adapters_expand_k<X, W, 1, 4>), dim3(tiles, (a.O - 1) / (16 * W) + 1),
+    hipLaunchKernelGGL((adapters_expand_k<X, W, 4>), dim3(tiles, (a.O - 1) / (16 * W) + 1),
                        block, 0, stream, a);
     return (int)hipGetLastError();
   }
   const int tiles = (a.T - 1) / kManyTokens + 1;
   const dim3 grid(tiles, a.splits), wide(8 * kWave);
-  if (a.R <= 32)
-    hipLaunchKernelGGL((adapters_shrink_many_k<X, 1>), grid, wide, 0, stream, a);
-  else
-    hipLaunchKernelGGL((adapters_shrink_many_k<X, 2>), grid, wide, 0, stream, a);
+  hipLaunchKernelGGL((adapters_shrink_many_k<X>), grid, wide, 0, stream, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
-  hipLaunchKernelGGL((adapters_expand_many_k<X, 8>), dim3((a.O - 1) / (64 * 8) + 1, tiles), wide, 0, stream, a);
+  hipLaunchKernelGGL((adapters_expand_many_k<X, 8>), dim3((a.O - 1) / (64 * 8) + 1, tiles), wide, 0,
+                     stream, a);
   return (int)hipGetLastError();
 }
 
@@ -490,7 +520,8 @@ int expert_cache_route(const void* logits, int type, long row_stride, const floa
                        int E, int top_k, int scoring, int groups, int topk_groups,
                        int renormalize, float scale, float* weights, void* ids, int id_bytes,
                        hipStream_t stream) {
-  if (T < 0 || E <= 0 || E > kRouteMaxExperts || (row_stride < E && T > 1)) return -1;
+  if (T < 0 || T > kMaxTokens) return -1;
+  if (E <= 0 || E > kRouteMaxExperts || (row_stride < E && T > 1)) return -1;
   if (scoring < 0 || scoring > 1 || (id_bytes != 4 && id_bytes != 8)) return -1;
   if (groups < 1 || groups > kRouteMaxGroups || E % groups) return -1;
   if (topk_groups < 1 || topk_groups > groups) return -1;
@@ -498,6 +529,14 @@ int expert_cache_route(const void* logits, int type, long row_stride, const floa
   if (type < EXPERT_CACHE_F32 || type > EXPERT_CACHE_F16) return -1;
   if (T == 0) return 0;
   if (logits == nullptr || weights == nullptr || ids == nullptr) return -1;
+  const long long n = (long long)T * top_k, read = ((T - 1LL) * row_stride + E) *
+                                                   (type == EXPERT_CACHE_F32 ? 4 : 2);
+  if (ranges_meet(logits, read, weights, 4 * n) || ranges_meet(logits, read, ids, id_bytes * n) ||
+      ranges_meet(weights, 4 * n, ids, id_bytes * n))
+    return -1;
+  if (bias && (ranges_meet(bias, 4LL * E, weights, 4 * n) ||
+               ranges_meet(bias, 4LL * E, ids, id_bytes * n)))
+    return -1;
   const RouteArgs a = {logits,       row_stride,       bias,          T,     E,       top_k, groups,
                        topk_groups,  scoring == 1,     renormalize != 0, id_bytes == 8, scale,
                        weights,      ids};
@@ -507,7 +546,7 @@ int expert_cache_route(const void* logits, int type, long row_stride, const floa
 
 int expert_cache_moe_workspace(const expert_cache_experts* e, int T, int top_k, long* bytes) {
   if (bytes == nullptr || experts_bad(e, T, top_k)) return -1;
-  *bytes = moe_plan(e->H, e->I, T, top_k).bytes;
+  *bytes = moe_plan(e->S, e->H, e->I, T, top_k).bytes;
   return 0;
 }
 
@@ -524,8 +563,11 @@ int expert_cache_moe(const expert_cache_experts* e, const void* x, long x_stride
   if (out == nullptr || (out_stride < e->H && T > 1)) return -1;
   if (topk_weights == nullptr || ids == nullptr) return -1;
   if (workspace == nullptr || !aligned16(workspace)) return -1;
-  if (ranges_meet(x, 2 * ((T - 1LL) * x_stride + e->H), out,
-                  2 * ((T - 1LL) * out_stride + e->H)))
+  // the last launch reads the ids and weights again while it writes the result
+  const long long out_bytes = 2 * ((T - 1LL) * out_stride + e->H), n = (long long)T * top_k;
+  if (ranges_meet(x, 2 * ((T - 1LL) * x_stride + e->H), out, out_bytes) ||
+      ranges_meet(ids, n * id_bytes, out, out_bytes) ||
+      ranges_meet(topk_weights, 4 * n, out, out_bytes))
     return -1;
   ExpertsArgs a;
   a.x = x;
@@ -542,8 +584,10 @@ int expert_cache_moe(const expert_cache_experts* e, const void* x, long x_stride
   a.H = e->H;
   a.I = e->I;
   a.wide = id_bytes == 8;
+  // a workgroup for every slot where those are fewer than pairs: 32 tokens, top-8 of 128, 2048 x
+  // 768 bf16 199 us, 223 with one for every pair; 64 tokens, top-4 of 32, 2048 x 256 34.4 and 45.0
   a.by_slot = a.n > a.S;
-  const MoePlan plan = moe_plan(e->H, e->I, T, top_k);
+  const MoePlan plan = moe_plan(e->S, e->H, e->I, T, top_k);
   a.few = plan.few;
   a.down_groups = plan.down_groups;
   a.splits = plan.splits;
@@ -587,7 +631,9 @@ int expert_cache_adapt(const expert_cache_adapters* l, const void* x, long x_str
   const bool in_place = out == base && (out_stride == base_stride || T == 1);
   if (!in_place && ranges_meet(base, 2 * ((T - 1LL) * base_stride + l->O), out, out_bytes))
     return -1;
-  if (ranges_meet(x, 2 * ((T - 1LL) * x_stride + l->H), out, out_bytes)) return -1;
+  if (ranges_meet(x, 2 * ((T - 1LL) * x_stride + l->H), out, out_bytes) ||
+      ranges_meet(ids, (long long)T * id_bytes, out, out_bytes))
+    return -1;
   AdaptersArgs a;
   a.x = x;
   a.x_stride = x_stride;

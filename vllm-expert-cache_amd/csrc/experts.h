@@ -57,6 +57,16 @@ struct ExpertsArgs {
   long long out_stride;  // elements
 };
 
+// f(0), f(1), ... f(N - 1) with compile-time arguments: arrays that they index stay in registers.
+template <class F, int... I>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  each(f, std::make_integer_sequence<int, N>());
+}
+
 // Which of a lane's 16-byte loads of a unit starts at which k, and which operand of eight
 // values (f of 4) does.
 template <class W>
@@ -89,33 +99,49 @@ __device__ __forceinline__ int list_pairs(const ExpertsArgs& a, int p, int& slot
   slot = a.by_slot ? p : __builtin_amdgcn_readfirstlane(id_of(own, a.wide, a.S));
   if (slot < 0) return 0;
   int count = 0, last = -1;  // last token seen
-  for (int base = 0;;) {
+  // 64 pairs from `base`; false if the slot is another workgroup's
+  const auto take = [&](int base, int at, int id, float w) EC_INLINE {
     const bool mine = id == slot && w != 0.f && base + lane < a.n;
     const unsigned long long m = ballot(mine);
-    if (m != 0) {
-      if (count == 0 && !a.by_slot && base + __builtin_ctzll(m) != p) return 0;
-      const int token = at / a.k;
-      const unsigned long long before = m & lanes_below();
-      const int prev = __shfl(token, before ? 63 - __builtin_clzll(before) : 0);
-      const bool again = mine && token == (before ? prev : last);
-      const unsigned long long firsts = ballot(mine && !again);
-      const int pos = count + __builtin_popcountll(firsts & lanes_below()) - (again ? 1 : 0);
-      if (writer) {
-        if (mine && !again) {
-          list.pair[pos] = (unsigned short)at;
-          list.weight[pos] = w;
-        }
-        for (unsigned long long r = m & ~firsts; r; r &= r - 1)
-          if (lane == __builtin_ctzll(r)) list.weight[pos] += w;
+    if (m == 0) return true;
+    if (count == 0 && !a.by_slot && base + __builtin_ctzll(m) != p) return false;
+    const int token = at / a.k;
+    const unsigned long long before = m & lanes_below();
+    const int prev = __shfl(token, before ? 63 - __builtin_clzll(before) : 0);
+    const bool again = mine && token == (before ? prev : last);
+    const unsigned long long firsts = ballot(mine && !again);
+    const int pos = count + __builtin_popcountll(firsts & lanes_below()) - (again ? 1 : 0);
+    if (writer) {
+      if (mine && !again) {
+        list.pair[pos] = (unsigned short)at;
+        list.weight[pos] = w;
       }
-      count += __builtin_popcountll(firsts);
-      last = __shfl(token, 63 - __builtin_clzll(m));
+      for (unsigned long long r = m & ~firsts; r; r &= r - 1)
+        if (lane == __builtin_ctzll(r)) list.weight[pos] += w;
     }
-    base += kWave;
-    if (base >= a.n) break;
-    at = min(base + lane, a.n - 1);
-    id = load_id(a.ids, at, a.wide, a.S);
-    w = a.probs[at];
+    count += __builtin_popcountll(firsts);
+    last = __shfl(token, 63 - __builtin_clzll(m));
+    return true;
+  };
+  if (!take(0, at, id, w)) return 0;
+  // Loads of four lots are under way at once: one lot at a time, 128 tokens, top-8, 2048 x 256
+  // take 123 us and not 111.
+  constexpr int kAhead = 4;
+  for (int base = kWave; base < a.n; base += kAhead * kWave) {
+    RawId raws[kAhead];
+    float ws[kAhead];
+    each<kAhead>([&](auto j) EC_INLINE {
+      at = min(base + j * kWave + lane, a.n - 1);
+      raws[j] = raw_id(a.ids, at, a.wide);
+      ws[j] = a.probs[at];
+    });
+    bool own_slot = true;
+    each<kAhead>([&](auto j) EC_INLINE {
+      const int from = base + j * kWave;
+      if (own_slot && from < a.n)
+        own_slot = take(from, min(from + lane, a.n - 1), id_of(raws[j], a.wide, a.S), ws[j]);
+    });
+    if (!own_slot) return 0;
   }
   return count;
 }
@@ -299,16 +325,6 @@ __device__ __forceinline__ void add_whole_split(const Rows<W>& r, const u32x4 (&
   } else {
     acc = c;
   }
-}
-
-// f(0), f(1), ... f(N - 1) with compile-time arguments: arrays that they index stay in registers.
-template <class F, int... I>
-__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>()), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void each(F&& f) {
-  each(f, std::make_integer_sequence<int, N>());
 }
 
 // n units through D stages, D loads ahead of the computing. The loop's loads are unconditional,
@@ -648,9 +664,11 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_down_k(ExpertsArgs a) {
 }
 
 // More tokens: down projection of one expert for its pairs, 16 * TILES rows a wave, which share
-// what it loads of the columns. a.k_waves of the waves split the length of the same rows.
+// what it loads of the columns. a.k_waves of the waves split the length of the same rows. Two
+// workgroups a compute unit: for three the compiler spills (32 tokens, top-8 of 128, 2048 x 768
+// bf16 211 us, not 181).
 template <class W, bool ONCE, int WAVES, int TILES, int D>
-__global__ __launch_bounds__(WAVES* kWave, sizeof(W) == 1 ? 3 : 2) void experts_pairs_k(ExpertsArgs a) {
+__global__ __launch_bounds__(WAVES* kWave, 2) void experts_pairs_k(ExpertsArgs a) {
   constexpr int kThreads = WAVES * kWave, kRows = TILES * kTile;  // rows of a wave
   __shared__ Pairs list;
   __shared__ __attribute__((aligned(16))) union {

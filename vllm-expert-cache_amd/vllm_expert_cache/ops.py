@@ -35,6 +35,9 @@ MAX_TOP_K = 64
 MAX_EXPERTS = 1024  # of one routing
 MAX_GROUPS = 64
 MAX_RANK = 256
+MAX_TOKENS = 1 << 21   # of one routing or Adapters call
+MAX_OUTPUTS = 1 << 21  # of an adapter
+MAX_LENGTH = 1 << 24   # of a row of weights: H and I
 
 
 def _check(rc: int, name: str) -> None:
@@ -107,6 +110,8 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
         raise ValueError(f"scoring {scoring!r} (softmax or sigmoid), ids of {id_dtype} (int32 or "
                          f"int64)")
     T, E = logits.shape
+    if T > MAX_TOKENS:
+        raise ValueError(f"{T} tokens (at most {MAX_TOKENS})")
     if not 0 < E <= MAX_EXPERTS:
         raise ValueError(f"{E} experts (1 to {MAX_EXPERTS})")
     if not 1 <= groups <= MAX_GROUPS or E % groups or not 1 <= topk_groups <= groups:
@@ -169,6 +174,7 @@ class Experts:
         least = 16 if dtype in _BYTES else 8
         _need(H % least == 0 and (two // 2) % least == 0,
               f"H {H} and I {two // 2} must be multiples of {least}")
+        _need(max(H, two // 2) <= MAX_LENGTH, f"H {H} and I {two // 2} (at most {MAX_LENGTH})")
         for name, w in (("w13", w13), ("w2", w2)):
             _need(w.is_contiguous() and w.data_ptr() % 16 == 0,
                   f"{name} must be contiguous and 16-byte aligned")
@@ -199,7 +205,7 @@ class Experts:
         weight (float32 [T, top_k]) times the expert. slot_ids [T, top_k] are int32 or int64;
         T x top_k is at most 1024. A pair whose id is outside [0, S) or whose weight is 0 adds
         nothing (and an infinity in that expert does not show); a token without any other
-        pair gets zeros. `out`, if given, has contiguous rows and does not overlap x."""
+        pair gets zeros. `out`, if given, has contiguous rows and overlaps no other argument."""
         struct = self._structs.get(x.dtype)
         if struct is None or x.dim() != 2 or x.shape[1] != self.H or x.device != self.device:
             raise ValueError(f"x must be [T, {self.H}] on {self.device} of {self.dtypes}, not "
@@ -259,6 +265,8 @@ class Adapters:
               f"a {list(a.shape)} does not go with b {list(b.shape)}")
         _need(H % 8 == 0 and R % 8 == 0 and R <= MAX_RANK,
               f"H {H} and R {R} must be multiples of 8, R at most {MAX_RANK}")
+        _need(H <= MAX_LENGTH and b.shape[1] <= MAX_OUTPUTS,
+              f"H {H} (at most {MAX_LENGTH}) and {b.shape[1]} outputs (at most {MAX_OUTPUTS})")
         for name, w in (("a", a), ("b", b)):
             _need(w.is_contiguous() and w.data_ptr() % 16 == 0,
                   f"{name} must be contiguous and 16-byte aligned")
@@ -278,7 +286,7 @@ class Adapters:
         """base + scale * b[s] (a[s] x) for every token, s its slot id ([T], int32 or int64);
         x [T, H], base [T, O]. A token whose id is outside [0, S) has no adapter: its row is
         base's. `out` may be base, whose rows without an adapter are then not written; any
-        other `out` does not overlap base or x."""
+        other `out` overlaps no other argument."""
         dtype, device = self.dtype, self.device
         if x.dim() != 2 or x.shape[1] != self.H or x.dtype != dtype or x.device != device:
             raise ValueError(f"x must be {dtype} [T, {self.H}] on {device}, not {x.dtype} "
@@ -287,8 +295,9 @@ class Adapters:
         if base.shape != (T, self.O) or base.dtype != dtype or base.device != device:
             raise ValueError(f"base must be {dtype} [{T}, {self.O}] on {device}, not {base.dtype} "
                              f"{list(base.shape)} on {base.device}")
-        if slot_ids.shape != (T,):
-            raise ValueError(f"slot_ids must be [{T}], not {list(slot_ids.shape)}")
+        if slot_ids.shape != (T,) or T > MAX_TOKENS:
+            raise ValueError(f"slot_ids must be [{T}], not {list(slot_ids.shape)}, of at most "
+                             f"{MAX_TOKENS} tokens")
         ids, nbytes = _ids(slot_ids, device)
         x = _rows(x)
         if out is None:
