@@ -236,7 +236,8 @@ MoePlan moe_plan(int S, int H, int I, int T, int top_k) {
   p.splits = 1;
   // Workgroups that share their rows: as fill the device, a unit a wave at least. Shared / not: 16
   // tokens, top-8 of 64, 512 x 2048 bf16 113 / 174; one token on 2 experts, 1024 x 4096 bf16 15.8 /
-  // 16.4; on 8, 1024 x 512 13.0 / 12.3.
+  // 16.4; on 8, 1024 x 512 13.0 / 12.3. Up to twice as many are worth 9 % at best (one token, 4 of
+  // 1280 x 5120 bf16 39.4 / 35.9) and cost as much (int8, 2048 x 768, one token 13.9 / 15.3).
   if (p.few) {
     const int want = 256 / p.down_groups, most = (int)n * units / kDownWaves;
     p.splits = want < 2 || most < 2 ? 1 : want < most ? want : most;

@@ -9,6 +9,10 @@
 // orders of the same operations in 32 bits disagree about which of two near experts comes
 // first; in 64 bits the difference is far below what inputs of 32 bits can be apart, so that
 // key is a double. The weights of the few selected experts are computed in 64 bits too.
+// A token is a few hundred bytes, so a call is bound by one wave's chain of latencies: the row's
+// load, then k minima over the wave by DPP. One token of 128 experts, top-8 takes
+// 3.5 us in a graph where an empty launch takes 1.9; 60 tokens of 256 with groups and a bias 7.8,
+// for its keys of 64 bits and the groups' own rounds; 8192 tokens of 128 7.0.
 #pragma once
 #include "mfma.h"
 #include "wave.h"
