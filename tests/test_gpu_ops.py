@@ -679,3 +679,47 @@ def test_two_streams_at_once():
     for outs in got:
         for o in outs:
             assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("T", [20, 300])
+def test_many_tokens_captured_and_on_two_streams(T):
+    """The launches of more than 16 tokens of experts and more than 256 of adapters: replayed on
+    new inputs, and two at once. The last tokens are padding: no ids, and x that is no number."""
+    S, H, k = 12, 256, 3
+    e, l = _experts(T, S, H, 128, E4), _adapters(T, S, 24, H, H, BF16)
+    x, probs, ids = _tokens(T, T, k, S, H, BF16)
+    _, base, slots = _adapter_tokens(T, T, S, H, H, BF16, 30)
+    pad = T - 4
+    ids[pad:], slots[pad:], x[pad:] = -1, -1, float("nan")
+
+    def step():
+        return l(x, base, slots), e(x, probs, ids)
+
+    def check(got):
+        low, y = got
+        _close(low[:pad], *(v[:pad] for v in _adapt(l, x, base, slots)))
+        _close(y[:pad], *(v[:pad] for v in _moe(e, torch.nan_to_num(x), probs, ids)))
+        assert torch.equal(low[pad:], base[pad:]) and not y[pad:].any()
+
+    check(step())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        x[:pad].copy_(torch.randn((pad, H), device=DEV, generator=_gen(i)))
+        probs.copy_(torch.rand((T, k), device=DEV, generator=_gen(50 + i)))
+        ids[:pad] = ids[:pad].flip(0)
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        check(out)
+        assert all(torch.equal(a, b) for a, b in zip(out, eager)), i
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step())
+    torch.cuda.synchronize()
+    for pair in got:
+        assert all(torch.equal(a, b) for a, b in zip(pair, out))

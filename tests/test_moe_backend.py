@@ -98,6 +98,19 @@ def test_other_steps_go_to_the_stock_kernel(own_experts, kw):
     assert len(method.calls) == 1 and not own_experts
 
 
+@pytest.mark.parametrize("x,weights", [(torch.zeros(1, H + 8), torch.ones(1, 2)),
+                                       (torch.zeros(1, 1, H), torch.ones(1, 2)),
+                                       (torch.zeros(1, H), torch.ones(1, 2, 1))],
+                         ids=["padded", "batched", "weights"])
+def test_steps_of_other_shapes_go_to_the_stock_kernel(own_experts, x, weights):
+    layer = layer_of()
+    method = MoEMethod(layer)
+    assert armed(layer, method)[0]
+    layer._expert_cache.refresh = lambda i: i.clone()
+    method.apply(layer, x.bfloat16(), weights, torch.zeros(1, 2, dtype=torch.int32))
+    assert len(method.calls) == 1 and not own_experts
+
+
 @pytest.mark.parametrize("layer,method,reason", [
     (lambda: moe_layer(), lambda l: MoEMethod(l), "float32"),
     (lambda: layer_of(activation="gelu"), lambda l: MoEMethod(l), "gelu"),

@@ -258,7 +258,8 @@ def _plan(layer, method, logger):
 def _takes(experts: Experts | None, x, topk_weights, topk_ids, shared_experts) -> bool:
     """Whether a served step's arguments are ones that `experts` computes."""
     return (experts is not None and shared_experts is None and x.dim() == 2
-            and x.dtype in experts.dtypes and topk_weights.dtype == torch.float32
+            and x.shape[1] == experts.H and x.dtype in experts.dtypes
+            and topk_weights.dtype == torch.float32 and topk_weights.shape == topk_ids.shape
             and topk_ids.dim() == 2 and topk_ids.dtype in (torch.int32, torch.int64)
             and topk_ids.shape[1] <= MAX_TOP_K and topk_ids.numel() <= MAX_PAIRS)
 
