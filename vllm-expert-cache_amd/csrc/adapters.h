@@ -46,7 +46,7 @@ __device__ __forceinline__ int tile_slot(const AdaptersArgs& a, int t0) {
 // A's product for one tile and the adapters blockIdx.y, blockIdx.y + gridDim.y, ... of its
 // tokens that are an adapter's first, over one split of the hidden length: 16 * TILES ranks at
 // a time, which share what is loaded of the tokens. 33 tokens with an adapter each, rank 32, H
-// 4096: 7.3 us for 7.6 MB, of which the launch and one chain of loads are most.
+// 4096: 7.2 us for 7.6 MB, of which the launch and one chain of loads are most.
 template <class X, int WAVES, int TILES>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a) {
   constexpr int kRows = TILES * kTile, D = 2;
@@ -118,9 +118,11 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a
 }
 
 // B's product and the sum with the base for one tile, 16 outputs a wave: few, so that a tile has
-// many waves. AHEAD adapters of a tile are loaded at a time: 33 tokens, rank 64, H and O 4096,
-// an adapter each take 27.1 us one by one and 23.4 us four by four. With rank 32 the kernel
-// takes 6.4 us, three loads one behind another (id, values, B) and the launch.
+// many waves. Of the tile's adapters a workgroup takes every gridDim.z-th and writes the rows of
+// their tokens; the first one writes those without an adapter as well. AHEAD adapters are loaded
+// at a time: 33 tokens, rank 64, H and O 4096, an adapter each, all of a tile's in one workgroup,
+// take 27.1 us a call one by one and 23.4 us four by four. With rank 32 and four workgroups the
+// kernel takes 5.8 us: two chains of loads (ids, then values and B) and the launch.
 template <class X, int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a) {
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
@@ -128,16 +130,25 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
   const int t0 = blockIdx.x * kTile, token = t0 + column;
   const int row0 = (blockIdx.y * WAVES + wave) * kTile;
   if (row0 >= a.O) return;
-  const int id = tile_slot(a, t0);
+  int id = tile_slot(a, t0);
+  bool mine = id < 0 && blockIdx.z == 0 && a.base != a.out;
+  int which = 0;
+  for (unsigned left = (unsigned)ballot(id >= 0) & 0xFFFFu; left; ++which) {
+    const bool same = id == __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+    left &= ~(unsigned)ballot(same);
+    if (which % gridDim.z == blockIdx.z) mine |= same;
+  }
+  const bool write = token < a.T && mine;
+  if (ballot(write) == 0) return;
+  if (!mine) id = -1;  // another workgroup's
   const bool fast = a.aligned && row0 + kTile <= a.O;
-  const bool write = token < a.T && !(id < 0 && a.base == a.out);
   const int o0 = row0 + quarter * 4;
   const unsigned short* base = static_cast<const unsigned short*>(a.base) +
                                min(token, a.T - 1) * a.base_stride + o0;
-  unsigned short in[4];
-  if (fast) {
+  unsigned short in[4] = {};
+  if (write && fast) {
     __builtin_memcpy(in, __builtin_assume_aligned(base, 8), sizeof in);
-  } else {
+  } else if (write) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) in[i] = o0 + i < a.O ? base[i] : 0;
   }
@@ -147,9 +158,26 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
     const float scale = id < 0 ? 0.f : a.scales ? a.scales[id] : 1.f;
     for (int k0 = 0; k0 < a.R; k0 += 32) {
       const int k = k0 + quarter * 8;
-      const bool live = id >= 0 && k < a.R;
+      const unsigned at = (k < a.R ? k : 0) * 2u;
+      unsigned left = (unsigned)ballot(id >= 0) & 0xFFFFu;
+      int slot[AHEAD];
+      u32x4 w[AHEAD];
+      const auto load = [&]() EC_INLINE {
+        each<AHEAD>([&](auto n) EC_INLINE {
+          // (past the last adapter: the one before once more, for no column)
+          const bool more = n == 0 || left != 0;
+          const int s = more ? __builtin_amdgcn_readlane(id, __builtin_ctz(left | 1u << 31))
+                             : slot[n > 0 ? n - 1 : 0];
+          const int read = s < 0 ? 0 : s;
+          left &= ~(unsigned)ballot(id == s);
+          slot[n] = more ? s : -2;
+          w[n] = load16(static_cast<const char*>(a.b) +
+                        ((long long)read * a.O + row0) * (2LL * a.R) + (row + at));
+        });
+      };
+      load();  // under way while the tokens' values are joined
       f32x4 v0 = {0, 0, 0, 0}, v1 = v0;
-      if (live) {
+      if (id >= 0 && k < a.R) {
         const float* from = a.v + (long long)token * a.R + k;
 #pragma unroll 4
         for (int s = 0; s < a.splits; ++s) {
@@ -166,27 +194,14 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
         hi[i] = h0.v | (unsigned)h1.v << 16;
         lo[i] = l0.v | (unsigned)l1.v << 16;
       }
-      const unsigned at = (k < a.R ? k : 0) * 2u;
-      unsigned long long left = ballot(id >= 0) & 0xFFFFu;
-      while (left) {
-        int slot[AHEAD];
-        u32x4 w[AHEAD];
-        each<AHEAD>([&](auto n) EC_INLINE {
-          // (past the last adapter: the one before once more, for no column)
-          const bool more = n == 0 || left != 0;
-          const int s = more ? __builtin_amdgcn_readlane(id, __builtin_ctzll(left | 1ull << 32))
-                             : slot[n > 0 ? n - 1 : 0];
-          const int read = s < 0 ? 0 : s;
-          left &= ~ballot(id == s);
-          slot[n] = more ? s : -2;
-          w[n] = load16(static_cast<const char*>(a.b) +
-                        ((long long)read * a.O + row0) * (2LL * a.R) + (row + at));
-        });
+      for (;;) {
         each<AHEAD>([&](auto n) EC_INLINE {
           const f32x4 c = mfma_split<X>(keep(k < a.R, w[n]), 0, hi, lo, f32x4{0, 0, 0, 0});
 #pragma unroll
           for (int i = 0; i < 4; ++i) total[i] += id == slot[n] ? c[i] : 0.f;
         });
+        if (left == 0) break;
+        load();
       }
     }
   }
@@ -212,7 +227,7 @@ constexpr int kManyTiles = kManyTokens / kTile;
 // of the tokens and of A goes through LDS: from the L1 each wave would take the rows it shares
 // with the others for itself, and what a compute unit gets from its L1 (56 bytes/ns) is the
 // bound then. A wave has 32 of the ranks, 32 of the tokens and a part of each unit. 4096 tokens, H
-// 4096, rank 64, 7 adapters: 17.6 us for 33.5 MB of tokens, bound by the barriers of a unit and by
+// 4096, rank 64, 7 adapters: 18.0 us for 33.5 MB of tokens, bound by the barriers of a unit and by
 // workgroups whose tokens have two adapters. 32 ranks at a time for short ranks gain nothing
 // (rank 16 18.9 / 18.7, rank 32 35.6 / 36.3 us a call).
 template <class X>
@@ -326,7 +341,7 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
 // scaled and split into two bfloat16 once for the workgroup, in LDS. A wave has 64 outputs; the
 // rows of its instructions are interleaved so that a lane ends with two runs of eight neighbouring
 // outputs and the wave reads and writes 64 bytes of a token at a time. 4096 tokens, rank 64, O
-// 4096: 27.7 us for 67 MB read and written (2.4 TB/s), bound by the chain from ids over values and
+// 4096: 27.4 us for 67 MB read and written (2.4 TB/s), bound by the chain from ids over values and
 // split to the products, which 512 workgroups of eight waves overlap twice at most.
 template <class X, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersArgs a) {

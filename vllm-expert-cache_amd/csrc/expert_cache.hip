@@ -296,6 +296,11 @@ bool adapters_bad(const expert_cache_adapters* l, int T) {
 constexpr int kAdapterWaves = 4;
 // Up to this many tokens every adapter of a tile has workgroups of its own.
 constexpr int kAdapterFewTokens = 256;
+// Up to this many tiles of 16 tokens a tile's adapters are shared out to four workgroups of
+// adapters_expand_k. Four / one, us in a graph, H and O 4096: 16 tokens, rank 64, 64 adapters 14.8
+// / 20.6, two 13.8 / 15.2; 33 tokens, 64 adapters 21.0 / 24.6, two 19.4 / 16.0; 64 tokens, rank 16,
+// 64 adapters 13.4 / 13.5; but 128 tokens 21.9 / 18.0, 256 tokens 36 / 26.
+constexpr int kAdapterPartTiles = 4;
 
 // Workgroups that share the hidden length of a tile's product: as fill the device, a unit a wave
 // at least. Half as many for many tokens: 4096 tokens, rank 64 39.3 and not 37.7 us with one
@@ -316,6 +321,7 @@ int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
   if (few) {
     const int tiles = (a.T - 1) / kTile + 1;
     const dim3 shrink(tiles, kTile, a.splits);
+    const int parts = tiles <= kAdapterPartTiles ? 4 : 1;
     // as many ranks at a time as there are: 16 tokens, rank 16 one tile at a time 8.6 us, four 9.5;
     // rank 64 21.0 and 19.3; rank 32, two 11.8, one 13.0, four 12.7
     if (a.R <= 16)
@@ -326,7 +332,7 @@ int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
       hipLaunchKernelGGL((adapters_shrink_k<X, W, 4>), shrink, block, 0, stream, a);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    hipLaunchKernelGGL((adapters_expand_k<X, W, 4>), dim3(tiles, (a.O - 1) / (16 * W) + 1),
+    hipLaunchKernelGGL((adapters_expand_k<X, W, 4>), dim3(tiles, (a.O - 1) / (16 * W) + 1, parts),
                        block, 0, stream, a);
     return (int)hipGetLastError();
   }
