@@ -319,7 +319,8 @@ def _adapter_tokens(seed, T, S, H, O, dtype, run, id_dtype=torch.int32):
 @pytest.mark.parametrize("T,run,S,R,H,O", [
     (1, 1, 1, 8, 8, 1), (1, 1, 4, 16, 256, 64), (3, 1, 8, 8, 128, 17), (16, 1, 32, 32, 264, 130),
     (17, 2, 5, 24, 520, 63), (50, 9, 6, 64, 1048, 96), (200, 40, 3, 40, 64, 256),
-    (33, 1, 64, 256, 136, 48), (5, 1, 5, 16, 4104, 8)])
+    (33, 1, 64, 256, 136, 48), (5, 1, 5, 16, 4104, 8),
+    (7, 2, 4, 48, 72, 40), (16, 1, 20, 72, 136, 33), (40, 3, 9, 136, 200, 70)])
 def test_adapters(dtype, T, run, S, R, H, O):
     l = _adapters(T + R, S, R, H, O, dtype, scaled=T % 2 == 1)
     x, base, ids = _adapter_tokens(T, T, S, H, O, dtype, run,

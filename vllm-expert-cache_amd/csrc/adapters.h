@@ -43,76 +43,72 @@ __device__ __forceinline__ int tile_slot(const AdaptersArgs& a, int t0) {
   return t < a.T ? id : -1;
 }
 
-// A's product for one tile and the adapters blockIdx.y, blockIdx.y + gridDim.y, ... of its
-// tokens that are an adapter's first, over one split of the hidden length: 16 * TILES ranks at
-// a time, which share what is loaded of the tokens. 33 tokens with an adapter each, rank 32, H
-// 4096: 7.2 us for 7.6 MB, of which the launch and one chain of loads are most.
+// A's product for one tile and the adapter of its token blockIdx.y, if that is the adapter's
+// first, over one split of the hidden length and 16 * TILES ranks, which share what is loaded of
+// the tokens. 33 tokens with an adapter each, rank 32, H 4096: 7.2 us for 7.6 MB, of which the
+// launch and one chain of loads are most.
 template <class X, int WAVES, int TILES>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a) {
   constexpr int kRows = TILES * kTile, D = 2;
   __shared__ float red[WAVES][TILES][4][kWave];
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int t0 = blockIdx.x * kTile;
+  const int t0 = blockIdx.x * kTile, which = blockIdx.y;
   const int id = tile_slot(a, t0);
+  const int slot = __builtin_amdgcn_readlane(id, which);
+  const unsigned own = (unsigned)ballot(id == slot) & 0xFFFFu;
+  if (slot < 0 || __builtin_ctz(own) != which) return;
+  const int split = blockIdx.z % a.splits, r0 = blockIdx.z / a.splits * kRows;
   const int units = (a.H + kUnit - 1) / kUnit, per = (units + a.splits - 1) / a.splits;
-  const int first = blockIdx.z * per, count = min(units - first, per);
-  for (int which = blockIdx.y; which < kTile; which += gridDim.y) {
-    const int slot = __builtin_amdgcn_readlane(id, which);
-    const unsigned own = (unsigned)ballot(id == slot) & 0xFFFFu;
-    if (slot < 0 || __builtin_ctz(own) != which) continue;
-    // the columns of other adapters read what this one's first token has
-    const int token = t0 + (own >> column & 1 ? column : which);
-    const unsigned short* x = static_cast<const unsigned short*>(a.x) + token * a.x_stride;
-    for (int r0 = 0; r0 < a.R; r0 += kRows) {
-      const X* from = static_cast<const X*>(a.a) + ((long long)slot * a.R + r0) * a.H;
-      unsigned rows[TILES];
+  const int first = split * per, count = min(units - first, per);
+  // the columns of other adapters read what this one's first token has
+  const int token = t0 + (own >> column & 1 ? column : which);
+  const unsigned short* x = static_cast<const unsigned short*>(a.x) + token * a.x_stride;
+  const X* from = static_cast<const X*>(a.a) + ((long long)slot * a.R + r0) * a.H;
+  unsigned rows[TILES];
 #pragma unroll
-      for (int t = 0; t < TILES; ++t)
-        rows[t] = row_bytes<X>(r0 + t * kTile + column, r0, a.R, a.H);
-      f32x4 acc[TILES];
+  for (int t = 0; t < TILES; ++t)
+    rows[t] = row_bytes<X>(r0 + t * kTile + column, r0, a.R, a.H);
+  f32x4 acc[TILES];
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0, 0, 0, 0};
-      Rows<X> w[D][TILES];
-      u32x4 b[D][4];
-      pipeline<D>(
-          (count - wave + WAVES - 1) / WAVES,
-          [&](auto d, int i) EC_INLINE {
-            const int u = first + wave + i * WAVES;
-            each<TILES>([&](auto t) EC_INLINE {
-              w[d][t].load(from, rows[t], nullptr, u, a.H, quarter);
-            });
+  for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0, 0, 0, 0};
+  Rows<X> w[D][TILES];
+  u32x4 b[D][4];
+  pipeline<D>(
+      (count - wave + WAVES - 1) / WAVES,
+      [&](auto d, int i) EC_INLINE {
+        const int u = first + wave + i * WAVES;
+        each<TILES>([&](auto t) EC_INLINE {
+          w[d][t].load(from, rows[t], nullptr, u, a.H, quarter);
+        });
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              const int k = u * kUnit + operand_at<X>(f, quarter);
-              b[d][f] = load16(x + (k < a.H ? k : 0));
-            }
-          },
-          [&](auto d, int i) EC_INLINE {
-            const int u = first + wave + i * WAVES;
-            if ((u + 1) * kUnit > a.H) {
-              each<TILES>([&](auto t) EC_INLINE { w[d][t].cut(u, a.H, quarter); });
-#pragma unroll
-              for (int f = 0; f < 4; ++f)
-                b[d][f] = keep(u * kUnit + operand_at<X>(f, quarter) < a.H, b[d][f]);
-            }
-            each<TILES>([&](auto t) EC_INLINE { add_whole<X, X>(w[d][t], b[d], acc[t]); });
-          });
-      each<TILES>([&](auto t) EC_INLINE {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) red[wave][t][i][lane] = acc[t][i];
-      });
-      lds_sync();
-      for (int j = threadIdx.x; j < kRows * kTile; j += WAVES * kWave) {
-        const int r = j % kRows, col = j / kRows;
-        if (r0 + r < a.R && own >> col & 1) {
-          float y = 0;
-#pragma unroll
-          for (int w = 0; w < WAVES; ++w) y += red[w][r / kTile][r & 3][r % kTile / 4 * 16 + col];
-          a.v[((long long)blockIdx.z * a.T + t0 + col) * a.R + r0 + r] = y;
+        for (int f = 0; f < 4; ++f) {
+          const int k = u * kUnit + operand_at<X>(f, quarter);
+          b[d][f] = load16(x + (k < a.H ? k : 0));
         }
-      }
-      lds_sync();
+      },
+      [&](auto d, int i) EC_INLINE {
+        const int u = first + wave + i * WAVES;
+        if ((u + 1) * kUnit > a.H) {
+          each<TILES>([&](auto t) EC_INLINE { w[d][t].cut(u, a.H, quarter); });
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            b[d][f] = keep(u * kUnit + operand_at<X>(f, quarter) < a.H, b[d][f]);
+        }
+        each<TILES>([&](auto t) EC_INLINE { add_whole<X, X>(w[d][t], b[d], acc[t]); });
+      });
+  each<TILES>([&](auto t) EC_INLINE {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[wave][t][i][lane] = acc[t][i];
+  });
+  lds_sync();
+  for (int j = threadIdx.x; j < kRows * kTile; j += WAVES * kWave) {
+    const int r = j % kRows, col = j / kRows;
+    if (r0 + r < a.R && own >> col & 1) {
+      float y = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) y += red[w][r / kTile][r & 3][r % kTile / 4 * 16 + col];
+      a.v[((long long)split * a.T + t0 + col) * a.R + r0 + r] = y;
     }
   }
 }

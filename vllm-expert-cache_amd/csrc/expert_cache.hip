@@ -320,13 +320,17 @@ int launch_adapt(const AdaptersArgs& a, hipStream_t stream) {
   const dim3 block(W * kWave);
   if (few) {
     const int tiles = (a.T - 1) / kTile + 1;
-    const dim3 shrink(tiles, kTile, a.splits);
     const int parts = tiles <= kAdapterPartTiles ? 4 : 1;
-    // as many ranks at a time as there are: 16 tokens, rank 16 one tile at a time 8.6 us, four 9.5;
-    // rank 64 21.0 and 19.3; rank 32, two 11.8, one 13.0, four 12.7
-    if (a.R <= 16)
+    // Tiles of 16 ranks a workgroup takes at once, and workgroups that share the ranks. One / two
+    // / four tiles, us in a graph, H and O 4096: 16 tokens with 64 adapters, rank 16 8.6 / - / 9.5,
+    // rank 32 13.0 / 11.8 / 12.7, rank 64 13.1 / 13.2 / 15.1; one token, rank 64 9.6 / 9.6 / 11.6;
+    // but 64 tokens, 64 adapters 28.6 / 27.0 / 25.5. Ranks shared / one workgroup after another:
+    // one token, rank 256 24.4 / 34.8; 256 tokens, rank 256, 64 adapters 274 / 278.
+    const int rows = a.R <= 16 ? 1 : a.R <= 32 || (tiles == 1 && a.R <= 64) ? 2 : 4;
+    const dim3 shrink(tiles, kTile, a.splits * ((a.R - 1) / (16 * rows) + 1));
+    if (rows == 1)
       hipLaunchKernelGGL((adapters_shrink_k<X, W, 1>), shrink, block, 0, stream, a);
-    else if (a.R <= 32)
+    else if (rows == 2)
       hipLaunchKernelGGL((adapters_shrink_k<X, W, 2>), shrink, block, 0, stream, a);
     else
       hipLaunchKernelGGL((adapters_shrink_k<X, W, 4>), shrink, block, 0, stream, a);
