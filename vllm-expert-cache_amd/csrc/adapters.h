@@ -45,7 +45,7 @@ __device__ __forceinline__ int tile_slot(const AdaptersArgs& a, int t0) {
 
 // A's product for one tile and the adapter of its token blockIdx.y, if that is the adapter's
 // first, over one split of the hidden length and 16 * TILES ranks, which share what is loaded of
-// the tokens. 33 tokens with an adapter each, rank 32, H 4096: 7.2 us for 7.6 MB, of which the
+// the tokens. 33 tokens with an adapter each, rank 32, H 4096: 6.8 us for 7.6 MB, of which the
 // launch and one chain of loads are most.
 template <class X, int WAVES, int TILES>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a) {
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a
 // their tokens; the first one writes those without an adapter as well. AHEAD adapters are loaded
 // at a time: 33 tokens, rank 64, H and O 4096, an adapter each, all of a tile's in one workgroup,
 // take 27.1 us a call one by one and 23.4 us four by four. With rank 32 and four workgroups the
-// kernel takes 5.8 us: two chains of loads (ids, then values and B) and the launch.
+// kernel takes 5.6 us: two chains of loads (ids, then values and B) and the launch.
 template <class X, int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a) {
   const int lane = __lane_id(), quarter = lane >> 4, column = lane & 15;
@@ -223,7 +223,7 @@ constexpr int kManyTiles = kManyTokens / kTile;
 // of the tokens and of A goes through LDS: from the L1 each wave would take the rows it shares
 // with the others for itself, and what a compute unit gets from its L1 (56 bytes/ns) is the
 // bound then. A wave has 32 of the ranks, 32 of the tokens and a part of each unit. 4096 tokens, H
-// 4096, rank 64, 7 adapters: 18.0 us for 33.5 MB of tokens, bound by the barriers of a unit and by
+// 4096, rank 64, 7 adapters: 17.7 us for 33.5 MB of tokens, bound by the barriers of a unit and by
 // workgroups whose tokens have two adapters. 32 ranks at a time for short ranks gain nothing
 // (rank 16 18.9 / 18.7, rank 32 35.6 / 36.3 us a call).
 template <class X>
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
 // scaled and split into two bfloat16 once for the workgroup, in LDS. A wave has 64 outputs; the
 // rows of its instructions are interleaved so that a lane ends with two runs of eight neighbouring
 // outputs and the wave reads and writes 64 bytes of a token at a time. 4096 tokens, rank 64, O
-// 4096: 27.4 us for 67 MB read and written (2.4 TB/s), bound by the chain from ids over values and
+// 4096: 27.7 us for 67 MB read and written (2.4 TB/s), bound by the chain from ids over values and
 // split to the products, which 512 workgroups of eight waves overlap twice at most.
 template <class X, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersArgs a) {
