@@ -14,8 +14,8 @@ import pytest
 import torch
 
 import gpu_util as gu
-from test_gpu_ops import (E4, HALF, I8, KINDS, SPLIT, TINY, _close, _gamma, _gen, _tokens,
-                          _weights, _whole)
+from test_gpu_ops import (BF16, E4, F16, HALF, I8, KINDS, SPLIT, TINY, _adapter_tokens, _close,
+                          _gamma, _gen, _tokens, _weights, _whole)
 from vllm_expert_cache import ops
 
 pytestmark = pytest.mark.gpu
@@ -106,3 +106,57 @@ def test_experts_of_few_tokens(dtype, kind, T, k, S, H, I):
 ])
 def test_experts_of_more_tokens(dtype, kind, T, k, S, H, I):
     _check(T + H, T, k, S, _fit(H, kind), _fit(I, kind), dtype, kind)
+
+
+# ---- adapters -----------------------------------------------------------------------------
+
+def _adapters(seed, S, R, H, O, dtype):
+    g = _gen(seed)
+    return ops.Adapters(_small(g, (S, R, H), 6, dtype, 2.0 ** -6),
+                        (torch.randn((S, O, R), device=DEV, generator=g) * R ** -0.5).to(dtype),
+                        0.5 + torch.rand(S, device=DEV, generator=g))
+
+
+def _adapt(l, x, base, ids):
+    """(output, bound) where A's sums are exact, slot by slot."""
+    y, size = base.double().clone(), torch.zeros(base.shape, dtype=torch.float64, device=DEV)
+    for s in torch.unique(ids[(ids >= 0) & (ids < l.S)]).tolist():
+        t = torch.nonzero(ids == s)[:, 0]
+        v = (x[t].double() @ l.a[s].double().t().contiguous()) * l.scales[s].double()
+        b = l.b[s].double().t().contiguous()
+        y.index_add_(0, t, v @ b)
+        size.index_add_(0, t, v.abs() @ b.abs())
+    err = (_gamma(2 * l.R + 8) + SPLIT) * size * 1.01
+    return y, err + HALF[x.dtype] * (y.abs() + err) + TINY[x.dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,run,S,R,H,O", [
+    (2100, 25, 6, 72, 2056, 40),    # two or three units a workgroup
+    (2100, 200, 6, 16, 4104, 136),  # four or five
+    (4096, 30, 9, 64, 4096, 72),    # eight
+    (4160, 90, 5, 136, 4104, 40),   # eight or nine, three lots of ranks
+    (8200, 100, 4, 24, 4104, 24),   # 33, all of a row
+])
+def test_adapters_of_many_tokens(dtype, T, run, S, R, H, O):
+    l = _adapters(T + R, S, R, H, O, dtype)
+    _, base, ids = _adapter_tokens(T, T, S, 8, O, dtype, run)
+    x = _small(_gen(T + 1), (T, H), 2, dtype)
+    y = l(x, base, ids)
+    _close(y, *_adapt(l, x, base, ids))
+    none = ids < 0
+    assert none.any() and torch.equal(y[none], base[none])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,run,S,R,H,O", [
+    (1, 1, 2, 16, 65544, 72),    # one split a unit and wave
+    (256, 3, 5, 8, 65544, 24),   # four units a wave, and five
+    (250, 90, 3, 40, 81928, 8),
+])
+def test_adapters_of_long_rows(dtype, T, run, S, R, H, O):
+    l = _adapters(T + R, S, R, H, O, dtype)
+    _, base, ids = _adapter_tokens(T, T, S, 8, O, dtype, run)
+    ids[0] = 1
+    x = _small(_gen(T + 1), (T, H), 2, dtype)
+    _close(l(x, base, ids), *_adapt(l, x, base, ids))
