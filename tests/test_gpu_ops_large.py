@@ -160,3 +160,35 @@ def test_adapters_of_long_rows(dtype, T, run, S, R, H, O):
     ids[0] = 1
     x = _small(_gen(T + 1), (T, H), 2, dtype)
     _close(l(x, base, ids), *_adapt(l, x, base, ids))
+
+# ---- values of two bfloat16 ---------------------------------------------------------------
+
+# 1 + 2^-8 is two bfloat16 (a tie: 1 and 2^-8), 1 + 7 * 2^-10 a float16 that is none. Eight of
+# their products are 8 + 88 * 2^-10 + 56 * 2^-18, and ODD lifts that over the middle of two float16
+# at 8 + 92 * 2^-10, which it does not reach without the last term. All products are multiples of
+# 2^-18 and their sums below 2^4: exact in 32 bits in any order, so the result is exact, too.
+LOW, ODD, WIDE, SUM = 1 + 2.0 ** -8, 2.0 ** -8 - 2.0 ** -13, 1 + 7 * 2.0 ** -10, 8 + 96 * 2.0 ** -10
+
+
+@pytest.mark.parametrize("T", [1, 2, 20, 300])
+def test_float16_experts_take_both_halves_of_a_value(T):
+    w13 = torch.zeros((1, 64, 16), dtype=F16, device=DEV)
+    w13[0, :9, 0] = 64.0                 # SiLU of 64 is 64 in 32 bits
+    w13[0, 32:40, 1], w13[0, 40, 1] = LOW, ODD
+    w2 = torch.zeros((1, 16, 32), dtype=F16, device=DEV)
+    w2[0, :, :8], w2[0, :, 8] = WIDE, 1.0
+    x = torch.zeros((T, 16), dtype=F16, device=DEV)
+    x[:, :2] = 1.0
+    y = ops.Experts(w13, w2)(x, torch.full((T, 1), 2.0 ** -6, device=DEV),
+                             torch.zeros((T, 1), dtype=torch.int32, device=DEV))
+    assert (y == SUM).all()
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+def test_float16_adapters_take_both_halves_of_a_value(T):
+    a = torch.eye(8, dtype=F16, device=DEV)[None].contiguous()
+    b = torch.full((1, 24, 8), WIDE, dtype=F16, device=DEV)
+    x = torch.full((T, 8), LOW, dtype=F16, device=DEV)
+    base = torch.full((T, 24), ODD, dtype=F16, device=DEV)
+    y = ops.Adapters(a, b)(x, base, torch.zeros(T, dtype=torch.int32, device=DEV))
+    assert (y == SUM).all()

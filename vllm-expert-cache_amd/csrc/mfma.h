@@ -168,7 +168,9 @@ __device__ __forceinline__ f32x4 mfma_split(u32x4 w, int part, u32x4 hi, u32x4 l
   if constexpr (sizeof(W) == 2 && !__is_same(W, Bf16)) {
     u32x4 wh, wl;
     split_f16(w, wh, wl);
-    acc = B::mfma(wl, hi, acc);  // wl * lo is below 2^-16 of the product
+    // wl * lo is up to 2^-15 of the product, more than what lo itself is off by
+    acc = B::mfma(wl, lo, acc);
+    acc = B::mfma(wl, hi, acc);
     acc = B::mfma(wh, lo, acc);
     return B::mfma(wh, hi, acc);
   } else {
