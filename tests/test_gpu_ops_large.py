@@ -83,10 +83,11 @@ def _fit(length, kind):
 @pytest.mark.parametrize("dtype,kind", KINDS)
 @pytest.mark.parametrize("T,k,S,H,I", [
     (1, 2, 4, 4096, 1032),      # 16 rows a workgroup, two experts
-    (4, 8, 20, 4104, 392),      # the same, an expert after another in a wave, a part of a tile
+    (4, 8, 20, 3992, 392),      # the same, an expert after another in a wave, a part of a tile
+    (4, 8, 20, 4104, 392),      # 8 rows a workgroup
     (8, 2, 3, 4360, 264),       # two to four tokens an expert and more
-    (1, 8, 16, 2056, 776),      # 8 rows a workgroup, four units a wave up
-    (8, 8, 24, 2056, 520),
+    (1, 8, 16, 2040, 776),      # four units a wave up
+    (8, 8, 24, 2056, 520),      # 16 rows again
     (2, 4, 6, 520, 4104),       # workgroups that share a length
     (16, 4, 12, 2056, 1032),    # nine and more tokens, at most 2^22 weights
 ])

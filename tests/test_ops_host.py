@@ -163,6 +163,21 @@ def test_workspaces_cover_what_is_written(lib):
                                                 ctypes.addressof(size)) == 0
         assert size.value >= 4 * T * R
 
+@pytest.mark.parametrize("H,rows", [(32, 8), (2048, 8), (2064, 16), (2816, 16), (4080, 16),
+                                    (4096, 16), (4112, 8), (6144, 8), (6160, 16), (8192, 16),
+                                    (8208, 8), (14336, 8)])
+def test_rows_of_a_workgroup_down(lib, H, rows):
+    """Down projections of a few tokens: 16 rows a workgroup, or 8 where the fullest of 256 compute
+    units then has fewer rows. The workspace has a counter of 4 bytes a workgroup (and, where
+    several share their rows, 16 x rows floats each)."""
+    fullest = {r: -(-(-(-H // r)) // 256) * r for r in (8, 16)}
+    assert rows == (8 if fullest[8] < fullest[16] else 16)
+    size = ctypes.c_long()
+    e = _layer(H=H, I=16)
+    assert lib.expert_cache_moe_workspace(ctypes.addressof(e), 1, 1, ctypes.addressof(size)) == 0
+    groups = -(-H // rows)
+    assert size.value == 4 * 16 + 64 * rows * groups + 48 + 4 * groups
+
 
 # ---- Python -------------------------------------------------------------------------------
 

@@ -204,10 +204,17 @@ constexpr long kFewWeights = 1 << 22;
 // Up to 8 tokens few is the better one or close: 8 tokens, few / not: top-8 of 64, 2048 x 768 int8
 // 46 / 51; 2048 x 1408 bf16 124 / 139; top-2 of 8, 4096 x 7168 bf16 216 / 201.
 constexpr int kAlwaysFew = 8;
-// A workgroup of experts_down_k takes 8 rows where that makes 512 workgroups at most, else 16:
-// 8 / 16 rows: one token on 8 int8 experts, H 2048 14.1 / 15.6; on 8 fp8 experts, H 7168 62.1 /
-// 59.8.
-constexpr int kRowGroups = 510;
+// Compute units of the device.
+constexpr int kUnits = 256;
+// A workgroup of experts_down_k takes 16 rows, or 8 where the compute unit with the most rows then
+// has fewer: a unit's workgroups run side by side, so the call lasts as long as the fullest unit.
+// 8 / 16 rows, one token on 2 bf16 experts of H x 2048, us: H 2048 (8 rows a unit, or 16) 14.5 /
+// 16.5; 4112 (24 or 32) to 6144 3-9 % for 8 rows (5120 27.6 / 29.3). As many either way, 16 rows
+// read longer runs: 3584 (16) 21.5 / 21.2, 7168 (32) 34.6 / 34.9; with 4 tokens on 16 int8 experts
+// 71.9 / 67.8 and 126.8 / 120.9.
+bool eight_rows(int H) {
+  return (H - 1) / 8 / kUnits * 8 + 8 < (H - 1) / 16 / kUnits * 16 + 16;
+}
 // Down projection of more tokens: the waves of a workgroup share a row's length only as far as
 // rows alone do not make this many workgroups. Each for itself / four together: 32 tokens, top-8
 // of 64, 2048 x 512 int8 (512 workgroups) 56 / 64; 2048 x 1408 bf16 184 / 192; but 64 tokens, top-4
@@ -231,7 +238,7 @@ MoePlan moe_plan(int S, int H, int I, int T, int top_k) {
   while (p.k_waves < 4 && 2 * p.k_waves <= units &&
          all * ((H - 1) / (kPairRows * (4 / p.k_waves)) + 1) < kPairGroups)
     p.k_waves *= 2;
-  p.groups = p.few ? (H <= 8 * kRowGroups ? 1 : 2) : 2 * kPairTiles * (4 / p.k_waves);
+  p.groups = p.few ? (eight_rows(H) ? 1 : 2) : 2 * kPairTiles * (4 / p.k_waves);
   p.down_groups = (H - 1) / (8 * p.groups) + 1;
   p.splits = 1;
   // Workgroups that share their rows: as fill the device, a unit a wave at least. Shared / not: 16
@@ -239,7 +246,7 @@ MoePlan moe_plan(int S, int H, int I, int T, int top_k) {
   // 16.4; on 8, 1024 x 512 13.0 / 12.3. Up to twice as many are worth 9 % at best (one token, 4 of
   // 1280 x 5120 bf16 39.4 / 35.9) and cost as much (int8, 2048 x 768, one token 13.9 / 15.3).
   if (p.few) {
-    const int want = 256 / p.down_groups, most = (int)n * units / kDownWaves;
+    const int want = kUnits / p.down_groups, most = (int)n * units / kDownWaves;
     p.splits = want < 2 || most < 2 ? 1 : want < most ? want : most;
   }
   p.lo = 2 * n * I;
