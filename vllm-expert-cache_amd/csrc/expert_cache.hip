@@ -204,8 +204,7 @@ constexpr long kFewWeights = 1 << 22;
 // Up to 8 tokens few is the better one or close: 8 tokens, few / not: top-8 of 64, 2048 x 768 int8
 // 46 / 51; 2048 x 1408 bf16 124 / 139; top-2 of 8, 4096 x 7168 bf16 216 / 201.
 constexpr int kAlwaysFew = 8;
-// Compute units of the device.
-constexpr int kUnits = 256;
+constexpr int kComputeUnits = 256;
 // A workgroup of experts_down_k takes 16 rows, or 8 where the compute unit with the most rows then
 // has fewer: a unit's workgroups run side by side, so the call lasts as long as the fullest unit.
 // 8 / 16 rows, one token on 2 bf16 experts of H x 2048, us: H 2048 (8 rows a unit, or 16) 14.5 /
@@ -213,7 +212,7 @@ constexpr int kUnits = 256;
 // read longer runs: 3584 (16) 21.5 / 21.2, 7168 (32) 34.6 / 34.9; with 4 tokens on 16 int8 experts
 // 71.9 / 67.8 and 126.8 / 120.9.
 bool eight_rows(int H) {
-  return (H - 1) / 8 / kUnits * 8 + 8 < (H - 1) / 16 / kUnits * 16 + 16;
+  return (H - 1) / 8 / kComputeUnits * 8 + 8 < (H - 1) / 16 / kComputeUnits * 16 + 16;
 }
 // Down projection of more tokens: the waves of a workgroup share a row's length only as far as
 // rows alone do not make this many workgroups. Each for itself / four together: 32 tokens, top-8
@@ -246,7 +245,7 @@ MoePlan moe_plan(int S, int H, int I, int T, int top_k) {
   // 16.4; on 8, 1024 x 512 13.0 / 12.3. Up to twice as many are worth 9 % at best (one token, 4 of
   // 1280 x 5120 bf16 39.4 / 35.9) and cost as much (int8, 2048 x 768, one token 13.9 / 15.3).
   if (p.few) {
-    const int want = kUnits / p.down_groups, most = (int)n * units / kDownWaves;
+    const int want = kComputeUnits / p.down_groups, most = (int)n * units / kDownWaves;
     p.splits = want < 2 || most < 2 ? 1 : want < most ? want : most;
   }
   p.lo = 2 * n * I;
@@ -301,7 +300,14 @@ bool adapters_bad(const expert_cache_adapters* l, int T) {
 }
 
 constexpr int kAdapterWaves = 4;
-// Up to this many tokens every adapter of a tile has workgroups of its own.
+// Up to this many tokens (few) every adapter of a tile of 16 has workgroups of its own; above
+// (many) 64 tokens go through their adapters one after another. Few reads an adapter once a tile,
+// many works through a tile of 64 once an adapter, and how many adapters a tile has is on the
+// device only. Few / many, us in a graph, H and O 4096, one adapter and 64: 64 tokens, rank 16 9.4 /
+// 15.0 and 13.2 / 142; 256 tokens, rank 16 17.2 / 15.7 and 24 / 142, rank 64 33 / 18.3 and 76 / 191;
+// 320 tokens, rank 16 16.8 / 16.0 and 32 / 142, rank 64 40 / 19.0 and 97 / 189; 1024 tokens, rank 16
+// 32 / 18.6 and 76 / 146, rank 64 95 / 23 and 252 / 199. Steps of more than 256 tokens are prompts,
+// where neighbours share an adapter.
 constexpr int kAdapterFewTokens = 256;
 // Up to this many tiles of 16 tokens a tile's adapters are shared out to four workgroups of
 // adapters_expand_k. Four / one, us in a graph, H and O 4096: 16 tokens, rank 64, 64 adapters 14.8
