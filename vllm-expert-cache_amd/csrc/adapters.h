@@ -97,6 +97,7 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_shrink_k(AdaptersArgs a
         }
         each<TILES>([&](auto t) EC_INLINE { add_whole<X, X>(w[d][t], b[d], acc[t]); });
       });
+  products_done();
   each<TILES>([&](auto t) EC_INLINE {
 #pragma unroll
     for (int i = 0; i < 4; ++i) red[wave][t][i][lane] = acc[t][i];
@@ -196,6 +197,7 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
 #pragma unroll
           for (int i = 0; i < 4; ++i) total[i] += id == slot[n] ? c[i] : 0.f;
         });
+        settled(total);
         if (left == 0) break;
         load();
       }
@@ -308,6 +310,7 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
               });
             });
           });
+      products_done();
       lds_sync();
       if (part) {
         each<2>([&](auto r) EC_INLINE {
@@ -449,6 +452,7 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersA
         each<N>([&](auto n) EC_INLINE {
 #pragma unroll
           for (int i = 0; i < 4; ++i) total[c][n][i] += mine ? sum[n][i] : 0.f;
+          settled(total[c][n]);
         });
       });
     }

@@ -275,6 +275,7 @@ struct PackedSum {
         const f32x4 v = pick(t[0], t[1]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[g][0][i] = fmaf(r.s, v[i], c[g][0][i]);
+        settled(c[g][0]);
       } else {
         c[g][0] = t[0];
         c[g][1 % kApart] = t[1];
@@ -309,6 +310,7 @@ __device__ __forceinline__ void add_whole(const Rows<W>& r, const u32x4 (&cols)[
   if constexpr (__is_same(W, E4m3)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = fmaf(r.s, c[i], acc[i]);
+    settled(acc);
   } else {
     acc = c;
   }
@@ -322,6 +324,7 @@ __device__ __forceinline__ void add_whole_split(const Rows<W>& r, const u32x4 (&
   if constexpr (__is_same(W, E4m3)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = fmaf(r.s, c[i], acc[i]);
+    settled(acc);
   } else {
     acc = c;
   }
@@ -452,6 +455,7 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_up_k(ExpertsArgs a) {
           pg.template add<X>(g[d]);
           pu.template add<X>(u[d]);
         });
+    products_done();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const f32x4 vg = pg.template total<4>(t), vu = pu.template total<4>(t);
@@ -503,6 +507,7 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_up_k(ExpertsArgs a) {
           add_whole<W, X>(g[d], b[d], vg);
           add_whole<W, X>(u[d], b[d], vu);
         });
+    products_done();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       red.whole[wave][0][i][lane] = vg[i];
@@ -632,6 +637,7 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_down_k(ExpertsArgs a) {
           if (++cu == units || i + 1 == end - first) {
             const unsigned p = pairs[ce], pair = column == 0 ? p & 0xFFFFu : p >> 16;
             const bool here = (column & 7) == 0 && quarter < 2 && pair != 0xFFFFu;
+            products_done();
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               f32x4 v = acc.template total<8>(g);
@@ -730,12 +736,12 @@ __global__ __launch_bounds__(WAVES* kWave, 2) void experts_pairs_k(ExpertsArgs a
             [&](auto d, int i) EC_INLINE {
               const int u = unit(i);
               each<TILES>([&](auto t) EC_INLINE { w[d][t].b = w[d][0].b; });
-              // all cuts before the first sum: with a branch between two tiles' sums, the block
-              // after it read the first one's result sooner than the matrix unit wrote it
+              // (all cuts before the first sum, so that no branch is between two tiles' sums)
               if ((u + 1) * kUnit > a.I)
                 each<TILES>([&](auto t) EC_INLINE { w[d][t].cut(u, a.I); });
               each<TILES>([&](auto t) EC_INLINE { acc[t].template add<Bf16>(w[d][t]); });
             });
+        products_done();
         each<TILES>([&](auto t) EC_INLINE {
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -779,6 +785,7 @@ __global__ __launch_bounds__(WAVES* kWave, 2) void experts_pairs_k(ExpertsArgs a
               }
               each<TILES>([&](auto t) EC_INLINE { add_whole_split<W>(w[d][t], b[d], v[t]); });
             });
+        products_done();
         each<TILES>([&](auto t) EC_INLINE {
 #pragma unroll
           for (int i = 0; i < 4; ++i) red.whole[wave][t][i][lane] = v[t][i];

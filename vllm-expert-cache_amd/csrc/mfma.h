@@ -180,6 +180,18 @@ __device__ __forceinline__ f32x4 mfma_split(u32x4 w, int part, u32x4 hi, u32x4 l
   }
 }
 
+// A product's result is in its registers eight wait states after it and nothing holds an earlier
+// read back: the compiler counts them, but (clang 22 of ROCm 7.2) not for the first instruction of
+// a block that two others lead to, and moves what reads a result behind a branch if one follows.
+// So where a branch does: settled() keeps what was made of a result in its product's block, and
+// products_done() stands before sums are read that products were added to up to a branch.
+__device__ __forceinline__ void settled(f32x4& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void products_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 7");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // ---- memory -------------------------------------------------------------------------------
 
 __device__ __forceinline__ u32x4 load16(const void* p) {
