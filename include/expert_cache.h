@@ -236,9 +236,10 @@ enum {
  *   weights float[T, top_k]: the selected experts' scores, divided by their sum where
  *           `renormalize` is not 0 (a sum of 0 gives weights of 0), times `scale`
  *   ids     int32 (id_bytes 4) or int64 (8) [T, top_k]
- * An expert whose logit or bias is NaN or -infinity is never selected and takes no part in
- * the softmax; places that no expert is left for get id -1 and weight 0. Where logits are
- * +infinity, they share the softmax.
+ * An expert whose logit or bias is NaN or -infinity is never selected. One whose logit is takes
+ * no part in the softmax either; a bias changes no score, its own expert's or others'. Places
+ * that no expert is left for get id -1 and weight 0. Where logits are +infinity, they share the
+ * softmax, and all other scores are 0.
  * Fails with -1 unless 0 <= T <= 2^21, 0 < E <= 1024, row_stride >= E or T <= 1, type in 0-2,
  * scoring in {0, 1}, groups in 1..64 divides E, 0 < topk_groups <= groups,
  * 0 < top_k <= min(64, topk_groups * E / groups), id_bytes is 4 or 8, and no array but

@@ -99,8 +99,9 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     renormalize  divide the selected scores by their sum
     scale   factor on the weights
 
-    Among equals the lowest id comes first. Experts whose logit is NaN or -inf are never
-    selected; where too few are left the id is -1 and the weight 0."""
+    Among equals the lowest id comes first. Experts whose logit or bias is NaN or -inf are never
+    selected (one that a bias excludes still counts in the softmax); where too few are left the
+    id is -1 and the weight 0. Selected scores that are all 0 give weights of 0."""
     kind = _LOGITS.get(logits.dtype)
     if kind is None or logits.dim() != 2:
         raise ValueError(f"logits must be float32, bfloat16 or float16 [T, E], not {logits.dtype} "
