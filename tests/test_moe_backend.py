@@ -160,3 +160,20 @@ def test_packed_weights_keep_the_stock_kernel(own_experts):
     ok, log = armed(layer, method)
     assert ok and log.has("packed")
     assert generic.settings.moe
+
+
+@pytest.mark.parametrize("kw", [dict(x=True), dict(weights=True)], ids=["x", "weights"])
+def test_steps_that_need_a_gradient_go_to_the_stock_kernel(own_experts, kw):
+    layer = layer_of()
+    method = MoEMethod(layer)
+    assert armed(layer, method)[0]
+    layer._expert_cache.refresh = lambda i: i.clone()
+    x, weights = torch.randn(1, H).bfloat16(), torch.ones(1, 2)
+    x.requires_grad_("x" in kw)
+    weights.requires_grad_("weights" in kw)
+    ids = torch.zeros(1, 2, dtype=torch.int32)
+    method.apply(layer, x, weights, ids)
+    assert len(method.calls) == 1 and not own_experts
+    with torch.no_grad():
+        method.apply(layer, x, weights, ids)
+    assert len(method.calls) == 1 and len(own_experts) == 1

@@ -321,3 +321,56 @@ def test_what_is_too_long_is_refused(anywhere):
     with pytest.raises(ValueError):
         ops.Adapters(*_ab(H=8, O=1))(torch.empty(T, 8, dtype=BF16), torch.empty(T, 1, dtype=BF16),
                                      torch.empty(T, dtype=torch.int32))
+
+
+@pytest.fixture
+def no_kernels(anywhere, monkeypatch):
+    """Calls that every check lets through, without a device."""
+    calls = []
+    monkeypatch.setattr(ops, "_on_device", lambda device, call, *args: calls.append(args) or 0)
+    return calls
+
+
+GRAD_CALLS = {
+    "route": (lambda t: ops.route(t["logits"], 2, bias=t["bias"]), ("logits", "bias")),
+    "experts": (lambda t: ops.Experts(t["w13"], t["w2"], t["s13"], t["s2"])(t["x"], t["p"], t["i"]),
+                ("s13", "s2", "x", "p")),
+    "bf16": (lambda t: ops.Experts(t["v13"], t["v2"])(t["x"], t["p"], t["i"], out=t["out"]),
+             ("v13", "v2", "x", "p", "out")),
+    "adapters": (lambda t: ops.Adapters(t["a"], t["b"], t["f"])(t["x"], t["base"], t["j"]),
+                 ("a", "b", "f", "x", "base")),
+    "out": (lambda t: ops.Adapters(t["a"], t["b"])(t["x"], t["base"], t["j"], out=t["low"]),
+            ("low",)),
+}
+
+
+def _grad_tensors():
+    w13, w2 = _w(dtype=I8)
+    v13, v2 = _w()
+    x, p, i = _call()
+    a, b = _ab()
+    _, base, j = _rows()
+    return dict(logits=torch.zeros(2, 8), bias=torch.zeros(8), w13=w13, w2=w2,
+                s13=torch.ones(2, 32), s2=torch.ones(2, 32), v13=v13, v2=v2, x=x, p=p, i=i,
+                out=torch.zeros(3, 32, dtype=BF16), a=a, b=b, f=torch.ones(2), base=base, j=j,
+                low=torch.zeros(3, 24, dtype=BF16))
+
+
+@pytest.mark.parametrize("op,name", [(op, n) for op, (_, names) in GRAD_CALLS.items()
+                                     for n in names])
+def test_what_needs_a_gradient_is_refused(no_kernels, op, name):
+    """A result without a graph would leave the gradient out without a word."""
+    t = _grad_tensors()
+    call = GRAD_CALLS[op][0]
+    call(t)
+    t[name].requires_grad_()
+    with pytest.raises(ValueError, match="backward"):
+        call(t)
+    assert len(no_kernels) == 1
+    with torch.no_grad():
+        call(t)
+    with torch.inference_mode():
+        call(t)
+    t[name] = t[name].detach()
+    call(t)
+    assert len(no_kernels) == 4

@@ -261,7 +261,8 @@ def _takes(experts: Experts | None, x, topk_weights, topk_ids, shared_experts) -
             and x.shape[1] == experts.H and x.dtype in experts.dtypes
             and topk_weights.dtype == torch.float32 and topk_weights.shape == topk_ids.shape
             and topk_ids.dim() == 2 and topk_ids.dtype in (torch.int32, torch.int64)
-            and topk_ids.shape[1] <= MAX_TOP_K and topk_ids.numel() <= MAX_PAIRS)
+            and topk_ids.shape[1] <= MAX_TOP_K and topk_ids.numel() <= MAX_PAIRS
+            and not (torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad)))
 
 
 def _serve_from_slots(layer, method, cache: ExpertSlotCache, slot_cfg,

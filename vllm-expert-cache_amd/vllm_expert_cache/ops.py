@@ -13,6 +13,8 @@ cache's slot tensors never move, so a handle over them stays good. Weights are u
 without another layout. Calls run on the current stream of the tensors' device, allocate only
 their result and a workspace through torch, and read nothing back, so they can be captured.
 
+There is no backward pass: with gradients enabled, a tensor that requires one is refused.
+
 ValueError names an argument that an operator does not take; nothing has run then.
 """
 from __future__ import annotations
@@ -85,6 +87,14 @@ def _on_gpu(*tensors) -> torch.device:
     return device
 
 
+def _no_gradient(*tensors) -> None:
+    """Refuses what autograd would have to record (checked only while it records)."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError(f"a tensor {list(t.shape)} requires a gradient and there is no backward "
+                             f"pass: detach it, or call under torch.no_grad()")
+
+
 def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
           bias: torch.Tensor | None = None, groups: int = 1, topk_groups: int = 1,
           renormalize: bool = True, scale: float = 1.0,
@@ -125,6 +135,8 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
                              not bias.is_contiguous()):
         raise ValueError(f"bias must be contiguous float32 [{E}], not {bias.dtype} "
                          f"{list(bias.shape)}")
+    if torch.is_grad_enabled():
+        _no_gradient(logits, bias)
     device = _on_gpu(logits, bias)
     step = logits.stride()
     if step[1] != 1 or step[0] < E:
@@ -221,6 +233,8 @@ class Experts:
         if not 1 <= k <= MAX_TOP_K or T * k > MAX_PAIRS:
             raise ValueError(f"{T} tokens x top_k {k} (top_k at most {MAX_TOP_K}, {MAX_PAIRS} in "
                              f"all)")
+        if torch.is_grad_enabled():
+            _no_gradient(x, topk_weights, out, self.w13, self.w2, self.w13_scale, self.w2_scale)
         ids, nbytes = _ids(slot_ids, self.device)
         if not topk_weights.is_contiguous():
             topk_weights = topk_weights.contiguous()
@@ -299,6 +313,8 @@ class Adapters:
         if slot_ids.shape != (T,) or T > MAX_TOKENS:
             raise ValueError(f"slot_ids must be [{T}], not {list(slot_ids.shape)}, of at most "
                              f"{MAX_TOKENS} tokens")
+        if torch.is_grad_enabled():
+            _no_gradient(x, base, out, self.a, self.b, self.scales)
         ids, nbytes = _ids(slot_ids, device)
         x = _rows(x)
         if out is None:
