@@ -278,8 +278,14 @@ int expert_cache_moe_workspace(const expert_cache_experts* e, int T, int top_k, 
  * element must not meet that of x, ids or topk_weights. ids (int32 or int64 by id_bytes) are
  * slot ids as expert_cache_refresh hands them out. A pair whose id is outside
  * [0, S) or whose weight is 0 adds nothing and reads no weights; a token without any other
- * pair gets zeros. All sums are in 32 bits, and only `out` is rounded to `type`. `workspace`
- * (16-byte aligned, expert_cache_moe_workspace bytes) is the call's own until it has run.
+ * pair gets zeros. Sums are in 32 bits. Hidden values go from one projection to the other as two
+ * bfloat16 each, within 2^-17 of the value (a float's own rounding is 2^-24), and `out` is rounded
+ * to `type`: results are as near the formula as with hidden values in 32 bits, but their last bit
+ * is more often another than that of sums in 32 bits throughout. The same call gives the same bits;
+ * the same token among others may not, as its sums may have another order. Outputs that an
+ * infinite hidden value or weight of w2 reaches are infinite or NaN, not always what the formula
+ * gives. `workspace` (16-byte aligned, expert_cache_moe_workspace bytes) is the call's own until it
+ * has run.
  * Fails with -1 unless the layer is as above, H and I are multiples of 8 (of 16 with one-byte
  * weights) and at most 2^24, 0 <= T, 0 < top_k <= 64, T * top_k <= 1024, id_bytes is 4 or 8,
  * and no array is null (unless T is 0).
@@ -308,8 +314,10 @@ int expert_cache_adapt_workspace(const expert_cache_adapters* l, int T, long* by
  * x [T, H], base [T, O] and out [T, O] are of the adapters' type, rows x_stride, base_stride
  * and out_stride elements apart, x 16-byte aligned with x_stride a multiple of 8. out is base
  * itself (same address and stride) or meets neither base nor x, and never ids. A token whose id
- * is outside [0, S) has no adapter: its row is base's, and is not written where out is base. All
- * sums are in 32 bits, and only `out` is rounded to `type`. `workspace` as for expert_cache_moe.
+ * is outside [0, S) has no adapter: its row is base's, and is not written where out is base. Sums
+ * are in 32 bits, `out` is rounded to `type`, and between the two products a[s] x_t times its
+ * factor is two bfloat16, with what expert_cache_moe says of those, of bits and of infinities.
+ * `workspace` as for expert_cache_moe.
  * Fails with -1 unless S > 0, 0 < O <= 2^21, H and R are positive multiples of 8, H <= 2^24,
  * R <= 256, 0 <= T <= 2^21, id_bytes is 4 or 8, and no array but `scales` is null (unless T is 0).
  */

@@ -172,8 +172,10 @@ class Experts:
     scales a 128 x 128 block, [S, ceil(2*I/128), ceil(H/128)] and [S, ceil(H/128), ceil(I/128)].
     H and I are multiples of 8, with one-byte weights of 16.
 
-    Activations are not quantised: one-byte weights are widened to the tokens' type, sums are
-    32-bit, and only the result is rounded."""
+    Activations are not quantised: one-byte weights are widened to the tokens' type and sums are
+    32-bit. Hidden values are rounded to two bfloat16 (2^-17 of the value), the result to its type.
+    The same call gives the same bits; a token's last bits may differ with the tokens beside it.
+    Infinite hidden values or weights of w2 make infinities or NaN of the outputs they reach."""
 
     def __init__(self, w13: torch.Tensor, w2: torch.Tensor, w13_scale: torch.Tensor | None = None,
                  w2_scale: torch.Tensor | None = None):
@@ -270,7 +272,8 @@ class Adapters:
     """Low-rank adapters in slots, added for every token to a projection that all share.
 
     a  [S, R, H], b  [S, O, R] in bfloat16 or float16; scales float32 [S] or None (1).
-    H and R are multiples of 8, R at most 256."""
+    H and R are multiples of 8, R at most 256. Sums are 32-bit; between the products a token's
+    values are rounded to two bfloat16, with what `Experts` says of those."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None):
         _need(a.dim() == 3 and b.dim() == 3 and a.dtype == b.dtype and a.dtype in _TOKENS,
