@@ -221,13 +221,14 @@ __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_k(AdaptersArgs a
 constexpr int kManyTokens = 64;  // of a workgroup of the kernels below: a lane each
 constexpr int kManyTiles = kManyTokens / kTile;
 
-// A's product for 64 tokens over one split of the hidden length, 64 ranks at a time. A unit
-// of the tokens and of A goes through LDS: from the L1 each wave would take the rows it shares
-// with the others for itself, and what a compute unit gets from its L1 (56 bytes/ns) is the
-// bound then. A wave has 32 of the ranks, 32 of the tokens and a part of each unit. 4096 tokens, H
-// 4096, rank 64, 7 adapters: 17.7 us for 33.5 MB of tokens, bound by the barriers of a unit and by
-// workgroups whose tokens have two adapters. 32 ranks at a time for short ranks gain nothing
-// (rank 16 18.9 / 18.7, rank 32 35.6 / 36.3 us a call).
+// A's product for 64 tokens over one split of the hidden length, 64 ranks at a time. A unit of
+// the tokens and of A goes through LDS: from the L1 each wave would take the rows it shares with
+// the others for itself, and what a compute unit gets from its L1 (56 bytes/ns) is the bound
+// then. A wave has 32 of the ranks, 32 of the tokens and a part of each unit. 4096 tokens, H
+// 4096, rank 64, 7 adapters: 18.6 us for 33.5 MB of tokens, one workgroup a compute unit (170
+// registers), bound by the barriers of a unit and by workgroups whose tokens have two adapters.
+// 32 ranks at a time for short ranks gain nothing (rank 16 18.9 / 18.7, rank 32 35.6 / 36.3 us a
+// call).
 template <class X>
 __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersArgs a) {
   constexpr int kRows = 64, D = 4;
@@ -340,8 +341,10 @@ __global__ __launch_bounds__(8 * kWave, 2) void adapters_shrink_many_k(AdaptersA
 // scaled and split into two bfloat16 once for the workgroup, in LDS. A wave has 64 outputs; the
 // rows of its instructions are interleaved so that a lane ends with two runs of eight neighbouring
 // outputs and the wave reads and writes 64 bytes of a token at a time. 4096 tokens, rank 64, O
-// 4096: 27.7 us for 67 MB read and written (2.4 TB/s), bound by the chain from ids over values and
-// split to the products, which 512 workgroups of eight waves overlap twice at most.
+// 4096: 28.0 us for 67 MB read and written (2.4 TB/s), bound by the chain from ids over values and
+// split to the products: at 212 registers a compute unit holds one workgroup, so the 512 of them
+// run in two rounds with nothing beside a chain. Float16 takes all 256 registers and 100 bytes of
+// scratch a lane, for weights in halves; the whole call takes 58 us and not 49.
 template <class X, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void adapters_expand_many_k(AdaptersArgs a) {
   constexpr int T = kManyTiles, N = 4, kRanks = 64;

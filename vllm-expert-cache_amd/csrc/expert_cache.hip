@@ -301,13 +301,13 @@ bool adapters_bad(const expert_cache_adapters* l, int T) {
 
 constexpr int kAdapterWaves = 4;
 // Up to this many tokens (few) every adapter of a tile of 16 has workgroups of its own; above
-// (many) 64 tokens go through their adapters one after another. Few reads an adapter once a tile,
-// many works through a tile of 64 once an adapter, and how many adapters a tile has is on the
-// device only. Few / many, us in a graph, H and O 4096, one adapter and 64: 64 tokens, rank 16 9.4 /
-// 15.0 and 13.2 / 142; 256 tokens, rank 16 17.2 / 15.7 and 24 / 142, rank 64 33 / 18.3 and 76 / 191;
-// 320 tokens, rank 16 16.8 / 16.0 and 32 / 142, rank 64 40 / 19.0 and 97 / 189; 1024 tokens, rank 16
-// 32 / 18.6 and 76 / 146, rank 64 95 / 23 and 252 / 199. Steps of more than 256 tokens are prompts,
-// where neighbours share an adapter.
+// (many) 64 tokens go through their adapters one after another. Few reads an adapter once a
+// tile, many works through a tile of 64 once an adapter, and how many adapters a tile has is on
+// the device only. Few / many, us in a graph, H and O 4096, one adapter and 64: 64 tokens, rank
+// 16 9.4 / 15.0 and 13.2 / 142; 256 tokens, rank 16 17.2 / 15.7 and 24 / 142, rank 64 33 / 18.3
+// and 76 / 191; 320 tokens, rank 16 16.8 / 16.0 and 32 / 142, rank 64 40 / 19.0 and 97 / 189;
+// 1024 tokens, rank 16 32 / 18.6 and 76 / 146, rank 64 95 / 23 and 252 / 199. Steps of more than
+// 256 tokens are prompts, where neighbours share an adapter.
 constexpr int kAdapterFewTokens = 256;
 // Up to this many tiles of 16 tokens a tile's adapters are shared out to four workgroups of
 // adapters_expand_k. Four / one, us in a graph, H and O 4096: 16 tokens, rank 64, 64 adapters 14.8

@@ -677,10 +677,10 @@ __global__ __launch_bounds__(WAVES* kWave) void experts_down_k(ExpertsArgs a) {
 }
 
 // More tokens: down projection of one expert for its pairs, 16 * TILES rows a wave, which share
-// what it loads of the columns. a.k_waves of the waves split the length of the same rows. Two
-// workgroups a compute unit: for three the compiler spills (32 tokens, top-8 of 128, 2048 x 768
-// bf16 211 us, not 181). 16 tokens on fp8 experts of 44 MB: 800 MB here in 152 us (5.3 TB/s),
-// bound by the latency of the one unit that a wave has under way.
+// what it loads of the columns. a.k_waves of the waves split the length of the same rows. At least
+// two workgroups a compute unit (168 to 254 registers): held to three the compiler spills (32
+// tokens, top-8 of 128, 2048 x 768 bf16 211 us, not 181). 16 tokens on fp8 experts of 44 MB: 800 MB
+// here in 143 us (5.6 TB/s), bound by the latency of the one unit that a wave has under way.
 template <class W, bool ONCE, int WAVES, int TILES, int D>
 __global__ __launch_bounds__(WAVES* kWave, 2) void experts_pairs_k(ExpertsArgs a) {
   constexpr int kThreads = WAVES * kWave, kRows = TILES * kTile;  // rows of a wave
