@@ -13,7 +13,8 @@ cache's slot tensors never move, so a handle over them stays good. Weights are u
 without another layout. Calls run on the current stream of the tensors' device, allocate only
 their result and a workspace through torch, and read nothing back, so they can be captured.
 
-There is no backward pass: with gradients enabled, a tensor that requires one is refused.
+There is no backward pass: with gradients enabled, a tensor that requires one (a handle's weights:
+when the handle is made) is refused.
 
 ValueError names an argument that an operator does not take; nothing has run then.
 """
@@ -88,11 +89,17 @@ def _on_gpu(*tensors) -> torch.device:
 
 
 def _no_gradient(*tensors) -> None:
-    """Refuses what autograd would have to record (checked only while it records)."""
+    """Refuses a call that autograd would have to record."""
     for t in tensors:
         if t is not None and t.requires_grad:
             raise ValueError(f"a tensor {list(t.shape)} requires a gradient and there is no backward "
                              f"pass: detach it, or call under torch.no_grad()")
+
+
+def _graded(*weights) -> list:
+    """A handle's weights that require a gradient: looked for once, since each look at a tensor
+    is a tenth of a microsecond of a call."""
+    return [w for w in weights if w is not None and w.requires_grad]
 
 
 def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
@@ -135,9 +142,9 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
                              not bias.is_contiguous()):
         raise ValueError(f"bias must be contiguous float32 [{E}], not {bias.dtype} "
                          f"{list(bias.shape)}")
-    if torch.is_grad_enabled():
-        _no_gradient(logits, bias)
     device = _on_gpu(logits, bias)
+    if torch.is_grad_enabled() and (logits.requires_grad or bias is not None):
+        _no_gradient(logits, bias)
     step = logits.stride()
     if step[1] != 1 or step[0] < E:
         logits, step = logits.contiguous(), (E, 1)
@@ -212,6 +219,7 @@ class Experts:
                              *[s.data_ptr() if s is not None else None
                                for s in (w13_scale, w2_scale)])
             self._structs[t] = (e, ctypes.addressof(e))
+        self._graded = _graded(w13, w2, w13_scale, w2_scale)
         self._bytes: dict = {}
 
     def __call__(self, x: torch.Tensor, topk_weights: torch.Tensor, slot_ids: torch.Tensor,
@@ -235,8 +243,9 @@ class Experts:
         if not 1 <= k <= MAX_TOP_K or T * k > MAX_PAIRS:
             raise ValueError(f"{T} tokens x top_k {k} (top_k at most {MAX_TOP_K}, {MAX_PAIRS} in "
                              f"all)")
-        if torch.is_grad_enabled():
-            _no_gradient(x, topk_weights, out, self.w13, self.w2, self.w13_scale, self.w2_scale)
+        if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or
+                                        self._graded or out is not None):
+            _no_gradient(x, topk_weights, out, *self._graded)
         ids, nbytes = _ids(slot_ids, self.device)
         if not topk_weights.is_contiguous():
             topk_weights = topk_weights.contiguous()
@@ -297,6 +306,7 @@ class Adapters:
                                      b.data_ptr(), scales.data_ptr() if scales is not None
                                      else None)
         self._at = ctypes.addressof(self._struct)
+        self._graded = _graded(a, b, scales)
         self._bytes: dict = {}
 
     def __call__(self, x: torch.Tensor, base: torch.Tensor, slot_ids: torch.Tensor,
@@ -316,8 +326,9 @@ class Adapters:
         if slot_ids.shape != (T,) or T > MAX_TOKENS:
             raise ValueError(f"slot_ids must be [{T}], not {list(slot_ids.shape)}, of at most "
                              f"{MAX_TOKENS} tokens")
-        if torch.is_grad_enabled():
-            _no_gradient(x, base, out, self.a, self.b, self.scales)
+        if torch.is_grad_enabled() and (x.requires_grad or base.requires_grad or self._graded or
+                                        out is not None):
+            _no_gradient(x, base, out, *self._graded)
         ids, nbytes = _ids(slot_ids, device)
         x = _rows(x)
         if out is None:
