@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import gpu_util as gu
+from test_gpu_ops import _close, _experts, _moe, _tokens
 from vllm_expert_cache import ops
 
 pytestmark = pytest.mark.gpu
@@ -166,6 +167,18 @@ def test_float16_weights_and_tokens_below_its_normal_numbers(T):
                                                                     device=DEV))
     want = tiny[0, :8, 5].double() * 2.0 ** 10 * 300 * 2.0 ** -24 * 2.0 ** 18
     assert torch.equal(y, want.to(F16).expand(T, 8))
+
+
+@pytest.mark.parametrize("T,k,S", [(16, 5, 3), (16, 5, 200), (9, 33, 20), (26, 5, 3), (26, 5, 200),
+                                   (200, 5, 4), (31, 33, 20), (31, 33, 1100)])
+def test_experts_named_twice_in_pairs_of_two_lots(T, k, S):
+    """Ids are gone through 64 at a time; here tokens begin in one lot and end in the next, name
+    slots twice or more, once with a weight of 0 first."""
+    e = _experts(T + k, S, 64, 48, BF16)
+    x, probs, ids = _tokens(T, T, k, S, 64, BF16)
+    ids[:, k - 1] = ids[:, 1]
+    probs[::3, 1] = 0.0
+    _close(e(x, probs, ids), *_moe(e, x, probs, ids))
 
 
 # ---- adapters -----------------------------------------------------------------------------
