@@ -210,8 +210,9 @@ constexpr int kComputeUnits = 256;
 // 8 / 16 rows, one token on 2 bf16 experts of H x 2048, us: H 2048 (8 rows a unit, or 16) 14.5 /
 // 16.5; 4112 (24 or 32) to 6144 3-9 % for 8 rows (5120 27.6 / 29.3). As many either way, 16 rows
 // read longer runs: 3584 (16) 21.5 / 21.2, 7168 (32) 34.6 / 34.9; with 4 tokens on 16 int8 experts
-// 71.9 / 67.8 and 126.8 / 120.9. Worst of 300 shapes up to H 16384: 4 tokens on 16 bf16 experts, 4080
-// x 7168 452 / 476 (16 taken).
+// 71.9 / 67.8 and 126.8 / 120.9. Most against the rule, of shapes up to H 16384: one token on 2
+// int8 experts, 8208 x 768 21.7 / 19.4 (8 taken); 4 tokens on 16 bf16 experts, 4080 x 7168 452 /
+// 476 (16 taken).
 bool eight_rows(int H) {
   return (H - 1) / 8 / kComputeUnits * 8 + 8 < (H - 1) / 16 / kComputeUnits * 16 + 16;
 }
