@@ -326,6 +326,114 @@ int expert_cache_adapt(const expert_cache_adapters* l, const void* x, long x_str
                        long base_stride, void* out, long out_stride, void* workspace,
                        hipStream_t stream);
 
+/*
+ * Pairs of token and slot, T x top_k of them (pair t * top_k + j is ids[t, j]), sorted by slot;
+ * those of a slot stay in their own order.
+ *   offsets int32[S + 1]     the first place of every slot's pairs; offsets[S] pairs have a slot
+ *   rows    int32[T * top_k] the pair at every place, -1 behind the last
+ *   places  int32[T, top_k]  the place of every pair, -1 where its id is outside [0, S)
+ * `workspace` (16-byte aligned, expert_cache_sort_workspace bytes, null where those are 0) is the
+ * call's own until it has run. The three results and ids must not meet.
+ * Fails with -1 unless 0 <= T, 0 < top_k <= 64, T * top_k <= 2^24, 0 < S <= 1024, id_bytes is 4 or
+ * 8, and no array is null (with T = 0: but offsets).
+ */
+int expert_cache_sort_workspace(int T, int top_k, int S, long* bytes);
+int expert_cache_sort(const void* ids, int id_bytes, int T, int top_k, int S, int* offsets,
+                      int* rows, int* places, void* workspace, hipStream_t stream);
+
+/*
+ * Rows in the order of expert_cache_sort: out[places[t, j]] = x[t], and zeros in the rows from
+ * offsets[S] on. x [T, H] and out [T * top_k, H] are of `type` (0-2), rows x_stride and out_stride
+ * elements apart. Places outside [0, T * top_k) are left out. The gradient of x is
+ * expert_cache_combine of out's without weights.
+ * Fails with -1 unless sizes are as for expert_cache_sort, 0 < H <= 2^20, strides are at least H
+ * (or there is one row), no array is null (unless T is 0), and out meets no other.
+ */
+int expert_cache_dispatch(const void* x, int type, long x_stride, const int* places,
+                          const int* offsets, int T, int top_k, int S, int H, void* out,
+                          long out_stride, hipStream_t stream);
+
+/*
+ * Back to the tokens: out[t] = sum_j weights[t, j] * y[places[t, j]], summed in 32 bits in the
+ * order of j and rounded to `type`. y [T * top_k, H], out [T, H]; weights float[T, top_k], or null
+ * for 1. A pair without a place or with a weight of 0 adds nothing. Fails with -1 as above.
+ */
+int expert_cache_combine(const void* y, int type, long y_stride, const float* weights,
+                         const int* places, int T, int top_k, int H, void* out, long out_stride,
+                         hipStream_t stream);
+
+/*
+ * Its gradients, from grad [T, H] of out:
+ *   dy[places[t, j]] = weights[t, j] * grad[t], zeros from offsets[S] on   [T * top_k, H]
+ *   dweights[t, j] = sum_h grad[t, h] * y[places[t, j], h], 0 without a place   float[T, top_k]
+ * One of the two may be null, and y then too if it is dweights. Neither may meet an input or the
+ * other. Fails with -1 as above.
+ */
+int expert_cache_combine_grad(const void* grad, int type, long grad_stride, const void* y,
+                              long y_stride, const float* weights, const int* places,
+                              const int* offsets, int T, int top_k, int S, int H, void* dy,
+                              long dy_stride, float* dweights, hipStream_t stream);
+
+/*
+ * Rows as 8-bit integers: m = max |x[t]|, scales[t] = m / 127, q[t] = 127 x[t] / m rounded to the
+ * nearest whole number, ties to the even one. x [T, H] of type BF16 or F16, rows x_stride elements
+ * apart; q int8 with rows q_stride bytes apart, 16-byte aligned with q_stride a multiple of 16, and
+ * zeros from H to the next multiple of 16. A row below 2^-119 throughout counts as zeros, scale 0;
+ * one with an infinity or NaN becomes zeros with a scale of NaN.
+ * Fails with -1 unless 0 <= T <= 2^24, 0 < H <= 2^20, strides hold a row (or there is one), no
+ * array is null (unless T is 0) and the results meet no other array.
+ */
+int expert_cache_quantize(const void* x, int type, long x_stride, int T, int H, void* q,
+                          long q_stride, float* scales, hipStream_t stream);
+
+/*
+ * A projection in 8-bit integers: w int8 [O, H], rows w_stride bytes apart, 16-byte aligned with
+ * w_stride a multiple of 16, and zeros from H to the next multiple of 16; scale float[O]; bias
+ * float[O] or null.
+ */
+typedef struct expert_cache_linear {
+  int O, H;
+  long w_stride;
+  const void* w;
+  const float* scale;
+  const float* bias;
+} expert_cache_linear;
+
+/* Bytes of workspace that expert_cache_linear8 needs, into *bytes. */
+int expert_cache_linear8_workspace(const expert_cache_linear* l, int type, int T, long* bytes);
+
+/*
+ * out[t, o] = x_scales[t] * scale[o] * sum_h x[t, h] w[o, h] + bias[o], the sum exact. x [T, H] is
+ * of type BF16 or F16 and quantised by the call as expert_cache_quantize does it (x_scales is not
+ * read then), or INT8 with x_scales float[T], laid out like expert_cache_quantize's q (what is
+ * behind H may be anything). out [T, O] is of out_type (0-2). `workspace` as for expert_cache_moe.
+ * Fails with -1 unless 0 < H <= 131056, 0 < O <= 2^24, 0 <= T <= 2^24, strides hold a row (or there
+ * is one) and those of 8-bit rows are at most 2^22, no array is null but as said (unless T is 0),
+ * and out meets neither x nor x_scales.
+ */
+int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, long x_stride,
+                         const float* x_scales, int T, void* out, int out_type, long out_stride,
+                         void* workspace, hipStream_t stream);
+
+/*
+ * A mixture-of-experts layer in 8-bit integers, for any number of tokens, over slots of INT8
+ * weights (with their scales, as for expert_cache_moe; the formula and what ids and weights mean
+ * are also its):
+ *   both projections' inputs are quantised row by row as by expert_cache_quantize, the hidden
+ *   values from 32 bits; their products are exact, the rest is in 32 bits, and out [T, H] is
+ *   rounded to the layer's type. A token with an infinity or NaN gets NaN.
+ * Pairs are sorted by slot, so that a slot's weights serve all its pairs. The same call gives the
+ * same bits, and a token's do not depend on the tokens beside it.
+ * Fails with -1 unless the layer is as for expert_cache_moe with INT8 weights, S <= 1024, H and I
+ * are multiples of 16 and at most 131056, 2 * I * H and T * H are at most 1.75 * 2^30, sizes are
+ * otherwise as for expert_cache_sort, strides hold a row (or there is one), id_bytes is 4 or 8, no array is null
+ * (unless T is 0), and out meets no other array.
+ */
+int expert_cache_moe8_workspace(const expert_cache_experts* e, int T, int top_k, long* bytes);
+int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_stride,
+                      const float* topk_weights, const void* ids, int id_bytes, int T, int top_k,
+                      void* out, long out_stride, void* workspace, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

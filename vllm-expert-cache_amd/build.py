@@ -1,6 +1,6 @@
 """Build the in-tree libraries of the vllm_expert_cache package.
 
-  libexpertcache.so  gfx950 kernels + C-ABI (csrc/expert_cache.hip), hipcc
+  libexpertcache.so  gfx950 kernels + C-ABI (csrc/expert_cache.hip, csrc/many_tokens.hip), hipcc
   libectrace.so      routing-trace generator (csrc/traces.c), host C
 
 Both land next to the package (vllm_expert_cache/), where _lib.py and traces.py look first.
@@ -67,7 +67,7 @@ def build_kernels(verbose: bool = False) -> Path:
     out = PKG / "libexpertcache.so"
     tmp = out.with_suffix(".so.tmp")
     _run([hipcc(), *HIP_FLAGS, "-I", str(ROOT / "include"), str(CSRC / "expert_cache.hip"),
-          "-o", str(tmp)], verbose)
+          str(CSRC / "many_tokens.hip"), "-o", str(tmp)], verbose)
     missing = [s for s in declared_symbols() if s not in exported_symbols(tmp)]
     if missing:
         tmp.unlink()

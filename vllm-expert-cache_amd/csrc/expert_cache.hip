@@ -15,19 +15,13 @@
 #include "align.h"
 #include "experts.h"
 #include "gather.h"
+#include "host.h"
 #include "manage.h"
 #include "refresh.h"
 #include "route.h"
 
 namespace ec {
 namespace {
-
-// [p, p + pn) and [q, q + qn) share a byte
-bool ranges_meet(const void* p, long long pn, const void* q, long long qn) {
-  const long long a = (long long)reinterpret_cast<uintptr_t>(p);
-  const long long b = (long long)reinterpret_cast<uintptr_t>(q);
-  return pn > 0 && qn > 0 && a < b + qn && b < a + pn;
-}
 
 bool manage_args_bad(int E, int S, int max_inserts, int policy) {
   if (E <= 0 || S <= 0 || S > kMaxSlots || S > kSlotMask) return true;
@@ -145,8 +139,6 @@ ManageArgs make_args(const void* ids, int mk, int E, int S, int max_distinct, in
 }
 
 // ---- operators over slots -----------------------------------------------------------------
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <class X, bool BIAS>
 void launch_route_of(const RouteArgs& a, hipStream_t stream) {

@@ -7,7 +7,7 @@ points that replace the reference's torch remap, `expert_cache_prefetch`,
 `expert_cache_manage_remap_prefetch` (one layer's policy step with another's prefetch step
 in one launch), `expert_cache_gather_live` (the prefetch copy that stops for dropped
 predictions), and `expert_cache_refresh` (policy step, remap and gather in one call); and the
-operators of ops.py with the workspace sizes of two of them. Every call is asynchronous on the
+operators of ops.py with the workspace sizes that some of them need. Every call is asynchronous on the
 caller's stream and never reads a device value back, so the whole path is HIP-graph capturable.
 
 There is no fallback: if the library or one of its symbols is missing, loading fails with
@@ -71,6 +71,29 @@ SIGNATURES = {
     # adapt(adapters, x, x_stride, ids, id_bytes, T, base, base_stride, out, out_stride,
     #       workspace, stream)
     "expert_cache_adapt": [_P, _P, _L, _P, _I, _I, _P, _L, _P, _L, _P, _P],
+    # sort_workspace(T, top_k, S, bytes)
+    "expert_cache_sort_workspace": [_I, _I, _I, _P],
+    # sort(ids, id_bytes, T, top_k, S, offsets, rows, places, workspace, stream)
+    "expert_cache_sort": [_P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
+    # dispatch(x, type, x_stride, places, offsets, T, top_k, S, H, out, out_stride, stream)
+    "expert_cache_dispatch": [_P, _I, _L, _P, _P, _I, _I, _I, _I, _P, _L, _P],
+    # combine(y, type, y_stride, weights, places, T, top_k, H, out, out_stride, stream)
+    "expert_cache_combine": [_P, _I, _L, _P, _P, _I, _I, _I, _P, _L, _P],
+    # combine_grad(grad, type, grad_stride, y, y_stride, weights, places, offsets, T, top_k, S, H,
+    #              dy, dy_stride, dweights, stream)
+    "expert_cache_combine_grad": ([_P, _I, _L, _P, _L, _P, _P, _P] + [_I] * 4
+                                  + [_P, _L, _P, _P]),
+    # quantize(x, type, x_stride, T, H, q, q_stride, scales, stream)
+    "expert_cache_quantize": [_P, _I, _L, _I, _I, _P, _L, _P, _P],
+    # linear8_workspace(linear, type, T, bytes)
+    "expert_cache_linear8_workspace": [_P, _I, _I, _P],
+    # linear8(linear, x, type, x_stride, x_scales, T, out, out_type, out_stride, workspace, stream)
+    "expert_cache_linear8": [_P, _P, _I, _L, _P, _I, _P, _I, _L, _P, _P],
+    # moe8_workspace(experts, T, top_k, bytes)
+    "expert_cache_moe8_workspace": [_P, _I, _I, _P],
+    # moe8(experts, x, x_stride, topk_weights, ids, id_bytes, T, top_k, out, out_stride,
+    #      workspace, stream)
+    "expert_cache_moe8": [_P, _P, _L, _P, _P, _I, _I, _I, _P, _L, _P, _P],
 }
 
 
@@ -95,6 +118,12 @@ class Adapters(ctypes.Structure):
 
     _fields_ = ([(n, _I) for n in ("S", "H", "O", "R", "type")]
                 + [(n, _P) for n in ("a", "b", "scales")])
+
+
+class Linear(ctypes.Structure):
+    """expert_cache_linear: the 8-bit weights of one projection."""
+
+    _fields_ = [("O", _I), ("H", _I), ("w_stride", _L), ("w", _P), ("scale", _P), ("bias", _P)]
 
 
 def library_path() -> str:

@@ -8,13 +8,22 @@ its slots hold.
     slots = adapter_cache.refresh(adapter_ids)        # the same for adapters of requests
     y = Adapters(a_slots, b_slots)(x, projected, slots)
 
-`Experts` and `Adapters` check their weights once and are kept like the weights themselves; a
-cache's slot tensors never move, so a handle over them stays good. Weights are used as they lie,
-without another layout. Calls run on the current stream of the tensors' device, allocate only
-their result and a workspace through torch, and read nothing back, so they can be captured.
+For many tokens, in parts or as a whole layer in 8-bit integers:
 
-There is no backward pass: with gradients enabled, a tensor that requires one (a handle's weights:
-when the handle is made) is refused.
+    order = sort(slots, S)                            # pairs of token and slot, slot by slot
+    rows = dispatch(x, order)                         # every slot's tokens side by side
+    y = combine(products_of(rows, order.offsets), weights, order)
+    y = Experts8(w13_slots, w2_slots, s13, s2)(x, weights, slots)
+    y = Linear8(w, w_scale)(x)                        # a projection; quantize(x) is its first half
+
+`Experts`, `Adapters`, `Linear8` and `Experts8` check their weights once and are kept like the
+weights themselves; a cache's slot tensors never move, so a handle over them stays good. Weights are
+used as they lie, without another layout (but see `Linear8`). Calls run on the current stream of the
+tensors' device, allocate only their result and a workspace through torch, and read nothing back, so
+they can be captured.
+
+`dispatch` and `combine` have a backward pass. The others have none: with gradients enabled, a tensor
+that requires one (a handle's weights: when the handle is made) is refused.
 
 ValueError names an argument that an operator does not take; nothing has run then.
 """
@@ -41,6 +50,10 @@ MAX_RANK = 256
 MAX_TOKENS = 1 << 21   # of one routing or Adapters call
 MAX_OUTPUTS = 1 << 21  # of an adapter
 MAX_LENGTH = 1 << 24   # of a row of weights: H and I
+MAX_SORTED = 1 << 24   # pairs of one sort: tokens x top_k
+MAX_ROW = 1 << 20      # values of a row that is dispatched, combined or quantised
+MAX_LENGTH8 = 131056   # of a sum of 8-bit products, which 32 bits hold
+MAX_BYTES8 = 7 << 28   # of Experts8's quantised tokens, and of an expert's w13
 
 
 def _check(rc: int, name: str) -> None:
@@ -345,4 +358,438 @@ class Adapters:
         _check(_on_device(device, h.expert_cache_adapt, self._at, x.data_ptr(), x.stride(0),
                           ids.data_ptr(), nbytes, T, base.data_ptr(), base.stride(0),
                           out.data_ptr(), out.stride(0), work.data_ptr()), "expert_cache_adapt")
+        return out
+
+
+# ---- pairs sorted by slot and back ---------------------------------------------------------
+
+class Order:
+    """Pairs of token and slot sorted by slot (`sort`). Pair t * k + j is token t's j-th.
+
+    offsets  int32 [S + 1]: slot s has places offsets[s] to offsets[s + 1]
+    rows     int32 [T * k]: the pair at every place, -1 from offsets[S] on
+    places   int32 [T, k]: the place of every pair, -1 if its id is outside [0, S)"""
+
+    __slots__ = ("offsets", "rows", "places", "T", "k", "S", "device")
+
+    def __init__(self, offsets: torch.Tensor, rows: torch.Tensor, places: torch.Tensor, S: int):
+        device = _on_gpu(offsets, rows, places)
+        _need(places.dim() == 2 and 1 <= places.shape[1] <= MAX_TOP_K and
+              places.numel() <= MAX_SORTED and 1 <= S <= MAX_EXPERTS and
+              rows.shape == (places.numel(),) and offsets.shape == (S + 1,),
+              f"offsets {list(offsets.shape)}, rows {list(rows.shape)} and places "
+              f"{list(places.shape)} are no order of pairs by {S} slots")
+        for t in (offsets, rows, places):
+            _need(t.dtype == torch.int32 and t.is_contiguous(),
+                  f"offsets, rows and places must be contiguous int32 on {device}")
+        self._set(offsets, rows, places, S)
+
+    def _set(self, offsets, rows, places, S):
+        self.offsets, self.rows, self.places, self.S = offsets, rows, places, S
+        self.T, self.k = places.shape
+        self.device = places.device
+        return self
+
+
+def sort(slot_ids: torch.Tensor, slots: int) -> Order:
+    """The pairs of token and slot, T x k int32 or int64 ids (or T of them: k is 1), slot by slot;
+    those of a slot stay in the order of the tokens. Up to 1024 slots and 2^24 pairs, k up to 64."""
+    shape = slot_ids.shape
+    if len(shape) == 1:
+        slot_ids, shape = slot_ids.unsqueeze(1), (shape[0], 1)
+    if len(shape) != 2 or not 1 <= shape[1] <= MAX_TOP_K or shape[0] * shape[1] > MAX_SORTED:
+        raise ValueError(f"slot_ids must be [T, k] or [T], k up to {MAX_TOP_K} and {MAX_SORTED} in "
+                         f"all, not {list(shape)}")
+    if not 1 <= slots <= MAX_EXPERTS:
+        raise ValueError(f"{slots} slots (1 to {MAX_EXPERTS})")
+    device = _on_gpu(slot_ids)
+    ids, nbytes = _ids(slot_ids, device)
+    T, k = shape
+    n = T * k
+    new = torch.empty(2 * n + slots + 1, dtype=torch.int32, device=device)
+    rows, places, offsets = new.split((n, n, slots + 1))
+    h = _lib.lib()
+    size = _SORT_BYTES.get((n, slots))
+    if size is None:
+        need = ctypes.c_long()
+        _check(h.expert_cache_sort_workspace(T, k, slots, ctypes.addressof(need)),
+               "expert_cache_sort_workspace")
+        if len(_SORT_BYTES) >= 4096:
+            _SORT_BYTES.clear()
+        size = _SORT_BYTES[n, slots] = need.value
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _check(_on_device(device, h.expert_cache_sort, ids.data_ptr(), nbytes, T, k, slots,
+                      offsets.data_ptr(), rows.data_ptr(), places.data_ptr(),
+                      work.data_ptr() if size else None), "expert_cache_sort")
+    return Order.__new__(Order)._set(offsets, rows, places.view(T, k), slots)
+
+
+_SORT_BYTES: dict = {}  # workspace by pairs and slots
+
+
+def _pitched(t: torch.Tensor) -> torch.Tensor:
+    """`t` with its rows' values side by side and rows apart: itself, or a copy."""
+    step = t.stride()
+    return t if step[1] == 1 and (t.shape[0] < 2 or step[0] >= t.shape[1]) else t.contiguous()
+
+
+def _movable(t, rows: int, order: Order, what: str) -> int:
+    kind = _LOGITS.get(t.dtype)
+    if kind is None or t.dim() != 2 or t.shape[0] != rows or t.device != order.device:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16 [{rows}, H] on "
+                         f"{order.device}, not {t.dtype} {list(t.shape)} on {t.device}")
+    if not 0 < t.shape[1] <= MAX_ROW:
+        raise ValueError(f"rows of {t.shape[1]} (1 to {MAX_ROW})")
+    return kind
+
+
+def _recordable() -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("a captured call cannot be recorded for a backward pass: capture it under "
+                         "torch.no_grad(), with combine and combine_grad for the gradients")
+
+
+def dispatch(x: torch.Tensor, order: Order) -> torch.Tensor:
+    """The tokens' rows in the slots' order, [T * k, H]: row p is x[order.rows[p] // k], and rows
+    from order.offsets[S] on are zeros. x [T, H] is float32, bfloat16 or float16; H up to 2^20.
+
+    Differentiable in x, once: a token's gradient is the 32-bit sum of its rows', rounded to x's
+    type. `combine(gradient, None, order)` is the same without autograd, for a call that is
+    captured; one that autograd would record is refused then."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        _movable(x, order.T, order, "x")
+        _recordable()
+        return _Dispatch.apply(x, order)
+    return _dispatch(x, order)
+
+
+def _dispatch(x, order):
+    kind = _movable(x, order.T, order, "x")
+    x = _pitched(x)
+    H, n = x.shape[1], order.T * order.k
+    out = x.new_empty((n, H))
+    _check(_on_device(order.device, _lib.lib().expert_cache_dispatch, x.data_ptr(), kind,
+                      max(H, x.stride(0)), order.places.data_ptr(), order.offsets.data_ptr(),
+                      order.T, order.k, order.S, H, out.data_ptr(), H), "expert_cache_dispatch")
+    return out
+
+
+def combine(y: torch.Tensor, weights: torch.Tensor | None, order: Order) -> torch.Tensor:
+    """Rows back to their tokens: [T, H], token t the sum over j of weights[t, j] times
+    y[order.places[t, j]], in 32 bits and rounded to y's type. y [T * k, H] is float32, bfloat16 or
+    float16, weights float32 [T, k] or None (1). Pairs without a place or with a weight of 0 add
+    nothing (and an infinity in their rows does not show).
+
+    Differentiable in y and weights, once (`combine_grad` is the same without autograd, for a call
+    that is captured; one that autograd would record is refused then)."""
+    if torch.is_grad_enabled() and (y.requires_grad or
+                                    (weights is not None and weights.requires_grad)):
+        _combine_args(y, weights, order)
+        _recordable()
+        return _Combine.apply(y, weights, order)
+    return _combine(y, weights, order)
+
+
+def _combine_args(y, weights, order) -> int:
+    kind = _movable(y, order.T * order.k, order, "y")
+    if weights is not None and (weights.dtype != torch.float32 or weights.device != order.device or
+                                weights.shape != order.places.shape):
+        raise ValueError(f"weights must be float32 {list(order.places.shape)} on {order.device}, "
+                         f"not {weights.dtype} {list(weights.shape)} on {weights.device}")
+    return kind
+
+
+def _combine(y, weights, order):
+    kind = _combine_args(y, weights, order)
+    y = _pitched(y)
+    if weights is not None and not weights.is_contiguous():
+        weights = weights.contiguous()
+    H = y.shape[1]
+    out = y.new_empty((order.T, H))
+    _check(_on_device(order.device, _lib.lib().expert_cache_combine, y.data_ptr(), kind,
+                      max(H, y.stride(0)), None if weights is None else weights.data_ptr(),
+                      order.places.data_ptr(), order.T, order.k, H, out.data_ptr(), H),
+           "expert_cache_combine")
+    return out
+
+
+def combine_grad(grad: torch.Tensor, y: torch.Tensor | None, weights: torch.Tensor | None,
+                 order: Order, *, need_y: bool = True, need_weights: bool = True):
+    """The gradients of `combine` from that of its result: (dy [T * k, H], dweights float32
+    [T, k]), each None if it is not needed. dy[order.places[t, j]] is weights[t, j] * grad[t],
+    rounded to its type, and zero from order.offsets[S] on; dweights[t, j] is the 32-bit dot product
+    of grad[t] and y[order.places[t, j]], 0 without a place. y may be None without need_weights."""
+    kind = _movable(grad, order.T, order, "grad")
+    H, n = grad.shape[1], order.T * order.k
+    need_weights = need_weights and weights is not None
+    if y is not None:
+        _combine_args(y, weights, order)
+        _need(y.shape[1] == H and y.dtype == grad.dtype,
+              f"y {y.dtype} {list(y.shape)} does not go with grad {grad.dtype} {list(grad.shape)}")
+        y = _pitched(y)
+    else:
+        _need(not need_weights, "the gradient of weights needs y")
+        _need(weights is None or (weights.dtype == torch.float32 and
+                                  weights.shape == order.places.shape and
+                                  weights.device == order.device),
+              f"weights must be float32 {list(order.places.shape)} on {order.device}")
+    if torch.is_grad_enabled():
+        _no_gradient(grad, y, weights)
+    grad = _pitched(grad)
+    dy = grad.new_empty((n, H)) if need_y else None
+    dweights = grad.new_empty((order.T, order.k), dtype=torch.float32) if need_weights else None
+    if dy is None and dweights is None:
+        return None, None
+    if weights is not None and not weights.is_contiguous():
+        weights = weights.contiguous()
+    _check(_on_device(order.device, _lib.lib().expert_cache_combine_grad, grad.data_ptr(), kind,
+                      max(H, grad.stride(0)), None if y is None else y.data_ptr(),
+                      H if y is None else max(H, y.stride(0)),
+                      None if weights is None else weights.data_ptr(), order.places.data_ptr(),
+                      order.offsets.data_ptr(), order.T, order.k, order.S, H,
+                      None if dy is None else dy.data_ptr(), H,
+                      None if dweights is None else dweights.data_ptr()),
+           "expert_cache_combine_grad")
+    return dy, dweights
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, order):
+        ctx.order = order
+        return _dispatch(x, order)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _combine(grad, None, ctx.order), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, order):
+        ctx.order = order
+        ctx.save_for_backward(y if ctx.needs_input_grad[1] else None, weights)
+        return _combine(y, weights, order)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, weights = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return *combine_grad(grad, y, weights, ctx.order, need_y=need[0],
+                             need_weights=need[1]), None
+
+
+# ---- products in 8-bit integers ------------------------------------------------------------
+
+def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows as 8-bit integers and what 1 stands for: (q int8 [T, H], scales float32 [T]), with m a
+    row's largest magnitude scales = m / 127 and q = 127 x / m to the nearest, ties to even. x is
+    bfloat16 or float16 [T, H], H up to 2^20; q's rows lie in ones of a multiple of 16. A row below
+    2^-119 throughout counts as zeros, and one with an infinity or NaN becomes zeros with a scale
+    of NaN."""
+    kind = _TOKENS.get(x.dtype)
+    if kind is None or x.dim() != 2:
+        raise ValueError(f"x must be bfloat16 or float16 [T, H], not {x.dtype} {list(x.shape)}")
+    T, H = x.shape
+    if T > MAX_SORTED or not 0 < H <= MAX_ROW:
+        raise ValueError(f"{T} rows (at most {MAX_SORTED}) of {H} (1 to {MAX_ROW})")
+    device = _on_gpu(x)
+    if torch.is_grad_enabled() and x.requires_grad:
+        _no_gradient(x)
+    x = _pitched(x)
+    q = torch.empty((T, -(-H // 16) * 16), dtype=torch.int8, device=device)
+    scales = torch.empty(T, dtype=torch.float32, device=device)
+    _check(_on_device(device, _lib.lib().expert_cache_quantize, x.data_ptr(), kind,
+                      max(H, x.stride(0)), T, H, q.data_ptr(), q.shape[1], scales.data_ptr()),
+           "expert_cache_quantize")
+    return q[:, :H] if q.shape[1] != H else q, scales
+
+
+class Linear8:
+    """A projection in 8-bit integers: y = x w^T + bias, tokens quantised with a scale each.
+
+    w      int8 [O, H], H up to 131056        scale  float32 [O] or [O, 1], one a channel
+    bias   float32, bfloat16 or float16 [O], or None
+
+    Sums are exact; their product with both scales and the bias's sum are in 32 bits, and the result
+    is rounded to its type. w is used as it lies if H and its rows are whole 16 bytes, and is copied
+    otherwise, as is a bias that is not float32: a later change of those does not show."""
+
+    def __init__(self, w: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None):
+        _need(w.dim() == 2 and w.dtype == torch.int8 and min(w.shape) > 0,
+              f"w must be int8 [O, H], not {w.dtype} {list(w.shape)}")
+        O, H = w.shape
+        _need(H <= MAX_LENGTH8 and O <= MAX_SORTED,
+              f"w {list(w.shape)} (at most [{MAX_SORTED}, {MAX_LENGTH8}])")
+        self.device = _on_gpu(w, scale, bias)
+        _scales(scale, (O,), "scale", self.device)
+        if bias is not None:
+            _need(bias.dtype in _LOGITS and bias.shape == (O,),
+                  f"bias must be float32, bfloat16 or float16 [{O}], not {bias.dtype} "
+                  f"{list(bias.shape)}")
+        self._graded = _graded(w, scale, bias)
+        step = w.stride()
+        if H % 16 or w.data_ptr() % 16 or step[1] != 1 or \
+                (O > 1 and (step[0] % 16 or step[0] < H or step[0] > 1 << 22)):
+            laid = w.new_zeros((O, -(-H // 16) * 16))
+            laid[:, :H] = w.detach()
+            w = laid
+        if bias is not None:
+            bias = bias.detach().float().contiguous()
+        self.w, self.scale, self.bias = w, scale, bias
+        self.O, self.H = O, H
+        self._struct = _lib.Linear(O, H, w.stride(0) if O > 1 else -(-H // 16) * 16, w.data_ptr(),
+                                   scale.data_ptr(), None if bias is None else bias.data_ptr())
+        self._at = ctypes.addressof(self._struct)
+        self._bytes: dict = {}
+
+    def __call__(self, x: torch.Tensor, x_scales: torch.Tensor | None = None, *,
+                 dtype: torch.dtype | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+        """[T, O] for tokens x [T, H] in bfloat16 or float16, or in int8 with x_scales float32 [T]
+        as `quantize` makes them (projections that share their tokens quantise them once). The
+        result's type is `dtype`: float32, bfloat16 or float16, if not given x's (bfloat16 for
+        int8). `out`, if given, has contiguous rows and overlaps neither x nor x_scales."""
+        kind = 3 if x.dtype == torch.int8 else _TOKENS.get(x.dtype)
+        if kind is None or x.dim() != 2 or x.shape[1] != self.H or x.device != self.device:
+            raise ValueError(f"x must be bfloat16, float16 or int8 [T, {self.H}] on {self.device}, "
+                             f"not {x.dtype} {list(x.shape)} on {x.device}")
+        T = x.shape[0]
+        if T > MAX_SORTED:
+            raise ValueError(f"{T} tokens (at most {MAX_SORTED})")
+        if dtype is None:
+            dtype = torch.bfloat16 if kind == 3 else x.dtype
+        to = _LOGITS.get(dtype)
+        if to is None:
+            raise ValueError(f"results of {dtype} (float32, bfloat16 or float16)")
+        if (x_scales is None) != (kind != 3) or (x_scales is not None and (
+                x_scales.dtype != torch.float32 or x_scales.shape != (T,) or
+                x_scales.device != self.device)):
+            raise ValueError(f"int8 tokens, and no others, have x_scales: float32 [{T}] on "
+                             f"{self.device}")
+        if torch.is_grad_enabled() and (x.requires_grad or self._graded or out is not None or
+                                        x_scales is not None):
+            _no_gradient(x, x_scales, out, *self._graded)
+        if kind == 3:
+            x = self._whole(x)
+            if not x_scales.is_contiguous():
+                x_scales = x_scales.contiguous()
+        else:
+            x = _pitched(x)
+        if out is None:
+            out = torch.empty((T, self.O), dtype=dtype, device=self.device)
+        else:
+            _out(out, dtype, (T, self.O), self.device)
+        h, at = _lib.lib(), self._at
+        size = self._bytes.get((kind == 3, T))
+        if size is None:
+            if len(self._bytes) >= 4096:
+                self._bytes.clear()
+            size = self._bytes[kind == 3, T] = _workspace(h.expert_cache_linear8_workspace, at, kind,
+                                                          T)
+        work = torch.empty(size, dtype=torch.uint8, device=self.device)
+        _check(_on_device(self.device, h.expert_cache_linear8, at, x.data_ptr(), kind,
+                          max(x.stride(0), self.H), None if kind != 3 else x_scales.data_ptr(), T,
+                          out.data_ptr(), to, max(out.stride(0), self.O), work.data_ptr()),
+               "expert_cache_linear8")
+        return out
+
+    def _whole(self, x: torch.Tensor) -> torch.Tensor:
+        """8-bit rows that can be loaded 16 bytes at a time: `x`, or a copy."""
+        step, length = x.stride(), -(-self.H // 16) * 16
+        end = x.storage_offset() + (x.shape[0] - 1) * step[0] + length
+        if x.shape[0] and (step[1] != 1 or x.data_ptr() % 16 or
+                           end > x.untyped_storage().nbytes() or
+                           (x.shape[0] > 1 and (step[0] % 16 or not length <= step[0] <= 1 << 22))):
+            laid = x.new_zeros((x.shape[0], length))
+            laid[:, :self.H] = x
+            x = laid
+        return x
+
+
+class Experts8:
+    """The experts of one layer, in slots or all of them, in 8-bit integers for any number of tokens.
+
+    w13  int8 [S, 2*I, H]: gate rows, then up rows, w13_scale float32 [S, 2*I] or [S, 2*I, 1]
+    w2   int8 [S, H, I], w2_scale float32 [S, H] or [S, H, 1]
+    H and I are multiples of 16, S up to 1024.
+
+    Tokens and hidden values are quantised row by row (`quantize`; hidden values from 32 bits), so
+    results differ from `Experts`' by the rounding of those. Sums are exact, the rest is in 32 bits,
+    the result is rounded to the tokens' type. The same call gives the same bits, and a token's are
+    the same among any others. A token with an infinity or NaN gets NaN."""
+
+    def __init__(self, w13: torch.Tensor, w2: torch.Tensor, w13_scale: torch.Tensor,
+                 w2_scale: torch.Tensor):
+        _need(w13.dim() == 3 and w2.dim() == 3 and w13.dtype == w2.dtype == torch.int8,
+              "w13 and w2 must be int8 [S, 2*I, H] and [S, H, I]")
+        S, two, H = w13.shape
+        _need(two % 2 == 0 and tuple(w2.shape) == (S, H, two // 2) and min(S, two, H) > 0,
+              f"w13 {list(w13.shape)} does not go with w2 {list(w2.shape)}")
+        _need(H % 16 == 0 and (two // 2) % 16 == 0,
+              f"H {H} and I {two // 2} must be multiples of 16")
+        _need(max(H, two // 2) <= MAX_LENGTH8 and two * H <= MAX_BYTES8 and S <= MAX_EXPERTS,
+              f"{S} slots (at most {MAX_EXPERTS}) of H {H} and I {two // 2} (at most {MAX_LENGTH8}, "
+              f"w13 of {MAX_BYTES8} bytes)")
+        for name, w in (("w13", w13), ("w2", w2)):
+            _need(w.is_contiguous() and w.data_ptr() % 16 == 0,
+                  f"{name} must be contiguous and 16-byte aligned")
+        device = _on_gpu(w13, w2)
+        _scales(w13_scale, (S, two), "w13_scale", device)
+        _scales(w2_scale, (S, H), "w2_scale", device)
+        self.w13, self.w2, self.w13_scale, self.w2_scale = w13, w2, w13_scale, w2_scale
+        self.S, self.H, self.I, self.device = S, H, two // 2, device
+        self._structs = {}
+        for t, code in _TOKENS.items():
+            e = _lib.Experts(S, H, two // 2, code, _BYTES[torch.int8], w13.data_ptr(),
+                             w2.data_ptr(), w13_scale.data_ptr(), w2_scale.data_ptr())
+            self._structs[t] = (e, ctypes.addressof(e))
+        self._graded = _graded(w13_scale, w2_scale)
+        self._bytes: dict = {}
+
+    def __call__(self, x: torch.Tensor, topk_weights: torch.Tensor, slot_ids: torch.Tensor,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+        """The layer's output [T, H] for tokens x [T, H] in bfloat16 or float16: the sum over their
+        slots of the routing weight (float32 [T, top_k]) times the expert. slot_ids [T, top_k] are
+        int32 or int64; T x top_k is at most 2^24, T x H 1.75 * 2^30. A pair whose id is outside
+        [0, S) or whose weight is 0 adds nothing; a token without any other pair gets zeros. `out`,
+        if given, has contiguous rows and overlaps no other argument."""
+        struct = self._structs.get(x.dtype)
+        if struct is None or x.dim() != 2 or x.shape[1] != self.H or x.device != self.device:
+            raise ValueError(f"x must be bfloat16 or float16 [T, {self.H}] on {self.device}, not "
+                             f"{x.dtype} {list(x.shape)} on {x.device}")
+        T, shape = x.shape[0], slot_ids.shape
+        if len(shape) != 2 or shape[0] != T or topk_weights.shape != shape or \
+                topk_weights.dtype != torch.float32 or topk_weights.device != self.device:
+            raise ValueError(f"slot_ids {list(shape)} and float32 topk_weights must be [{T}, top_k] "
+                             f"on {self.device}, not {topk_weights.dtype} "
+                             f"{list(topk_weights.shape)} on {topk_weights.device}")
+        k = shape[1]
+        if not 1 <= k <= MAX_TOP_K or T * k > MAX_SORTED or T * self.H > MAX_BYTES8:
+            raise ValueError(f"{T} tokens of {self.H} x top_k {k} (top_k at most {MAX_TOP_K}, "
+                             f"{MAX_SORTED} pairs, {MAX_BYTES8} values)")
+        if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or
+                                        self._graded or out is not None):
+            _no_gradient(x, topk_weights, out, *self._graded)
+        ids, nbytes = _ids(slot_ids, self.device)
+        if not topk_weights.is_contiguous():
+            topk_weights = topk_weights.contiguous()
+        x = _pitched(x)
+        if out is None:
+            out = x.new_empty((T, self.H))
+        else:
+            _out(out, x.dtype, (T, self.H), self.device)
+        h, at = _lib.lib(), struct[1]
+        size = self._bytes.get((T, k))
+        if size is None:
+            if len(self._bytes) >= 4096:
+                self._bytes.clear()
+            size = self._bytes[T, k] = _workspace(h.expert_cache_moe8_workspace, at, T, k)
+        work = x.new_empty(size, dtype=torch.uint8)
+        _check(_on_device(self.device, h.expert_cache_moe8, at, x.data_ptr(),
+                          max(x.stride(0), self.H), topk_weights.data_ptr(), ids.data_ptr(), nbytes,
+                          T, k, out.data_ptr(), max(out.stride(0), self.H), work.data_ptr()),
+               "expert_cache_moe8")
         return out
