@@ -77,10 +77,12 @@ def _sorted(ids, S):
 # ---- sort ---------------------------------------------------------------------------------
 
 # one pair; fewer and more pairs than a wave; one slot, most slots; both sides of one workgroup's
-# pairs (16384) and of every cut by waves; runs of a wave that are empty
-SORTS = [(1, 1, 1), (1, 8, 64), (3, 21, 5), (64, 1, 2), (65, 1, 1024), (13, 5, 7), (300, 10, 257),
-         (128, 8, 1024), (1024, 16, 128), (1025, 16, 128), (5000, 10, 910), (20000, 3, 1023),
-         (70001, 1, 3), (40000, 64, 512)]
+# pairs (4096), of the cuts by waves (64, 256, 1024) and of a lot of several workgroups'; more lots
+# than workgroups
+SORTS = [(1, 1, 1), (1, 8, 64), (3, 21, 5), (64, 1, 2), (65, 1, 1024), (13, 5, 7), (64, 4, 9),
+         (257, 1, 64), (300, 10, 257), (128, 8, 1024), (41, 25, 1024), (512, 8, 128), (4097, 1, 128),
+         (1024, 16, 128), (1025, 16, 128), (5000, 10, 910), (20000, 3, 1023), (70001, 1, 3),
+         (40000, 64, 512)]
 
 
 @pytest.mark.parametrize("T,k,S", SORTS)
@@ -444,7 +446,13 @@ def _whole(g, *shape):
 LINEARS = [(1, 1, 1), (1, 16, 16), (2, 128, 128), (3, 129, 17), (5, 1045, 1003), (16, 2048, 96),
            (17, 144, 130), (31, 400, 128), (33, 256, 257), (64, 272, 64), (65, 1024, 48),
            (128, 128, 128), (129, 640, 384), (200, 96, 1000), (256, 512, 256), (257, 16, 513),
-           (300, 4112, 520), (513, 1040, 1045)]
+           (300, 4112, 520), (513, 1040, 1045),
+           # few tokens quantised beside the product, as many values as that takes and one row more
+           (4, 4096, 40), (8, 2048, 33), (9, 2048, 33), (1, 16384, 20), (1, 16400, 20), (48, 1000, 50),
+           # cut along the length: 6, 3 and 8 parts, of which the last is short or empty
+           (70, 6200, 130), (130, 6160, 1029), (20, 8300, 77),
+           # tiles of 128 and 256: filled, ragged, odd outputs, one step and several
+           (1000, 160, 2344), (1100, 96, 2043), (2500, 144, 2568), (2437, 272, 2701), (2304, 128, 2816)]
 
 
 def _linear(q, m, lin, bias):
@@ -605,6 +613,26 @@ def test_experts8(T, k, S, H, I, dtype, id_dtype):
     # a token's result does not depend on the tokens beside it
     some = torch.arange(0, T, max(1, T // 5), device=DEV)
     assert torch.equal(e(x[some], probs[some], ids[some]), got[some])
+
+
+FILLS = [0, 1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 95, 96, 97, 127, 128, 129, 159, 161, 191, 193, 223,
+         225, 255, 256, 257]
+
+
+@pytest.mark.parametrize("fills", [FILLS[:8] + [0] * 20, FILLS, [256 + n for n in FILLS]], ids=len)
+def test_experts8_of_every_fill(fills):
+    """Slots of as many pairs as fill a tile, its rounds and their operands, and one more or less;
+    tiles of 32, 128 and 256 rows. The rows of a slot's neighbours stay its neighbours'."""
+    S, H, I = len(fills), 144, 80
+    e = _experts(60 + S, S, H, I)
+    g = _gen(sum(fills))
+    ids = torch.repeat_interleave(torch.arange(S, device=DEV), torch.tensor(fills, device=DEV))
+    ids = ids[torch.randperm(len(ids), device=DEV, generator=g)].unsqueeze(1)
+    x = _randn(g, len(ids), H).to(BF16)
+    probs = torch.rand((len(ids), 1), device=DEV, generator=g) + 0.1
+    got = e(x, probs, ids)
+    _close(got, *_moe8(e, x, probs, ids))
+    assert torch.equal(got, e(x, probs, ids))
 
 
 def test_experts8_of_one_slot_and_of_none():

@@ -43,10 +43,10 @@ def test_sort_workspace(lib):
         assert lib.expert_cache_sort_workspace(T, k, S, at) == -1
     assert lib.expert_cache_sort_workspace(1, 1, 1, None) == -1
     assert size.value == -5
-    for T, k, S in ((0, 1, 1), (2048, 8, 1024)):
+    for T, k, S in ((0, 1, 1), (512, 8, 1024)):
         assert lib.expert_cache_sort_workspace(T, k, S, at) == 0 and size.value == 0
     # counts of every key and workgroup, at most 256 of those
-    assert lib.expert_cache_sort_workspace(2049, 8, 100, at) == 0
+    assert lib.expert_cache_sort_workspace(513, 8, 100, at) == 0
     assert size.value == 4 * 5 * 101
     assert lib.expert_cache_sort_workspace(2 ** 24, 1, 1024, at) == 0
     assert size.value == 4 * 256 * 1025

@@ -15,6 +15,8 @@ import re
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -24,6 +26,7 @@ PKG = HERE / "vllm_expert_cache"
 HEADER = ROOT / "include" / "expert_cache.h"
 
 ARCH = os.environ.get("EXPERT_CACHE_ARCH", "gfx950")
+SOURCES = ("expert_cache.hip", "many_tokens.hip")
 HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared", f"--offload-arch={ARCH}",
              # keep hipcc from emitting packed-FP32 instructions (v_pk_*_f32)
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -66,8 +69,16 @@ def _run(cmd: list[str], verbose: bool) -> None:
 def build_kernels(verbose: bool = False) -> Path:
     out = PKG / "libexpertcache.so"
     tmp = out.with_suffix(".so.tmp")
-    _run([hipcc(), *HIP_FLAGS, "-I", str(ROOT / "include"), str(CSRC / "expert_cache.hip"),
-          str(CSRC / "many_tokens.hip"), "-o", str(tmp)], verbose)
+    compile_only = [f for f in HIP_FLAGS if f != "-shared"]
+    with tempfile.TemporaryDirectory() as objects:
+        parts = [(CSRC / name, Path(objects) / f"{name}.o") for name in SOURCES]
+        with ThreadPoolExecutor() as pool:
+            for done in [pool.submit(_run, [hipcc(), *compile_only, "-c", "-I", str(ROOT / "include"),
+                                            str(src), "-o", str(obj)], verbose)
+                         for src, obj in parts]:
+                done.result()
+        _run([hipcc(), "-shared", f"--offload-arch={ARCH}", *[str(obj) for _, obj in parts],
+              "-o", str(tmp)], verbose)
     missing = [s for s in declared_symbols() if s not in exported_symbols(tmp)]
     if missing:
         tmp.unlink()

@@ -23,7 +23,6 @@ namespace ec {
 using i32x4 = __attribute__((ext_vector_type(4))) int;
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 
-constexpr int kStepBytes = 128;            // of a row in a step
 constexpr unsigned kFarOffset = 0x78000000u;  // behind the end of every descriptor
 constexpr unsigned kMaxRange = 0x70000000u;
 constexpr int kMaxLength8 = 131056;        // 16 K at most: sums stay below 2^31
@@ -114,7 +113,13 @@ __global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
   if (threadIdx.x == 0) a.scales[row] = quantizer.scale;
 }
 
+constexpr int kDieUnits = 32;  // compute units of a die
+
 // ---- tiles ----------------------------------------------------------------------------------
+
+// A dense product; sums of a part of its length as they are; an expert's gate and up projections with
+// the product of both; its down projection.
+enum class Form { kDense, kPart, kGateUp, kDown };
 
 struct Product8Args {
   const int8_t* a;       // tokens [rows, K], a_stride bytes apart
@@ -124,6 +129,7 @@ struct Product8Args {
   const float* bias;
   long long a_stride, w_stride, a_bytes, slab_bytes;
   int rows, N, K;        // of dense products: rows; of Experts8's: pairs
+  int splits;            // of the length, with Form::kPart
   int out_tiles;         // tiles along N
   // Experts8: tiles of the sorted rows
   const int2* tiles;
@@ -133,10 +139,39 @@ struct Product8Args {
   int k;
   void* out;
   long long out_stride;  // elements
-  bool wide_stores;
+  int scale_rows;        // of a_scale
+  bool whole_stores;     // results can be stored 16 bytes at a time
 };
 
-enum class Form { kDense, kGateUp, kDown };
+constexpr int kStepBytes = 128;  // of a row in a step: two products' lengths
+
+__device__ __forceinline__ void load_word_to_lds(__amdgpu_buffer_rsrc_t from, char* to,
+                                                 unsigned offset) {
+  using Lds = __attribute__((address_space(3))) void*;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Lds)to, 4, offset, 0, 0, 0);
+}
+
+template <class X>
+__device__ __forceinline__ unsigned two_of(float a, float b) {
+  using V = typename Frag<X>::V;
+  using Two = __attribute__((ext_vector_type(2))) __typeof__(V{}[0] + V{}[0]);
+  return bits_as<unsigned>(__builtin_convertvector(f32x2{a, b}, Two));
+}
+
+// Four words of every lane, its row of 16 lanes q has words 0..3 of its own: afterwards it has word q
+// of rows 0..3.
+__device__ __forceinline__ void exchange_quads(unsigned& w0, unsigned& w1, unsigned& w2,
+                                               unsigned& w3) {
+  const auto a = __builtin_amdgcn_permlane32_swap(w0, w2, false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(w1, w3, false, false);
+  const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+  const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  w0 = c[0];
+  w1 = c[1];
+  w2 = d[0];
+  w3 = d[1];
+}
+
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t range_of(const void* p, long long bytes) {
   const unsigned n = bytes < (long long)kMaxRange ? (unsigned)bytes : kMaxRange;
@@ -149,149 +184,477 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, char* t
   __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Lds)to, 16, offset, step, 0, 0);
 }
 
-// One tile a workgroup. Waves form WM x WN; the weights' rows of a gate-up tile are TN / 2 of the
-// gate and the same of the up projection, so that a lane holds both of a hidden value.
-template <int TM, int TN, int WM, int WN, Form FORM, class OUT>
-__global__ __launch_bounds__(WM* WN* kWave) void product8_k(Product8Args a) {
-  constexpr int kWaves = WM * WN;
-  constexpr int kStage = (TM + TN) * kStepBytes;
-  constexpr int kA = TM / 8 / kWaves, kB = TN / 8 / kWaves;  // loads a wave and step
-  constexpr int kM = TM / WM / 16, kN = TN / WN / 16;        // operands a wave
-  static_assert(kA * 8 * kWaves == TM && kB * 8 * kWaves == TN);
-  constexpr bool kGrouped = FORM != Form::kDense, kGated = FORM == Form::kGateUp;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+// Waits until at most LEFT of the wave's loads and stores are under way (they finish in order) and
+// its reads of LDS are done, then for the workgroup's other waves.
+template <int LEFT>
+__device__ __forceinline__ void landed() {
+  static_assert(LEFT < 64);
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | (LEFT >> 4) << 14 | 7 << 4);
+  lds_sync();
+}
 
-  // consecutive workgroups go to the eight dies in turn: each die gets a run of tiles, so that
-  // its second-level cache holds what they share
-  const int m_tiles = kGrouped ? *a.n_tiles : (a.rows + TM - 1) / TM;
-  const long long n = (long long)m_tiles * a.out_tiles, per = (n + 7) / 8;
-  const long long in_die = blockIdx.x / 8, at = (blockIdx.x % 8) * per + in_die;
-  if (in_die >= per || at >= n) return;
-  const int n_tile = (int)(at / m_tiles), m_tile = (int)(at - (long long)n_tile * m_tiles);
-  int slot = 0, m0 = m_tile * TM, m_end = a.rows;
-  if constexpr (kGrouped) {
-    const int2 t = a.tiles[m_tile];
-    slot = t.x;
-    m0 = t.y;
-    m_end = a.offsets[slot + 1];
-  }
-  const int n0 = n_tile * (kGated ? TN / 2 : TN);
+// A workgroup takes a tile of up to TM tokens and TN outputs. Waves form WM x WN;
+// wave row wm has the 16-token operands wm, wm + WM, ..., so that a tile with fewer tokens (MI rounds
+// of WM operands, at most TM / 16 / WM) gives every wave less to do. A gate-up tile's weights are
+// TN / 2 rows of the gate and the same of the up projection, so that a lane holds both of a hidden
+// value.
+template <int TM, int TN, int WM, int WN, int ST, Form FORM, class OUT>
+struct Product8 {
+  static constexpr int kWaves = WM * WN;
+  static constexpr int kStage = (TM + TN) * kStepBytes;
+  static constexpr int kMost = TM / WM / 16;                      // rounds
+  static constexpr int kA = (TM / 8 + kWaves - 1) / kWaves;       // loads a wave and step
+  static constexpr int kB = (TN / 8 + kWaves - 1) / kWaves;
+  static constexpr int kN = TN / WN / 16;                         // operands a wave
+  static constexpr bool kGrouped = FORM == Form::kGateUp || FORM == Form::kDown, kGated = FORM == Form::kGateUp;
+  static constexpr int kOut = kGated ? kN / 2 : kN;               // of them with a result
+  static constexpr int kScaleLoads = TN / kWave + (TM + kWave - 1) / kWave;  // 64 scales each
+  // behind the stages the scales of the tile's outputs and of its tokens
+  static constexpr int kLds = ST * kStage + kScaleLoads * 256;
+  static constexpr bool kCut = kMost >= 4;
+  static_assert(kN * WN * 16 == TN && kMost * WM * 16 == TM && TN % 8 == 0 && kLds <= 163840);
+  static_assert(ST == 2 || ST == 4);
+  static_assert(TM % 32 == 0 && TN % kWave == 0);
 
+  const Product8Args& a;
+  char* const lds;
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int row_in = lane >> 3, chunk = (lane & 7) ^ row_in;
-  unsigned a_at[kA], b_at[kB];
-  const int8_t* a_base = a.a;
-  long long a_bytes = a.a_bytes;
-  if constexpr (!kGated) {
-    a_base += (long long)m0 * a.a_stride;
-    a_bytes -= (long long)m0 * a.a_stride;
-  }
-#pragma unroll
-  for (int i = 0; i < kA; ++i) {
-    int r = (i * kWaves + wave) * 8 + row_in;
-    if constexpr (kGated) {
-      const int p = m0 + r;
-      r = (p < m_end ? a.pairs[p] : a.pairs[m0]) / a.k;
-    }
-    a_at[i] = (unsigned)(r * a.a_stride) + 16 * chunk;
-  }
-  const int8_t* const slab = a.w + slot * a.slab_bytes;
-  const int8_t* const b_base = slab + (kGated ? 0 : n0 * a.w_stride);
-  const long long b_bytes = a.slab_bytes - (b_base - slab);
-#pragma unroll
-  for (int i = 0; i < kB; ++i) {
-    int r = (i * kWaves + wave) * 8 + row_in;
-    if constexpr (kGated) {
-      const int half = a.N / 2, of = n0 + (r & (TN / 2 - 1));
-      r = r < TN / 2 ? min(of, half - 1) : half + min(of, half - 1);
-    }
-    b_at[i] = (unsigned)(r * a.w_stride) + 16 * chunk;
-  }
-  const __amdgpu_buffer_rsrc_t a_range = range_of(a_base, a_bytes);
-  const __amdgpu_buffer_rsrc_t b_range = range_of(b_base, b_bytes);
-
+  const int wm = wave / WN, wn = wave % WN, col = lane & 15, quad = lane >> 4;
+  const int chunk = (lane & 7) ^ (lane >> 3);
   const int steps = (a.K + kStepBytes - 1) / kStepBytes;
-  const auto load = [&](int step) {
-    char* const to = lds + (step & 1) * kStage;
-    const bool behind = step * kStepBytes + 16 * chunk >= a.K;
+  const int width = kGated ? a.N / 2 : a.N;
+
+  struct Tile {
+    int slot, m0, m_end, n0;
+    __device__ __forceinline__ int rounds() const {
+      return (m_end - m0 + WM * 16 - 1) / (WM * 16);
+    }
+  };
+  unsigned a_at[kA], b_at[kB];  // a lane's bytes from a tile's first
+
+  __device__ __forceinline__ Product8(const Product8Args& args, char* to) : a(args), lds(to) {
 #pragma unroll
     for (int i = 0; i < kA; ++i)
-      load_to_lds(a_range, to + (i * kWaves + wave) * 1024, behind ? kFarOffset : a_at[i],
-                  step * kStepBytes);
+      a_at[i] = (unsigned)(((i * kWaves + wave) * 8 + (lane >> 3)) * a.a_stride) + 16 * chunk;
 #pragma unroll
-    for (int i = 0; i < kB; ++i)
-      load_to_lds(b_range, to + TM * kStepBytes + (i * kWaves + wave) * 1024, b_at[i],
-                  step * kStepBytes);
-  };
-
-  const int wm = wave / WN, wn = wave % WN, col = lane & 15, quad = lane >> 4;
-  // a wave's outputs: kN operands of 16, of a gate-up tile half of them gate and half up
-  const auto b_row = [&](int j) {
-    if constexpr (kGated)
-      return (j < kN / 2 ? 0 : TN / 2) + wn * (kN / 2) * 16 + (j % (kN / 2)) * 16;
-    else
-      return wn * kN * 16 + j * 16;
-  };
-  i32x4 acc[kM][kN] = {};
-  load(0);
-  for (int step = 0; step < steps; ++step) {
-    mem_sync();
-    if (step + 1 < steps) load(step + 1);
-    const char* const from = lds + (step & 1) * kStage;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int place = 16 * ((half * 4 + quad) ^ (col & 7));
-      i32x4 av[kM], bv[kN];
-#pragma unroll
-      for (int i = 0; i < kM; ++i)
-        av[i] = *(const i32x4*)(from + (wm * kM * 16 + i * 16 + col) * kStepBytes + place);
-#pragma unroll
-      for (int j = 0; j < kN; ++j)
-        bv[j] = *(const i32x4*)(from + (TM + b_row(j) + col) * kStepBytes + place);
-#pragma unroll
-      for (int i = 0; i < kM; ++i)
-#pragma unroll
-        for (int j = 0; j < kN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[j], av[i], acc[i][j], 0, 0, 0);
+    for (int i = 0; i < kB; ++i) {
+      const int r = (i * kWaves + wave) * 8 + (lane >> 3);
+      b_at[i] = (unsigned)((kGated && r >= TN / 2 ? width + r - TN / 2 : r) * a.w_stride) +
+                16 * chunk;
     }
   }
-  products_done();
 
+  __device__ __forceinline__ int a_row(int i) const { return (i * WM + wm) * 16; }
+  __device__ __forceinline__ int b_row(int j) const {
+    if constexpr (kGated)
+      return (j < kOut ? 0 : TN / 2) + wn * kOut * 16 + (j % kOut) * 16;
+    else
+      return wn * kN * 16 + j * 16;
+  }
+
+  // A tile, or its part `part` of 2^cut.
+  __device__ __forceinline__ Tile tile_of(int m_tile, int n_tile, int part, int cut) const {
+    Tile t = {0, m_tile * TM, a.rows, n_tile * (kGated ? TN / 2 : TN)};
+    if constexpr (kGrouped) {
+      const u32x2 of = load_uniform(reinterpret_cast<const u32x2*>(a.tiles) + m_tile);
+      t.slot = (int)of[0];
+      t.m0 = (int)of[1];
+      t.m_end = load_uniform(a.offsets + of[0] + 1);
+    }
+    t.m_end = min(t.m_end, t.m0 + TM);
+    if (cut) {
+      t.m0 += part * (TM >> cut);
+      t.m_end = max(t.m0, min(t.m_end, t.m0 + (TM >> cut)));
+    }
+    return t;
+  }
+  // The token of a row of the tile; that of its last row for those behind it.
+  __device__ __forceinline__ int token(const Tile& t, int r) const {
+    const int m = max(0, min(t.m0 + r, t.m_end - 1));
+    return kGated ? a.pairs[m] / a.k : m;
+  }
+
+  __device__ __forceinline__ void load(const Tile& t, int step) const {
+    char* const to = lds + step % ST * kStage;
+    const int rows = t.rounds() * WM * 16;
+    // the step's own offset is added behind the descriptor's check, so what is behind a row's end is
+    // sent behind the array's
+    const bool behind = step * kStepBytes + 16 * chunk >= a.K;
+    const long long skipped = kGated ? 0 : t.m0 * a.a_stride;
+    const __amdgpu_buffer_rsrc_t a_range = range_of(a.a + skipped, max(0ll, a.a_bytes - skipped));
 #pragma unroll
-  for (int i = 0; i < kM; ++i) {
-    const int m = m0 + wm * kM * 16 + i * 16 + col;
-    if (m >= m_end) continue;
-    const float row_scale = a.a_scale[kGated ? a.pairs[m] / a.k : m];
-    OUT* const out = static_cast<OUT*>(a.out) + m * a.out_stride;
-    if constexpr (kGated) {
+    for (int i = 0; i < kA; ++i)
+      if ((i * kWaves + wave) * 8 < rows)
+        load_to_lds(a_range, to + (i * kWaves + wave) * 1024, behind ? kFarOffset : a_at[i],
+                    step * kStepBytes);
+    const long long ahead = t.n0 * a.w_stride;
+    const __amdgpu_buffer_rsrc_t b_range =
+        range_of(a.w + t.slot * a.slab_bytes + ahead, max(0ll, a.slab_bytes - ahead));
 #pragma unroll
-      for (int j = 0; j < kN / 2; ++j) {
-        const int o = n0 + b_row(j) + quad * 4, half = a.N / 2;
-        if (o >= half) continue;  // half is a multiple of 16
-        const float* const gs = a.w_scale + (long long)slot * a.N + o;
-        f32x4 h;
+    for (int i = 0; i < kB; ++i)
+      if ((i + 1) * kWaves * 8 <= TN || (i * kWaves + wave) * 8 < TN)
+        load_to_lds(b_range, to + TM * kStepBytes + (i * kWaves + wave) * 1024,
+                    behind ? kFarOffset : b_at[i], step * kStepBytes);
+  }
+  // A tile's scales and its first steps.
+  __device__ __forceinline__ void load_first(const Tile& t) {
+    if constexpr (kGated)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float g = (float)acc[i][j][e] * row_scale * gs[e];
-          const float u = (float)acc[i][j + kN / 2][e] * row_scale * gs[half + e];
-          h[e] = g / (1.f + __expf(-g)) * u;
-        }
-        __builtin_memcpy(out + o, &h, 16);
+      for (int i = 0; i < kA; ++i)
+        a_at[i] = (unsigned)(token(t, (i * kWaves + wave) * 8 + (lane >> 3)) * a.a_stride) +
+                  16 * chunk;
+    char* const to = lds + ST * kStage;
+    const __amdgpu_buffer_rsrc_t w_scales = range_of(a.w_scale + (long long)t.slot * a.N, 4ll * a.N);
+    const __amdgpu_buffer_rsrc_t a_scales = range_of(a.a_scale, 4ll * a.scale_rows);
+#pragma unroll
+    for (int i = 0; i < (kScaleLoads + kWaves - 1) / kWaves; ++i) {
+      const int part = i * kWaves + wave, r = part * kWave + lane;
+      if (part < TN / kWave) {
+        const int o = t.n0 + (kGated && r >= TN / 2 ? width + r - TN / 2 : r);
+        load_word_to_lds(w_scales, to + part * 256, 4 * o);
+      } else if (part < kScaleLoads) {
+        load_word_to_lds(a_scales, to + part * 256, 4 * token(t, r - TN));
       }
-    } else {
+    }
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const int o = n0 + b_row(j) + quad * 4;
-        const float* const ws = a.w_scale + (long long)slot * a.N;
+    for (int s = 0; s < ST; ++s) load(t, s);
+  }
+
+  // The tile's product, MI rounds of it, and its results.
+  template <int MI>
+  __device__ __forceinline__ void run(const Tile& t) {
+    struct Operands {
+      i32x4 a[MI], b[kN];
+    };
+    i32x4 acc[MI][kN] = {};
+    const auto read = [&](Operands& o, int step, int half) {
+      const char* const from = lds + step % ST * kStage + col * kStepBytes +
+                               16 * ((half * 4 + quad) ^ (col & 7));
+#pragma unroll
+      for (int j = 0; j < kN; ++j) o.b[j] = *(const i32x4*)(from + (TM + b_row(j)) * kStepBytes);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) o.a[i] = *(const i32x4*)(from + a_row(i) * kStepBytes);
+    };
+    const auto multiply = [&](const Operands& o) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.b[j], o.a[i], acc[i][j], 0, 0, 0);
+    };
+    // Operands of a half step are read from LDS while the half before is multiplied. In the middle
+    // of a step its last operands have been read and the next step's loads have landed, so that
+    // behind the barrier there a later step can be loaded over it. Steps past the last load nothing,
+    // but are counted.
+    Operands even, odd;
+    load_first(t);
+    // at least so many loads a step: with as many left, all before them have landed
+    constexpr int kLoads = MI * WM * 16 / 8 / kWaves + TN / 8 / kWaves;
+    landed<(ST - 1) * kLoads>();
+    read(even, 0, 0);
+    for (int step = 0; step < steps; ++step) {
+      read(odd, step, 1);
+      multiply(even);
+      landed<(ST - 2) * kLoads>();
+      if (ST > 2 || step + ST < steps) load(t, step + ST);
+      read(even, step + 1, 0);
+      multiply(odd);
+    }
+    landed<0>();  // LDS is the next workgroup's when this one ends
+    products_done();
+
+    const char* const scales = lds + ST * kStage;
+    f32x4 scale[kN];
+    float row_scale[MI];
+#pragma unroll
+    for (int j = 0; j < kN; ++j)
+      scale[j] = *(const f32x4*)(scales + 4 * (b_row(j) + quad * 4));
+#pragma unroll
+    for (int i = 0; i < MI; ++i) row_scale[i] = *(const float*)(scales + 4 * (TN + a_row(i) + col));
+
+    // A tile's results by a descriptor that ends behind its last row. 16-bit results of a lane, four
+    // of every 16 outputs, are exchanged in the wave so that a lane has the 16 of one operand.
+    constexpr bool kShort = sizeof(OUT) == 2;
+    constexpr int kCells = kShort ? 8 : 4;           // results a store
+    constexpr int kEach = kOut * 4 / kCells;         // stores a row
+    static_assert(!kShort || kOut == 4);
+    OUT* const out = static_cast<OUT*>(a.out) + t.m0 * a.out_stride;
+    const long long stride = a.out_stride * (long long)sizeof(OUT);
+    const __amdgpu_buffer_rsrc_t range =
+        range_of(out, (t.m_end - t.m0 - 1) * stride + width * (int)sizeof(OUT));
+    int o[kEach];
+    unsigned at[kEach];
+#pragma unroll
+    for (int c = 0; c < kEach; ++c) {
+      o[c] = t.n0 + (kShort ? b_row(0) + quad * 16 + c * 8 : b_row(c) + quad * 4);
+      at[c] = t.m0 < t.m_end && o[c] < width
+                  ? (unsigned)((wm * 16 + col) * stride) + o[c] * (unsigned)sizeof(OUT)
+                  : kFarOffset;
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      u32x4 cell[kEach];
+      unsigned pair[kOut][2];
+#pragma unroll
+      for (int j = 0; j < kOut; ++j) {
+        f32x4 y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (o + e >= a.N) continue;
-          float y = (float)acc[i][j][e] * row_scale * ws[o + e];
-          if (a.bias) y += a.bias[o + e];
-          out[o + e] = from_f32<OUT>(y);
+          if constexpr (FORM == Form::kPart) {
+            y[e] = bits_as<float>(acc[i][j][e]);
+            continue;
+          }
+          y[e] = (float)acc[i][j][e] * row_scale[i] * scale[j][e];
+          if constexpr (kGated) {
+            const float u = (float)acc[i][j + kOut][e] * row_scale[i] * scale[j + kOut][e];
+            y[e] = y[e] / (1.f + __expf(-y[e])) * u;
+          }
+        }
+        if constexpr (FORM == Form::kDense)
+          if (a.bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              y[e] += a.bias[min(t.n0 + b_row(j) + quad * 4 + e, width - 1)];
+          }
+        if constexpr (kShort) {
+          pair[j][0] = two_of<OUT>(y[0], y[1]);
+          pair[j][1] = two_of<OUT>(y[2], y[3]);
+        } else {
+          cell[j] = bits_as<u32x4>(y);
+        }
+      }
+      if constexpr (kShort) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          exchange_quads(pair[0][h], pair[1][h], pair[2][h], pair[3][h]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          cell[c] = u32x4{pair[2 * c][0], pair[2 * c][1], pair[2 * c + 1][0], pair[2 * c + 1][1]};
+      }
+#pragma unroll
+      for (int c = 0; c < kEach; ++c) {
+        if (a.whole_stores) {
+          __builtin_amdgcn_raw_buffer_store_b128(cell[c], range,
+                                                 at[c] + (unsigned)(i * WM * 16 * stride), 0, 0);
+        } else if (t.m0 + a_row(i) + col < t.m_end && o[c] < width) {
+          store_piece(out + (a_row(i) + col) * a.out_stride + o[c], bits_as<Piece<OUT>>(cell[c]),
+                      width - o[c]);
         }
       }
     }
+  }
+};
+
+template <int TM, int TN, int WM, int WN, int ST, Form FORM, class OUT>
+__global__ __launch_bounds__(WM* WN* kWave) void product8_k(Product8Args a) {
+  using P = Product8<TM, TN, WM, WN, ST, FORM, OUT>;
+  __shared__ __attribute__((aligned(1024))) char lds[P::kLds];
+  // Consecutive workgroups go to the eight dies in turn: each die gets a run of tiles, so that
+  // its second-level cache holds what they share. Of its last tiles, fewer than it has compute units,
+  // each is cut in two or four where that many parts fit beside each other.
+  const int m_tiles = P::kGrouped ? load_uniform(a.n_tiles) : (a.rows + TM - 1) / TM;
+  const int splits = FORM == Form::kPart ? a.splits : 1;
+  const int n = m_tiles * a.out_tiles * splits, per = (n + 7) / 8, from = (blockIdx.x & 7) * per;
+  const int here = min(per, n - from), at = blockIdx.x >> 3;
+  if (here <= 0) return;
+  const int whole = here / kDieUnits * kDieUnits, rest = here - whole;
+  const int cut = !P::kCut ? 0 : rest * 4 <= kDieUnits ? 2 : rest * 2 <= kDieUnits ? 1 : 0;
+  if (at >= whole + (rest << cut)) return;
+  const bool part = at >= whole;
+  int tile = from + (part ? whole + ((at - whole) >> cut) : at);
+  if constexpr (FORM == Form::kPart) {
+    // neighbours have the same part of the length; whole steps, as many each but for the last
+    const int split = __builtin_amdgcn_readfirstlane(tile / (m_tiles * a.out_tiles));
+    tile -= split * m_tiles * a.out_tiles;
+    const int steps = (a.K + kStepBytes - 1) / kStepBytes;
+    const int from_k = (steps + splits - 1) / splits * split * kStepBytes;
+    a.a += from_k;
+    a.w += from_k;
+    a.a_bytes -= from_k;
+    a.slab_bytes -= from_k;
+    a.K = max(0, min(a.K - from_k, (steps + splits - 1) / splits * kStepBytes));
+    a.out = static_cast<OUT*>(a.out) + (long long)split * a.rows * a.out_stride;
+  }
+  P p(a, lds);
+  const int n_tile = __builtin_amdgcn_readfirstlane(tile / m_tiles);
+  const auto t = p.tile_of(tile - n_tile * m_tiles, n_tile, (at - whole) & ((1 << cut) - 1),
+                           part ? cut : 0);
+  // a round more than a tile needs costs no more than one that it needs: variants for all of eight
+  // would double the code for a sixteenth of a tile
+  const int rounds = t.rounds();
+  if (rounds <= 0) return;
+  if (P::kMost >= 8 && rounds > 6)
+    p.template run<P::kMost < 8 ? 1 : 8>(t);
+  else if (P::kMost >= 6 && rounds > 4)
+    p.template run<P::kMost < 6 ? 1 : 6>(t);
+  else if (P::kMost >= 4 && rounds > 2)
+    p.template run<P::kMost < 4 ? 1 : 4>(t);
+  else if (P::kMost >= 2 && rounds > 1)
+    p.template run<P::kMost < 2 ? 1 : 2>(t);
+  else
+    p.template run<1>(t);
+}
+
+// Sums of parts of the length to results: four outputs a thread.
+struct JoinArgs {
+  const int* part;       // [splits, rows, stride]
+  const float* a_scale;
+  const float* w_scale;
+  const float* bias;
+  void* out;
+  long long out_stride;
+  int splits, rows, N, stride;
+};
+constexpr int kJoinThreads = 256;
+
+template <class OUT>
+__global__ __launch_bounds__(kJoinThreads) void join8_k(JoinArgs a) {
+  const int cells = a.stride / 4;
+  const long long i = (long long)blockIdx.x * kJoinThreads + threadIdx.x;
+  const int m = (int)(i / cells), o = (int)(i - (long long)m * cells) * 4;
+  if (m >= a.rows) return;
+  i32x4 sum = {};
+  for (int s = 0; s < a.splits; ++s)
+    sum += *(const i32x4*)(a.part + ((long long)s * a.rows + m) * a.stride + o);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (o + e >= a.N) continue;
+    float y = (float)sum[e] * a.a_scale[m] * a.w_scale[o + e];
+    if (a.bias) y += a.bias[o + e];
+    static_cast<OUT*>(a.out)[m * a.out_stride + o + e] = from_f32<OUT>(y);
+  }
+}
+
+// ---- few tokens -----------------------------------------------------------------------------
+
+// Up to 16 MI tokens: a workgroup takes 16 outputs, its waves a run of the length each, and their
+// sums meet in LDS. Weights go from memory to operands and are read once, and so do tokens in 8 bits.
+// Tokens of a 16-bit type X are quantised by every workgroup for itself into LDS: for a few thousand
+// values a second launch costs more than reading again what all others read.
+constexpr int kFewWaves = 8;
+constexpr int kFewValues = 16384;  // 16-bit values that a workgroup quantises, at most
+constexpr int kFewPieces = 8;      // of 8 values, a lane
+
+// Waves that share a row of T tokens.
+__host__ __device__ constexpr int few_row_waves(int T) {
+  return T <= 1 ? 8 : T <= 2 ? 4 : T <= 4 ? 2 : 1;
+}
+__host__ __device__ constexpr int few_longest(int T) {
+  return few_row_waves(T) * kFewPieces * kWave * 8;
+}
+
+template <int MI, class X, class OUT>
+__global__ __launch_bounds__(kFewWaves* kWave) void few8_k(Product8Args a, const X* x,
+                                                           long long x_stride, int H) {
+  constexpr bool kWhole = sizeof(X) == 1;
+  static_assert(kWhole || MI == 1);
+  constexpr int kSums = kFewWaves * MI * kWave * 4;
+  // rows 16 bytes further apart than their length: 16 of them start at other banks
+  constexpr int kTokens = kWhole ? 16 : kFewValues + 16 * 32;
+  __shared__ __attribute__((aligned(16))) char lds[kSums * 4 > kTokens ? kSums * 4 : kTokens];
+  __shared__ unsigned of_wave[kFewWaves];
+  __shared__ float token_scale[16];
+  const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int col = lane & 15, quad = lane >> 4, n0 = blockIdx.x * 16;
+  // a wave's units of 64 along k, two at least where there are enough: whole lines
+  const int units = (a.K + 63) / 64;
+  int per = (units + kFewWaves - 1) / kFewWaves;
+  per += per & (per > 1);
+  const int first = wave * per, end = min(units, first + per);
+
+  const int8_t* const w = a.w + min(n0 + col, a.N - 1) * a.w_stride;
+  constexpr int kAhead = MI > 2 ? 2 : 4;  // units under way
+  i32x4 wv[kAhead], tv[kAhead][MI];
+  const auto load_weights = [&](int u) {
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) {
+      const int k = max(0, min(u + g, end - 1)) * 64 + quad * 16;
+      wv[g] = *(const i32x4*)(w + (k < a.K ? k : 0));
+    }
+  };
+  load_weights(first);
+
+  const int pitch = a.K + 16;
+  if constexpr (!kWhole) {
+    const int share = few_row_waves(a.rows), in_row = wave % share;
+    for (int row = wave / share; row < a.rows; row += kFewWaves / share) {
+      const X* const t = x + row * x_stride;
+      Piece<X> kept[kFewPieces];
+      unsigned largest = 0;
+#pragma unroll
+      for (int p = 0; p < kFewPieces; ++p) {
+        const int k = ((p * share + in_row) * kWave + lane) * 8;
+        kept[p] = k < H ? load_piece(t + k, H - k) : Piece<X>{};
+      }
+#pragma unroll
+      for (int p = 0; p < kFewPieces; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          largest = max(largest, bits_as<unsigned>(to_f32(kept[p].v[e])) & 0x7FFFFFFFu);
+      largest = ~wave_min_u32(~largest);
+      if (share > 1) {  // then there is one row a wave, and every wave is here
+        if (lane == 0) of_wave[wave] = largest;
+        lds_sync();
+        for (int v = 0; v < share; ++v) largest = max(largest, of_wave[wave - in_row + v]);
+      }
+      const Quantizer<X> quantizer(largest);
+      if (lane == 0 && in_row == 0) token_scale[row] = quantizer.scale;
+#pragma unroll
+      for (int p = 0; p < kFewPieces; ++p) {
+        const int k = ((p * share + in_row) * kWave + lane) * 8;
+        if (k >= a.K) continue;
+        unsigned q[2] = {};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e / 4] |= quantizer.of(to_f32(kept[p].v[e])) << 8 * (e % 4);
+        *(u32x2*)(lds + row * pitch + k) = u32x2{q[0], q[1]};
+      }
+    }
+    lds_sync();
+  }
+  const int8_t* t[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int row = min(i * 16 + col, a.rows - 1);
+    t[i] = kWhole ? a.a + row * a.a_stride : (const int8_t*)lds + row * pitch;
+  }
+
+  i32x4 acc[MI] = {};
+  for (int u = first; u < end; u += kAhead) {
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) {
+      const int k = min(u + g, end - 1) * 64 + quad * 16;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        tv[g][i] = *(const i32x4*)(t[i] + (k < a.K ? k : 0));
+        if (u + g >= end || k >= a.K) tv[g][i] = i32x4{};
+      }
+    }
+    if (u > first) load_weights(u);
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g)
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[g], tv[g][i], acc[i], 0, 0, 0);
+  }
+  products_done();
+  if constexpr (!kWhole) lds_sync();  // the sums go where the tokens were
+  int* const part = reinterpret_cast<int*>(lds);
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+    *(i32x4*)(part + (wave * MI + i) * 256 + lane * 4) = acc[i];
+  lds_sync();
+  // consecutive threads have consecutive outputs of a token
+  for (int i = threadIdx.x; i < MI * 256; i += kFewWaves * kWave) {
+    const int o = i % 16, m = i / 16;
+    const int at = (m >> 4) * 256 + ((o >> 2) * 16 + (m & 15)) * 4 + (o & 3);
+    if (m >= a.rows || n0 + o >= a.N) continue;
+    int sum = 0;
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) sum += part[v * MI * 256 + at];
+    float y = (float)sum * (kWhole ? a.a_scale[m] : token_scale[m]) * a.w_scale[n0 + o];
+    if (a.bias) y += a.bias[n0 + o];
+    static_cast<OUT*>(a.out)[m * a.out_stride + n0 + o] = from_f32<OUT>(y);
   }
 }
 

@@ -18,6 +18,7 @@ constexpr int kMaxTopK = 64;
 constexpr int kMaxRow = 1 << 20;        // elements of a row that is moved
 constexpr long long kMaxGrid = 0x7FFFFFFFll;
 
+long up(long v, long to) { return (v + to - 1) / to * to; }
 bool type_bad(int type) { return type < EXPERT_CACHE_F32 || type > EXPERT_CACHE_F16; }
 int size_of(int type) { return type == EXPERT_CACHE_F32 ? 4 : type == EXPERT_CACHE_INT8 ? 1 : 2; }
 
@@ -34,7 +35,7 @@ long long span(long long rows, long long stride, long long length, int size) {
 
 int sort_blocks(int n) {
   if (n <= kSortOne) return 1;
-  const int want = (n + 4095) / 4096;
+  const int want = (n + kSortLot - 1) / kSortLot;
   return want < kSortMaxBlocks ? want : kSortMaxBlocks;
 }
 
@@ -43,20 +44,26 @@ long sort_bytes(int n, int S) {
   return blocks > 1 ? 4L * blocks * (S + 1) : 0;
 }
 
+template <int W, int R, bool MANY>
+void launch_place(const SortArgs& a, int blocks, hipStream_t stream) {
+  hipLaunchKernelGGL((sort_place_k<W, R, MANY>), dim3(blocks), dim3(W * kWave), 0, stream, a);
+}
+
 int launch_sort(SortArgs a, hipStream_t stream) {
   const int blocks = sort_blocks(a.n);
-  a.chunk = (a.n + blocks - 1) / blocks;
-  // a run of 64 pairs or more a wave, and 64 KB of counts at most
-  int waves = 1;
-  while (waves < 16 && waves * kWave < a.chunk) waves *= 2;
-  const int keys = a.S + 1;
-  while ((2 + waves) * keys * 4 + 4 > 65536) waves /= 2;
-  const size_t lds = (size_t)(2 + waves) * keys * 4 + 4;
+  // whole lots, so that none but the last is short
+  a.chunk = blocks > 1 ? ((a.n - 1) / blocks / kSortLot + 1) * kSortLot : a.n;
   if (blocks > 1) {
     hipLaunchKernelGGL(sort_count_k, dim3(blocks), dim3(1024), 0, stream, a);
-    hipLaunchKernelGGL(sort_place_k<true>, dim3(blocks), dim3(waves * kWave), lds, stream, a);
+    launch_place<16, 1, true>(a, blocks, stream);
+  } else if (a.n <= 64) {
+    launch_place<1, 1, false>(a, 1, stream);
+  } else if (a.n <= 256) {
+    launch_place<4, 1, false>(a, 1, stream);
+  } else if (a.n <= 1024) {
+    launch_place<16, 1, false>(a, 1, stream);
   } else {
-    hipLaunchKernelGGL(sort_place_k<false>, dim3(1), dim3(waves * kWave), lds, stream, a);
+    launch_place<16, 4, false>(a, 1, stream);
   }
   return (int)hipGetLastError();
 }
@@ -85,21 +92,114 @@ int launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
-template <int TM, int TN, int WM, int WN, Form FORM, class OUT>
-int launch_product(const Product8Args& a, long long m_tiles, hipStream_t stream) {
-  const long long blocks = (m_tiles * a.out_tiles + 7) / 8 * 8;
+template <int TM, int TN, int WM, int WN, int ST, Form FORM, class OUT>
+int launch_product(Product8Args& a, long long m_tiles, int outputs, hipStream_t stream) {
+  a.out_tiles = (outputs + TN - 1) / TN;
+  // every die's tiles, of which the last may be cut in parts: four of less than a quarter of its units
+  const long long per = (m_tiles * a.out_tiles * (FORM == Form::kPart ? a.splits : 1) + 7) / 8;
+  const long long blocks = 8 * (per + 3 * kDieUnits / 4);
   if (blocks > kMaxGrid) return -1;
-  hipLaunchKernelGGL((product8_k<TM, TN, WM, WN, FORM, OUT>), dim3((unsigned)blocks),
+  hipLaunchKernelGGL((product8_k<TM, TN, WM, WN, ST, FORM, OUT>), dim3((unsigned)blocks),
                      dim3(WM * WN * kWave), 0, stream, a);
   return (int)hipGetLastError();
 }
 
+// How a dense product of 8-bit rows is cut, us in a graph on MI355X with quantize:
+//   side 0   16 outputs a workgroup, the length over its waves. Few tokens and outputs: 32 tokens of
+//            2048 x 2048 7.2, with tiles of 64 9.3; 48 of 4096 x 4096 14.3 and 14.4; but 16 of 4096 x
+//            14336 15.9 and 15.5, and 32 of 14336 x 4096 27.8 and 21.9.
+//   64       while all tiles are beside each other: 128 tokens of 4096 x 14336 (448 tiles) 19.4, with
+//            tiles of 128 32.2; 512 of 4096 x 4096 (512) 21.3 and 26.8; 256 of 4096 x 14336 (896)
+//            32.8 and 31.8. Long products of few tiles are cut along the length as well, at the
+//            price of a launch that joins the sums: 64 tokens of 14336 x 4096 24.2, whole 36.4, 128
+//            29.9 and 41.8; but 64 of 4096 x 4096 15.2 and 14.7, and 256 of 14336 x 4096 46.9 and 43.5.
+//   256      where there is one for every third compute unit or more: 512 of 4096 x 14336 (112 tiles'
+//            area) 44.8, with tiles of 128 45.9; 4096 of 4096 x 4096 75.5 and 100.6; 384 of 4096 x
+//            14336 (84) 43 and 37
+struct DensePlan {
+  int side, splits;
+};
+
+DensePlan dense_plan(long T, long O, long K) {
+  if (O < 8192 && (T <= 16 || (T <= 48 && K <= 4096))) return {0, 1};
+  const long of_64 = ((T + 63) / 64) * ((O + 63) / 64), steps = (K + kStepBytes - 1) / kStepBytes;
+  if (of_64 <= 512) {
+    const long beside = 256 / of_64, long_enough = steps / 8;
+    const long splits = steps < 48 ? 1 : beside < long_enough ? beside : long_enough;
+    return {64, splits < 1 ? 1 : splits > 8 ? 8 : (int)splits};
+  }
+  return {T * O >= 96L * 65536 ? 256 : 128, 1};
+}
+
+template <int MI, class X, class OUT>
+int launch_few(const Product8Args& a, const void* x, long x_stride, int H, hipStream_t stream) {
+  hipLaunchKernelGGL((few8_k<MI, X, OUT>), dim3((a.N + 15) / 16),
+                     dim3(kFewWaves * kWave), 0, stream, a, static_cast<const X*>(x),
+                     (long long)x_stride, H);
+  return (int)hipGetLastError();
+}
+
+
+
 template <class OUT>
-int launch_dense(Product8Args& a, hipStream_t stream) {
-  a.out_tiles = (a.N + 127) / 128;
-  if (a.rows <= 32)
-    return launch_product<32, 128, 1, 4, Form::kDense, OUT>(a, (a.rows + 31) / 32, stream);
-  return launch_product<128, 128, 2, 2, Form::kDense, OUT>(a, (a.rows + 127) / 128, stream);
+int launch_dense(Product8Args& a, const DensePlan& plan, int* part, hipStream_t stream) {
+  if (plan.side == 0) {
+    if (a.rows <= 16) return launch_few<1, int8_t, OUT>(a, nullptr, 0, 0, stream);
+    if (a.rows <= 32) return launch_few<2, int8_t, OUT>(a, nullptr, 0, 0, stream);
+    return launch_few<4, int8_t, OUT>(a, nullptr, 0, 0, stream);
+  }
+  const long long m_tiles = (a.rows + plan.side - 1) / plan.side;
+  if (plan.side == 256)
+    return launch_product<256, 256, 2, 4, 2, Form::kDense, OUT>(a, m_tiles, a.N, stream);
+  if (plan.side == 128)
+    return launch_product<128, 128, 2, 2, 2, Form::kDense, OUT>(a, m_tiles, a.N, stream);
+  if (plan.splits == 1)
+    return launch_product<64, 64, 4, 1, 4, Form::kDense, OUT>(a, m_tiles, a.N, stream);
+  JoinArgs j = {part, a.a_scale, a.w_scale, a.bias, a.out, a.out_stride,
+                plan.splits, a.rows, a.N, (int)up(a.N, 4)};
+  a.splits = plan.splits;
+  a.N = j.stride;
+  a.out = part;
+  a.out_stride = j.stride;
+  a.whole_stores = true;
+  const int rc = launch_product<64, 64, 4, 1, 4, Form::kPart, float>(a, m_tiles, j.N, stream);
+  if (rc) return rc;
+  const long long blocks = ((long long)j.rows * (j.stride / 4) + kJoinThreads - 1) / kJoinThreads;
+  hipLaunchKernelGGL(join8_k<OUT>, dim3((unsigned)blocks), dim3(kJoinThreads), 0, stream, j);
+  return (int)hipGetLastError();
+}
+
+template <class X>
+int launch_few_of(const Product8Args& a, int out_type, const void* x, long x_stride, int H,
+                  hipStream_t stream) {
+  if (out_type == EXPERT_CACHE_F32) return launch_few<1, X, float>(a, x, x_stride, H, stream);
+  return out_type == EXPERT_CACHE_BF16 ? launch_few<1, X, Bf16>(a, x, x_stride, H, stream)
+                                       : launch_few<1, X, F16>(a, x, x_stride, H, stream);
+}
+
+// The workspace of a projection: tokens in 8 bits and their scales, sums of parts of the length.
+struct Linear8Layout {
+  long scales, part, bytes;
+};
+
+Linear8Layout linear8_layout(const expert_cache_linear* l, int type, long T) {
+  const long K = up(l->H, 16);
+  Linear8Layout p = {};
+  if (type != EXPERT_CACHE_INT8) {
+    p.scales = up(T * K, 256);
+    p.part = p.scales + up(4 * T, 256);
+  }
+  const DensePlan plan = dense_plan(T, l->O, K);
+  p.bytes = p.part + (plan.splits > 1 ? 4L * plan.splits * T * up(l->O, 4) : 0);
+  return p;
+}
+
+// Results go 16 bytes at a time by a descriptor of a tile's rows: whole cells of a row, and a range
+// that 32 bits hold.
+bool stores_whole(const void* out, long long stride, int width, long long rows, int size) {
+  const int cell = 16 / size;
+  return width % cell == 0 && aligned16(out) && (rows == 1 || stride % cell == 0) &&
+         256 * stride * size < (long long)kMaxRange;
 }
 
 bool linear_bad(const expert_cache_linear* l, int type, int T) {
@@ -110,18 +210,23 @@ bool linear_bad(const expert_cache_linear* l, int type, int T) {
   return T < 0 || T > (1 << 24) || l->O > (1 << 24);
 }
 
-long up(long v, long to) { return (v + to - 1) / to * to; }
-
 struct Moe8Plan {
   long offsets, rows, places, counts, tiles, n_tiles, q, q_scale, h, h8, h_scale, bytes;
   long max_tiles;
   int tile_rows;
 };
 
+// Rows of the experts' tiles by the pairs a slot, us a call on MI355X: 33 tokens, 8 of 64, 2048 x 768 (4
+// a slot) 74 with 32 rows, 79 with 128; 128 of 128 (8) 144 and 136; 2048 tokens (128) 357, 291, 296
+// with 256; 8192 (512) 1142, 807, 735.
+int moe8_rows(long pairs, long slots) {
+  return pairs >= 256 * slots ? 256 : pairs > 6 * slots ? 128 : 32;
+}
+
 Moe8Plan moe8_plan(const expert_cache_experts* e, long T, long k) {
   Moe8Plan p;
   const long n = T * k;
-  p.tile_rows = n > 32L * e->S ? 128 : 32;
+  p.tile_rows = moe8_rows(n, e->S);
   p.max_tiles = n / p.tile_rows + (e->S < n ? e->S : n);
   long at = 0;
   const auto take = [&](long bytes) {
@@ -154,9 +259,12 @@ bool moe8_bad(const expert_cache_experts* e, int T, int k) {
 }
 
 template <Form FORM>
-int launch_grouped(const Product8Args& a, const Moe8Plan& p, hipStream_t stream) {
-  if (p.tile_rows == 32) return launch_product<32, 128, 1, 4, FORM, float>(a, p.max_tiles, stream);
-  return launch_product<128, 128, 2, 2, FORM, float>(a, p.max_tiles, stream);
+int launch_grouped(Product8Args& a, const Moe8Plan& p, hipStream_t stream) {
+  if (p.tile_rows == 32)
+    return launch_product<32, 128, 1, 2, 4, FORM, float>(a, p.max_tiles, a.N, stream);
+  if (p.tile_rows == 128)
+    return launch_product<128, 128, 2, 2, 2, FORM, float>(a, p.max_tiles, a.N, stream);
+  return launch_product<256, 256, 2, 4, 2, FORM, float>(a, p.max_tiles, a.N, stream);
 }
 
 }  // namespace
@@ -332,7 +440,7 @@ int expert_cache_quantize(const void* x, int type, long x_stride, int T, int H, 
 
 int expert_cache_linear8_workspace(const expert_cache_linear* l, int type, int T, long* bytes) {
   if (bytes == nullptr || linear_bad(l, type, T)) return -1;
-  *bytes = type == EXPERT_CACHE_INT8 ? 0 : up(T * up(l->H, 16), 256) + 4L * T;
+  *bytes = linear8_layout(l, type, T).bytes;
   return 0;
 }
 
@@ -349,7 +457,8 @@ int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, 
   if (whole && (!aligned16(x) || (T > 1 && (x_stride % 16 || x_stride > (1 << 22))) ||
                 x_scales == nullptr))
     return -1;
-  if (!whole && (workspace == nullptr || !aligned16(workspace))) return -1;
+  const Linear8Layout layout = linear8_layout(l, type, T);
+  if (layout.bytes > 0 && (workspace == nullptr || !aligned16(workspace))) return -1;
   const long long x_bytes = span(T, x_stride, whole ? K : l->H, size_of(type));
   const long long out_bytes = span(T, out_stride, l->O, size_of(out_type));
   if (ranges_meet(x, x_bytes, out, out_bytes) ||
@@ -359,9 +468,25 @@ int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, 
   a.a = static_cast<const int8_t*>(x);
   a.a_stride = x_stride;
   a.a_scale = x_scales;
+  a.w = static_cast<const int8_t*>(l->w);
+  a.w_stride = l->w_stride;
+  a.w_scale = l->scale;
+  a.bias = l->bias;
+  a.slab_bytes = span(l->O, l->w_stride, K, 1);
+  a.rows = T;
+  a.scale_rows = T;
+  a.N = l->O;
+  a.K = (int)K;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.whole_stores = stores_whole(out, out_stride, l->O, T, size_of(out_type));
+  if (!whole && T <= 16 && T * K <= kFewValues && K <= few_longest(T)) {
+    if (type == EXPERT_CACHE_BF16) return launch_few_of<Bf16>(a, out_type, x, x_stride, l->H, stream);
+    return launch_few_of<F16>(a, out_type, x, x_stride, l->H, stream);
+  }
   if (!whole) {
     int8_t* const q = static_cast<int8_t*>(workspace);
-    float* const scales = reinterpret_cast<float*>(q + up(T * K, 256));
+    float* const scales = reinterpret_cast<float*>(q + layout.scales);
     const QuantizeArgs z = {x, x_stride, T, l->H, nullptr, q, K, scales};
     const int rc = type == EXPERT_CACHE_BF16 ? launch_quantize<Bf16>(z, stream)
                                              : launch_quantize<F16>(z, stream);
@@ -370,20 +495,12 @@ int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, 
     a.a_stride = K;
     a.a_scale = scales;
   }
-  a.w = static_cast<const int8_t*>(l->w);
-  a.w_stride = l->w_stride;
-  a.w_scale = l->scale;
-  a.bias = l->bias;
   a.a_bytes = span(T, a.a_stride, K, 1);
-  a.slab_bytes = span(l->O, l->w_stride, K, 1);
-  a.rows = T;
-  a.N = l->O;
-  a.K = (int)K;
-  a.out = out;
-  a.out_stride = out_stride;
-  if (out_type == EXPERT_CACHE_F32) return launch_dense<float>(a, stream);
-  return out_type == EXPERT_CACHE_BF16 ? launch_dense<Bf16>(a, stream)
-                                       : launch_dense<F16>(a, stream);
+  const DensePlan plan = dense_plan(T, l->O, K);
+  int* const part = reinterpret_cast<int*>(static_cast<char*>(workspace) + layout.part);
+  if (out_type == EXPERT_CACHE_F32) return launch_dense<float>(a, plan, part, stream);
+  return out_type == EXPERT_CACHE_BF16 ? launch_dense<Bf16>(a, plan, part, stream)
+                                       : launch_dense<F16>(a, plan, part, stream);
 }
 
 int expert_cache_moe8_workspace(const expert_cache_experts* e, int T, int top_k, long* bytes) {
@@ -446,7 +563,6 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   a.rows = (int)n;
   a.N = 2 * e->I;
   a.K = e->H;
-  a.out_tiles = (e->I + 63) / 64;
   a.tiles = s.tiles;
   a.n_tiles = s.n_tiles;
   a.offsets = s.offsets;
@@ -454,6 +570,8 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   a.k = top_k;
   a.out = floats(p.h);
   a.out_stride = e->I;
+  a.scale_rows = T;
+  a.whole_stores = true;  // H and I are multiples of 16
   rc = launch_grouped<Form::kGateUp>(a, p, stream);
   if (rc) return rc;
 
@@ -471,7 +589,7 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   a.slab_bytes = (long long)e->H * e->I;
   a.N = e->H;
   a.K = e->I;
-  a.out_tiles = (e->H + 127) / 128;
+  a.scale_rows = (int)n;
   a.out_stride = e->H;
   rc = launch_grouped<Form::kDown>(a, p, stream);
   if (rc) return rc;

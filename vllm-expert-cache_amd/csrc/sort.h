@@ -2,11 +2,11 @@
 // expert_cache_dispatch, expert_cache_combine, expert_cache_combine_grad.
 //
 // Sorting is a stable counting sort of n = T * k pairs by S + 1 keys, the last for pairs that have
-// no slot. A workgroup cuts its pairs into one run a wave, counts each run's keys in LDS, and from
-// the sums over lower keys and earlier runs every wave then knows where its first pair of every key
-// goes. Within 64 pairs a lane's place is the number of equal keys in lower lanes (ballots), so no
-// place depends on the order of atomics. Many pairs take two launches: the workgroups' counts, then
-// the same with the counts of earlier workgroups added.
+// no slot. Waves take 64 pairs at a time. A lane finds the lanes with its key by a ballot for every
+// bit of the key, so its rank among the wave's equal keys is a count of lower lanes and the wave's
+// own counter in LDS: no place depends on the order of atomics. Sums of the counters over lower keys
+// and earlier waves give the places. Up to 4096 pairs are one workgroup's, their keys and ranks in
+// registers; more take a launch before that which counts every workgroup's keys.
 //
 // The rows move as they lie: `dispatch` reads a token's row once and writes it to its k places,
 // `combine` reads the k rows and sums them in 32 bits in the order of j, and `combine_grad` is a
@@ -19,7 +19,8 @@ namespace ec {
 
 constexpr int kSortMaxSlots = 1024;
 constexpr int kSortMaxPairs = 1 << 24;
-constexpr int kSortOne = 16384;     // pairs that one workgroup sorts
+constexpr int kSortOne = 4096;      // pairs that one workgroup sorts
+constexpr int kSortLot = 1024;      // pairs that a workgroup of many takes at a time
 constexpr int kSortMaxBlocks = 256;
 constexpr int kMoveWaves = 4;       // waves of a workgroup that moves rows
 
@@ -48,101 +49,151 @@ __global__ __launch_bounds__(1024) void sort_count_k(SortArgs a) {
   for (int e = threadIdx.x; e <= a.S; e += blockDim.x) count[e] = 0;
   lds_sync();
   const int first = blockIdx.x * a.chunk, end = min(a.n, first + a.chunk);
+#pragma unroll 4
   for (int i = first + threadIdx.x; i < end; i += blockDim.x) atomicAdd(&count[sort_key(a, i)], 1);
   lds_sync();
   for (int e = threadIdx.x; e <= a.S; e += blockDim.x)
     a.counts[(long long)blockIdx.x * (a.S + 1) + e] = count[e];
 }
 
-// Exclusive prefix sums of v[0..m) in place by the first wave; v[m] becomes the sum.
-__device__ __forceinline__ void sort_scan(int* v, int m) {
-  if (threadIdx.x < kWave) {
-    const int lane = threadIdx.x, per = (m + kWave - 1) / kWave;
-    const int lo = min(m, lane * per), hi = min(m, lo + per);
-    int sum = 0;
-    for (int i = lo; i < hi; ++i) sum += v[i];
-    int at = wave_incl_scan(sum) - sum;
-    for (int i = lo; i < hi; ++i) {
-      const int c = v[i];
-      v[i] = at;
-      at += c;
-    }
-    if (lane == kWave - 1) v[m] = at;
-  }
+// Sum of v over lower threads of a workgroup of W waves, and over all of them; `word` is W ints.
+template <int W>
+__device__ __forceinline__ int before_me(int v, int* word, int& all) {
+  const int wave = threadIdx.x / kWave, scan = wave_incl_scan(v);
+  lds_sync();  // word's last use
+  if (__lane_id() == kWave - 1) word[wave] = scan;
+  lds_sync();
+  int before;
+  wave_sums<W>(word, wave, before, all);
+  return before + scan - v;
 }
 
-template <bool MANY>
-__global__ __launch_bounds__(1024) void sort_place_k(SortArgs a) {
-  extern __shared__ int sort_lds[];
-  const int keys = a.S + 1, waves = blockDim.x / kWave;
-  int* const start = sort_lds;              // [keys + 1] first place of every key
-  int* const tile = start + keys + 1;       // [keys] tiles before every key's
-  int* const of_wave = tile + keys;         // [waves, keys]
-  for (int i = threadIdx.x; i < waves * keys; i += blockDim.x) of_wave[i] = 0;
-  lds_sync();
-  const int wave = threadIdx.x / kWave;
+// W waves take R x 64 W pairs at a time, wave w the w-th R x 64 of them. A pair's place is its key's
+// first place, plus the key's pairs in earlier lots, in earlier waves, in this wave's earlier
+// groups of 64, and in lower lanes.
+template <int W, int R, bool MANY>
+__global__ __launch_bounds__(W* kWave) void sort_place_k(SortArgs a) {
+  constexpr int kThreads = W * kWave, kLot = kThreads * R, kKeys = kSortMaxSlots + 1;
+  constexpr int kPer = (kSortMaxSlots + kThreads - 1) / kThreads;  // keys a thread
+  __shared__ int start[kKeys], of_wave[W * kKeys], word[W];
+  const int keys = a.S + 1, wave = threadIdx.x / kWave, lane = __lane_id();
   const int lo = blockIdx.x * a.chunk, hi = min(a.n, lo + a.chunk);
-  const int run = ((hi - lo + waves - 1) / waves + kWave - 1) / kWave * kWave;
-  const int first = min(hi, lo + wave * run), end = min(hi, first + run);
-  int* const mine = of_wave + wave * keys;
-  for (int i = first + (int)__lane_id(); i < end; i += kWave) atomicAdd(&mine[sort_key(a, i)], 1);
+  const int bits = 32 - __builtin_clz(a.S);
+  volatile int* const mine = of_wave + wave * keys;
+  int key[R], rank[R];
+  const auto take = [&](int lot) {  // keys of this wave's groups, and their ranks in the wave
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = lot + (wave * R + r) * kWave + lane;
+      key[r] = i < hi ? sort_key(a, i) : -1;
+    }
+    for (int e = lane; e < keys; e += kWave) mine[e] = 0;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const unsigned long long same = wave_match(key[r], bits);
+      if (key[r] >= 0) {
+        rank[r] = mine[key[r]] + __popcll(same & lanes_below());
+        __builtin_amdgcn_wave_barrier();
+        // the last of the equal ones counts them all
+        if ((same >> lane) == 1) mine[key[r]] = rank[r] + 1;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  // of_wave to the key's pairs in earlier waves; the key's sum
+  const auto add_waves = [&](int e) {
+    int c[W], sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) c[w] = of_wave[w * keys + e];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      of_wave[w * keys + e] = sum;
+      sum += c[w];
+    }
+    return sum;
+  };
+
+  take(lo);
   lds_sync();
-  // every wave's counts to those of the waves before it, from what earlier workgroups have
-  for (int e = threadIdx.x; e < keys; e += blockDim.x) {
-    int before = 0, all = 0;
+  // thread t has keys t * kPer and on, the last one also that of pairs without a slot; `own` are
+  // a lot's pairs, `all` those of all workgroups, `first` those of lower keys of the thread and
+  // of earlier workgroups
+  int own[kPer], all[kPer], first[kPer], sum = 0, own_none = 0, none = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int e = threadIdx.x * kPer + j;
+    own[j] = all[j] = first[j] = 0;
+    if (e < a.S) {
+      own[j] = all[j] = add_waves(e);
+      if constexpr (MANY) {
+        all[j] = 0;
+#pragma unroll 8
+        for (int b = 0; b < (int)gridDim.x; ++b) {
+          const int c = a.counts[(long long)b * keys + e];
+          first[j] += b < (int)blockIdx.x ? c : 0;
+          all[j] += c;
+        }
+      }
+    }
+    first[j] += sum;
+    sum += all[j];
+  }
+  const bool last = threadIdx.x == kThreads - 1;
+  if (last) {
+    own_none = add_waves(a.S);
     if constexpr (MANY) {
 #pragma unroll 8
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const int c = a.counts[(long long)b * keys + e];
-        before += b < (int)blockIdx.x ? c : 0;
-        all += c;
-      }
+      for (int b = 0; b < (int)blockIdx.x; ++b) none += a.counts[(long long)b * keys + a.S];
     }
-    for (int w = 0; w < waves; ++w) {
-      const int c = of_wave[w * keys + e];
-      of_wave[w * keys + e] = before;
-      before += c;
-    }
-    start[e] = MANY ? all : before;
-    tile[e] = a.tiles && e < a.S ? (start[e] + a.tile_rows - 1) / a.tile_rows : 0;
   }
-  lds_sync();
-  sort_scan(start, keys);
-  lds_sync();
+  int live;
+  const int ahead = before_me<W>(sum, word, live);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (threadIdx.x * kPer + j < a.S) start[threadIdx.x * kPer + j] = ahead + first[j];
+  if (last) start[a.S] = live + none;
   if (blockIdx.x == 0) {
-    for (int e = threadIdx.x; e < keys; e += blockDim.x) a.offsets[e] = start[e];
+    int tiles = 0, n_tiles;
+#pragma unroll
+    for (int j = 0, at = ahead; j < kPer; at += all[j++]) {
+      if (threadIdx.x * kPer + j < a.S) a.offsets[threadIdx.x * kPer + j] = at;
+      if (a.tiles) tiles += (all[j] + a.tile_rows - 1) / a.tile_rows;
+    }
+    if (last) a.offsets[a.S] = live;
     if (a.tiles) {
-      sort_scan(tile, a.S);  // tile[S] is the last key's, whose own is 0
-      lds_sync();
-      const int n = tile[a.S];
-      for (int t = threadIdx.x; t < n; t += blockDim.x) {
-        int e = 0, top = a.S - 1;  // the last slot whose tiles begin at or before t
-        while (e < top) {
-          const int mid = (e + top + 1) / 2;
-          if (tile[mid] <= t) e = mid;
-          else top = mid - 1;
-        }
-        a.tiles[t] = make_int2(e, start[e] + (t - tile[e]) * a.tile_rows);
-      }
-      if (threadIdx.x == 0) *a.n_tiles = n;
+      int t = before_me<W>(tiles, word, n_tiles);
+#pragma unroll
+      for (int j = 0, at = ahead; j < kPer; at += all[j++])
+        for (int row = 0; row < all[j]; row += a.tile_rows)
+          a.tiles[t++] = make_int2(threadIdx.x * kPer + j, at + row);
+      if (last) *a.n_tiles = n_tiles;
     }
   }
-  const int bits = 32 - __builtin_clz(a.S);
-  volatile int* const at = mine;
-  for (int base = first; base < end; base += kWave) {
-    const int i = base + (int)__lane_id();
-    const int key = i < end ? sort_key(a, i) : -1;
-    const unsigned long long same = wave_match(key, bits);
-    if (key >= 0) {
-      const int rank = __popcll(same & lanes_below());
-      const int in_key = at[key] + rank, p = start[key] + in_key;
-      __builtin_amdgcn_wave_barrier();
-      // the last of the equal ones counts them all
-      if ((same >> __lane_id()) == 1) at[key] = in_key + 1;
-      a.rows[p] = key < a.S ? i : -1;
-      a.places[i] = key < a.S ? p : -1;
+  for (int lot = lo;;) {
+    lds_sync();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (key[r] < 0) continue;
+      const int i = lot + (wave * R + r) * kWave + lane;
+      const int p = start[key[r]] + mine[key[r]] + rank[r];
+      const bool has = key[r] < a.S;
+      a.rows[p] = has ? i : -1;
+      a.places[i] = has ? p : -1;
     }
-    __builtin_amdgcn_wave_barrier();
+    lot += kLot;
+    if (!MANY || lot >= hi) break;
+    lds_sync();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (threadIdx.x * kPer + j < a.S) start[threadIdx.x * kPer + j] += own[j];
+    if (last) start[a.S] += own_none;
+    take(lot);
+    lds_sync();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (threadIdx.x * kPer + j < a.S) own[j] = add_waves(threadIdx.x * kPer + j);
+    if (last) own_none = add_waves(a.S);
   }
 }
 
@@ -158,12 +209,13 @@ struct Piece {
 
 template <class X>
 __device__ __forceinline__ Piece<X> load_piece(const X* p, long long left) {
-  Piece<X> r;
+  Piece<X> r{};
   if (left >= Piece<X>::kN) {
     __builtin_memcpy(&r, p, 16);
   } else {
-    r = Piece<X>{};
-    for (int i = 0; i < left; ++i) r.v[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < Piece<X>::kN; ++i)
+      if (i < left) r.v[i] = p[i];
   }
   return r;
 }
@@ -172,7 +224,9 @@ __device__ __forceinline__ void store_piece(X* p, const Piece<X>& r, long long l
   if (left >= Piece<X>::kN) {
     __builtin_memcpy(p, &r, 16);
   } else {
-    for (int i = 0; i < left; ++i) p[i] = r.v[i];
+#pragma unroll
+    for (int i = 0; i < Piece<X>::kN; ++i)
+      if (i < left) p[i] = r.v[i];
   }
 }
 
@@ -258,7 +312,9 @@ __global__ __launch_bounds__(kMoveWaves* kWave) void combine_k(MoveArgs a) {
   if (h + kN <= a.H) {
     __builtin_memcpy(to, &o, sizeof o);
   } else {
-    for (int i = 0; i < a.H - h; ++i) to[i] = o.v[i];
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (h + i < a.H) to[i] = o.v[i];
   }
 }
 
