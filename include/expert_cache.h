@@ -342,16 +342,18 @@ int expert_cache_sort(const void* ids, int id_bytes, int T, int top_k, int S, in
                       int* rows, int* places, void* workspace, hipStream_t stream);
 
 /*
- * Rows in the order of expert_cache_sort: out[places[t, j]] = x[t], and zeros in the rows from
- * offsets[S] on. x [T, H] and out [T * top_k, H] are of `type` (0-2), rows x_stride and out_stride
- * elements apart. Places outside [0, T * top_k) are left out. The gradient of x is
- * expert_cache_combine of out's without weights.
- * Fails with -1 unless sizes are as for expert_cache_sort, 0 < H <= 2^20, strides are at least H
- * (or there is one row), no array is null (unless T is 0), and out meets no other.
+ * Rows in the order of expert_cache_sort, from its places and rows: out[places[t, j]] = x[t], and
+ * zeros in row p where rows[p] is outside [0, T * top_k), as it is behind the last pair with a slot;
+ * places outside [0, T * top_k) are left out. x [T, H] and out [T * top_k, H] are of `type` (0-2),
+ * rows x_stride and out_stride elements apart. The gradient of x is expert_cache_combine of out's
+ * without weights.
+ * Fails with -1 unless sizes are as for expert_cache_sort, 0 < H <= 2^20, T * H < 2^43,
+ * strides are at least H (or there is one row), no array is null (unless T is 0), and out meets no
+ * other.
  */
 int expert_cache_dispatch(const void* x, int type, long x_stride, const int* places,
-                          const int* offsets, int T, int top_k, int S, int H, void* out,
-                          long out_stride, hipStream_t stream);
+                          const int* rows, int T, int top_k, int H, void* out, long out_stride,
+                          hipStream_t stream);
 
 /*
  * Back to the tokens: out[t] = sum_j weights[t, j] * y[places[t, j]], summed in 32 bits in the
@@ -364,15 +366,16 @@ int expert_cache_combine(const void* y, int type, long y_stride, const float* we
 
 /*
  * Its gradients, from grad [T, H] of out:
- *   dy[places[t, j]] = weights[t, j] * grad[t], zeros from offsets[S] on   [T * top_k, H]
+ *   dy[places[t, j]] = weights[t, j] * grad[t], zeros in row p where rows[p] is outside
+ *           [0, T * top_k)                                                      [T * top_k, H]
  *   dweights[t, j] = sum_h grad[t, h] * y[places[t, j], h], 0 without a place   float[T, top_k]
- * One of the two may be null, and y then too if it is dweights. Neither may meet an input or the
- * other. Fails with -1 as above.
+ * rows and places are expert_cache_sort's. One of the two results may be null, and y then too if it
+ * is dweights. Neither may meet an input or the other. Fails with -1 as above.
  */
 int expert_cache_combine_grad(const void* grad, int type, long grad_stride, const void* y,
                               long y_stride, const float* weights, const int* places,
-                              const int* offsets, int T, int top_k, int S, int H, void* dy,
-                              long dy_stride, float* dweights, hipStream_t stream);
+                              const int* rows, int T, int top_k, int H, void* dy, long dy_stride,
+                              float* dweights, hipStream_t stream);
 
 /*
  * Rows as 8-bit integers: m = max |x[t]|, scales[t] = m / 127, q[t] = 127 x[t] / m rounded to the

@@ -127,8 +127,10 @@ def test_sort_takes_a_column_and_strided_ids():
 
 # ---- dispatch and combine -----------------------------------------------------------------
 
-# rows of one value, below, at and past a wave's 1 KB and 4 KB, of odd length
-MOVES = [(1, 1, 1, 1), (1, 8, 64, 2048), (5, 3, 4, 7), (37, 10, 19, 1045), (16, 2, 3, 512),
+# rows of one value, below, at and past a wave's 1 KB and 4 KB, of odd length; below, at and past a
+# piece of 16 bytes; past the caches, whole and with tails
+MOVES = [(12, 3, 5, 3), (12, 3, 5, 4), (12, 3, 5, 8), (12, 3, 5, 9), (40, 8, 17, 500),
+         (3, 2, 4, 12296), (2100, 8, 16, 4104), (1, 1, 1, 1), (1, 8, 64, 2048), (5, 3, 4, 7), (37, 10, 19, 1045), (16, 2, 3, 512),
          (9, 4, 300, 513), (130, 6, 31, 2056), (3, 64, 1024, 4100), (700, 2, 8, 48)]
 
 
@@ -243,6 +245,15 @@ def test_gradients_against_differences():
             diff = float(f(*up) - f(*down)) / 2
             want = float((d.double() * (up[i].double() - down[i].double()) / 2).sum())
         assert abs(diff - want) <= 3 * (_gamma(H) + _gamma(k) + 4 * U) * size, (i, diff, want)
+
+
+def test_differentiable_once():
+    order = ops.sort(_ids(_gen(2), 5, 2, 3), 3)
+    x = torch.ones((5, 8), device=DEV, requires_grad=True)
+    y = torch.ones((10, 8), device=DEV, requires_grad=True)
+    for out, leaf in ((ops.dispatch(x, order), x), (ops.combine(y, None, order), y)):
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(out.sum(), leaf, create_graph=True)
 
 
 def test_a_weight_of_zero_hides_infinities():
@@ -367,8 +378,8 @@ def test_rows_behind_the_result_stay():
     x = _randn(g, T, H)
     lib, P = gu.lib(), ctypes.c_void_p
     wide = torch.full((T * k + 1, H + 7), 5.0, device=DEV)
-    assert lib.expert_cache_dispatch(gu.ptr(x), 0, H, gu.ptr(order.places), gu.ptr(order.offsets),
-                                     T, k, S, H, gu.ptr(wide), H + 7, gu.stream()) == 0
+    assert lib.expert_cache_dispatch(gu.ptr(x), 0, H, gu.ptr(order.places), gu.ptr(order.rows), T,
+                                     k, H, gu.ptr(wide), H + 7, gu.stream()) == 0
     torch.cuda.synchronize()
     assert (wide[:, H:] == 5).all() and (wide[T * k] == 5).all()
     assert torch.equal(wide[:T * k, :H], ops.dispatch(x, order))

@@ -53,17 +53,18 @@ def test_sort_workspace(lib):
 
 
 def _dispatch(lib, **over):
-    a = dict(x=0x10000, type=1, xs=32, places=0x20000, offsets=0x30000, T=4, k=2, S=3, H=32,
+    a = dict(x=0x10000, type=1, xs=32, places=0x20000, rows=0x30000, T=4, k=2, H=32,
              out=0x40000, os=32)
     a.update(over)
     return lib.expert_cache_dispatch(*a.values(), None)
 
 
 @pytest.mark.parametrize("over", [
-    dict(T=-1), dict(k=0), dict(k=65), dict(S=0), dict(S=1025), dict(type=-1), dict(type=3),
-    dict(H=0), dict(H=2 ** 20 + 1, xs=2 ** 21, os=2 ** 21), dict(xs=31), dict(os=31), dict(x=None),
-    dict(places=None), dict(offsets=None), dict(out=None), dict(out=0x10000 + 254),
-    dict(out=0x20000), dict(out=0x30000 + 12), dict(x=0x40000 + 8 * 64 - 2),
+    dict(T=-1), dict(k=0), dict(k=65), dict(type=-1), dict(type=3), dict(H=0),
+    dict(H=2 ** 20 + 1, xs=2 ** 21, os=2 ** 21), dict(xs=31), dict(os=31), dict(x=None),
+    dict(places=None), dict(rows=None), dict(out=None), dict(out=0x10000 + 254),
+    dict(out=0x20000 + 28), dict(out=0x30000 + 28),
+    dict(x=0x40000 + 8 * 64 - 2),
     dict(T=2 ** 24, k=1, H=2 ** 20, xs=2 ** 20, os=2 ** 20)], ids=str)
 def test_dispatch_rejects(lib, over):
     assert _dispatch(lib, **over) == -1
@@ -87,14 +88,14 @@ def test_combine_rejects(lib, over):
 
 def _combine_grad(lib, **over):
     a = dict(g=0x10000, type=1, gs=32, y=0x20000, ys=32, w=0x30000, places=0x40000,
-             offsets=0x50000, T=4, k=2, S=3, H=32, dy=0x60000, ds=32, dw=0x70000)
+             rows=0x50000, T=4, k=2, H=32, dy=0x60000, ds=32, dw=0x70000)
     a.update(over)
     return lib.expert_cache_combine_grad(*a.values(), None)
 
 
 @pytest.mark.parametrize("over", [
-    dict(T=-1), dict(k=0), dict(S=0), dict(type=3), dict(H=0), dict(gs=31), dict(ys=31),
-    dict(ds=31), dict(g=None), dict(y=None), dict(places=None), dict(offsets=None),
+    dict(T=-1), dict(k=0), dict(type=3), dict(H=0), dict(gs=31), dict(ys=31),
+    dict(ds=31), dict(g=None), dict(y=None), dict(places=None), dict(rows=None),
     dict(dy=None, dw=None), dict(dy=0x10000), dict(dy=0x20000), dict(dy=0x30000), dict(dy=0x40000),
     dict(dy=0x50000), dict(dy=0x70000), dict(dw=0x10000), dict(dw=0x20000), dict(dw=0x30000),
     dict(dw=0x40000), dict(dw=0x50000), dict(dw=0x60000 + 508)], ids=str)
@@ -188,9 +189,9 @@ def test_null_handles_are_rejected(lib):
 
 
 def test_nothing_to_do_is_no_call(lib):
-    assert _dispatch(lib, T=0, x=None, out=None, places=None, offsets=None) == 0
+    assert _dispatch(lib, T=0, x=None, out=None, places=None, rows=None) == 0
     assert _combine(lib, T=0, y=None, out=None, places=None) == 0
-    assert _combine_grad(lib, T=0, g=None, y=None, places=None, offsets=None) == 0
+    assert _combine_grad(lib, T=0, g=None, y=None, places=None, rows=None) == 0
     assert _quantize(lib, T=0, x=None, q=None, scales=None) == 0
     assert _linear(lib, T=0, x=None, out=None, work=None) == 0
     assert _moe8(lib, T=0, x=None, out=None, ids=None, work=None) == 0

@@ -6,6 +6,9 @@
 // state and allocates nothing.
 #include <hip/hip_runtime.h>
 
+#include <initializer_list>
+#include <type_traits>
+
 #include "../../include/expert_cache.h"
 #include "host.h"
 #include "int8.h"
@@ -70,12 +73,30 @@ int launch_sort(SortArgs a, hipStream_t stream) {
 
 // ---- rows ---------------------------------------------------------------------------------
 
+// Rows of more bytes than this are moved past the caches: 512 tokens' 8 rows of 2048 bf16 (17 MB) 7.5
+// us through them and 8.1 past them (combine_grad), 4096 tokens' (134 MB) 57.7 and 53.6.
+constexpr long long kOnceBytes = 64ll << 20;
+
+// Calls f with the type of the values and how their rows can be moved: those of `rows` matrices that
+// begin at p[i], stride[i] elements apart.
 template <class F>
-int with_type(int type, F&& f) {
+int with_rows(int type, int H, long long moved, std::initializer_list<const void*> p,
+              std::initializer_list<long> stride, F&& f) {
+  const int size = size_of(type), piece = 16 / size;
+  bool whole = H % piece == 0;
+  for (const void* q : p) whole = whole && aligned16(q);
+  for (long n : stride) whole = whole && n % piece == 0;
+  const auto of = [&](auto x) {
+    using std::integral_constant;
+    if (H < piece) f(x, integral_constant<Move, Move::kElements>());
+    else if (!whole) f(x, integral_constant<Move, Move::kAnywhere>());
+    else if (moved >= kOnceBytes) f(x, integral_constant<Move, Move::kOnce>());
+    else f(x, integral_constant<Move, Move::kWhole>());
+  };
   switch (type) {
-    case EXPERT_CACHE_F32: f(float{}); break;
-    case EXPERT_CACHE_BF16: f(Bf16{}); break;
-    default: f(F16{}); break;
+    case EXPERT_CACHE_F32: of(float{}); break;
+    case EXPERT_CACHE_BF16: of(Bf16{}); break;
+    default: of(F16{}); break;
   }
   return (int)hipGetLastError();
 }
@@ -306,39 +327,38 @@ int expert_cache_sort(const void* ids, int id_bytes, int T, int top_k, int S, in
 }
 
 int expert_cache_dispatch(const void* x, int type, long x_stride, const int* places,
-                          const int* offsets, int T, int top_k, int S, int H, void* out,
-                          long out_stride, hipStream_t stream) {
-  if (pairs_bad(T, top_k) || type_bad(type) || S <= 0 || S > kSortMaxSlots) return -1;
-  if (H <= 0 || H > kMaxRow) return -1;
+                          const int* rows, int T, int top_k, int H, void* out, long out_stride,
+                          hipStream_t stream) {
+  if (pairs_bad(T, top_k) || type_bad(type) || H <= 0 || H > kMaxRow) return -1;
   if (T == 0) return 0;
   const long long n = (long long)T * top_k;
   if (rows_bad(T, x, x_stride, H) || rows_bad(n, out, out_stride, H)) return -1;
-  if (places == nullptr || offsets == nullptr) return -1;
+  if (places == nullptr || rows == nullptr) return -1;
   const long long out_bytes = span(n, out_stride, H, size_of(type));
   if (ranges_meet(x, span(T, x_stride, H, size_of(type)), out, out_bytes) ||
-      ranges_meet(places, 4 * n, out, out_bytes) ||
-      ranges_meet(offsets, 4LL * (S + 1), out, out_bytes))
+      ranges_meet(places, 4 * n, out, out_bytes) || ranges_meet(rows, 4 * n, out, out_bytes))
     return -1;
   MoveArgs a = {};
   a.x = x;
   a.x_stride = x_stride;
   a.places = places;
-  a.offsets = offsets;
+  a.rows = rows;
   a.out = out;
   a.out_stride = out_stride;
   a.T = T;
   a.k = top_k;
-  a.S = S;
   a.H = H;
   a.n = (int)n;
-  const int per = 4096 / size_of(type);
+  const int per = kMovePieces * 1024 / size_of(type);
   a.chunks = (H + per - 1) / per;
   const long long blocks = ((long long)T * a.chunks + kMoveWaves - 1) / kMoveWaves;
   if (blocks > kMaxGrid) return -1;
-  return with_type(type, [&](auto v) {
-    hipLaunchKernelGGL(dispatch_k<decltype(v)>, dim3((unsigned)blocks), dim3(kMoveWaves * kWave),
-                       0, stream, a);
-  });
+  return with_rows(type, H, out_bytes, {x, out}, {T > 1 ? x_stride : 0, n > 1 ? out_stride : 0},
+                   [&](auto v, auto move) {
+                     hipLaunchKernelGGL((dispatch_k<decltype(v), move.value>),
+                                        dim3((unsigned)blocks), dim3(kMoveWaves * kWave), 0, stream,
+                                        a);
+                   });
 }
 
 int expert_cache_combine(const void* y, int type, long y_stride, const float* weights,
@@ -369,28 +389,30 @@ int expert_cache_combine(const void* y, int type, long y_stride, const float* we
   a.chunks = (H + per - 1) / per;
   const long long blocks = ((long long)T * a.chunks + kMoveWaves - 1) / kMoveWaves;
   if (blocks > kMaxGrid) return -1;
-  return with_type(type, [&](auto v) {
-    hipLaunchKernelGGL(combine_k<decltype(v)>, dim3((unsigned)blocks), dim3(kMoveWaves * kWave),
-                       0, stream, a);
-  });
+  return with_rows(type, H, span(n, y_stride, H, size_of(type)), {y, out},
+                   {n > 1 ? y_stride : 0, T > 1 ? out_stride : 0}, [&](auto v, auto move) {
+                     hipLaunchKernelGGL((combine_k<decltype(v), move.value>),
+                                        dim3((unsigned)blocks), dim3(kMoveWaves * kWave), 0, stream,
+                                        a);
+                   });
 }
 
 int expert_cache_combine_grad(const void* grad, int type, long grad_stride, const void* y,
                               long y_stride, const float* weights, const int* places,
-                              const int* offsets, int T, int top_k, int S, int H, void* dy,
-                              long dy_stride, float* dweights, hipStream_t stream) {
-  if (pairs_bad(T, top_k) || type_bad(type) || S <= 0 || S > kSortMaxSlots) return -1;
-  if (H <= 0 || H > kMaxRow || (dy == nullptr && dweights == nullptr)) return -1;
+                              const int* rows, int T, int top_k, int H, void* dy, long dy_stride,
+                              float* dweights, hipStream_t stream) {
+  if (pairs_bad(T, top_k) || type_bad(type) || H <= 0 || H > kMaxRow) return -1;
+  if (dy == nullptr && dweights == nullptr) return -1;
   if (T == 0) return 0;
   const long long n = (long long)T * top_k;
-  if (rows_bad(T, grad, grad_stride, H) || places == nullptr || offsets == nullptr) return -1;
+  if (rows_bad(T, grad, grad_stride, H) || places == nullptr || rows == nullptr) return -1;
   if (dweights && rows_bad(n, y, y_stride, H)) return -1;
   if (dy && rows_bad(n, dy, dy_stride, H)) return -1;
   const int size = size_of(type);
-  const void* const in[] = {grad, dweights ? y : nullptr, weights, places, offsets};
+  const void* const in[] = {grad, dweights ? y : nullptr, weights, places, rows};
   const long long in_bytes[] = {span(T, grad_stride, H, size),
                                 dweights ? span(n, y_stride, H, size) : 0,
-                                weights ? 4 * n : 0, 4 * n, 4LL * (S + 1)};
+                                weights ? 4 * n : 0, 4 * n, 4 * n};
   const long long dy_bytes = dy ? span(n, dy_stride, H, size) : 0;
   const long long dw_bytes = dweights ? 4 * n : 0;
   for (int i = 0; i < 5; ++i)
@@ -405,20 +427,22 @@ int expert_cache_combine_grad(const void* grad, int type, long grad_stride, cons
   a.y_stride = y_stride;
   a.weights = weights;
   a.places = places;
-  a.offsets = offsets;
+  a.rows = rows;
   a.out = dy;
   a.out_stride = dy_stride;
   a.dweights = dweights;
   a.T = T;
   a.k = top_k;
-  a.S = S;
   a.H = H;
   a.n = (int)n;
   const unsigned blocks = (unsigned)((n + kMoveWaves - 1) / kMoveWaves);
-  return with_type(type, [&](auto v) {
-    hipLaunchKernelGGL(combine_grad_k<decltype(v)>, dim3(blocks), dim3(kMoveWaves * kWave), 0,
-                       stream, a);
-  });
+  return with_rows(type, H, dy_bytes, {grad, dweights ? y : nullptr, dy},
+                   {T > 1 ? grad_stride : 0, dweights && n > 1 ? y_stride : 0,
+                    dy && n > 1 ? dy_stride : 0},
+                   [&](auto v, auto move) {
+                     hipLaunchKernelGGL((combine_grad_k<decltype(v), move.value>), dim3(blocks),
+                                        dim3(kMoveWaves * kWave), 0, stream, a);
+                   });
 }
 
 int expert_cache_quantize(const void* x, int type, long x_stride, int T, int H, void* q,
@@ -607,12 +631,14 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   m.n = (int)n;
   m.chunks = (e->H + 255) / 256;
   const long long blocks = ((long long)T * m.chunks + kMoveWaves - 1) / kMoveWaves;
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kMoveWaves * kWave), 0, stream, m);
+  };
+  const bool once = 4 * n * e->H >= kOnceBytes;
   if (e->type == EXPERT_CACHE_BF16)
-    hipLaunchKernelGGL((combine_k<float, Bf16>), dim3((unsigned)blocks), dim3(kMoveWaves * kWave),
-                       0, stream, m);
+    once ? launch(combine_k<float, Move::kOnce, Bf16>) : launch(combine_k<float, Move::kWhole, Bf16>);
   else
-    hipLaunchKernelGGL((combine_k<float, F16>), dim3((unsigned)blocks), dim3(kMoveWaves * kWave),
-                       0, stream, m);
+    once ? launch(combine_k<float, Move::kOnce, F16>) : launch(combine_k<float, Move::kWhole, F16>);
   return (int)hipGetLastError();
 }
 

@@ -9,8 +9,8 @@
 // registers; more take a launch before that which counts every workgroup's keys.
 //
 // The rows move as they lie: `dispatch` reads a token's row once and writes it to its k places,
-// `combine` reads the k rows and sums them in 32 bits in the order of j, and `combine_grad` is a
-// wave for every pair, which has the pair's gradient row and its dot product from one pass.
+// `combine` reads the k rows and sums them in 32 bits in the order of j, and `combine_grad` is a wave
+// for every pair, which has the pair's gradient row and its dot product from one pass.
 #pragma once
 #include "mfma.h"
 #include "wave.h"
@@ -240,81 +240,151 @@ struct MoveArgs {
   const void* y;        // of combine_grad: the rows that were combined
   const float* weights;
   const int* places;
-  const int* offsets;
+  const int* rows;
   void* out;
   float* dweights;
   long long x_stride, y_stride, out_stride;  // elements
-  int T, k, S, H, n, chunks;                 // n = T * k; chunks a row
+  int T, k, H, n, chunks;                    // n = T * k; chunks a row
 };
 
-// Rows of the same address pattern: out[p] = x[token] at the token's k places, zeros behind the
-// last place. A wave takes 4 KB of a token's row.
-template <class X>
-__global__ __launch_bounds__(kMoveWaves* kWave) void dispatch_k(MoveArgs a) {
-  constexpr int kN = Piece<X>::kN, kPieces = 4;
-  const long long w = (long long)blockIdx.x * kMoveWaves + threadIdx.x / kWave;
-  const int t = __builtin_amdgcn_readfirstlane((int)(w / a.chunks));
-  if (t >= a.T) return;
-  const int first = (int)(w - (long long)t * a.chunks) * (kPieces * kWave * kN) +
-                    (int)__lane_id() * kN;
-  const X* const x = static_cast<const X*>(a.x) + t * a.x_stride;
-  Piece<X> r[kPieces];
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int h = first + i * kWave * kN;
-    if (h < a.H) r[i] = load_piece(x + h, a.H - h);
-  }
-  const auto put = [&](int p) {
-    X* const to = static_cast<X*>(a.out) + (long long)p * a.out_stride;
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int h = first + i * kWave * kN;
-      if (h < a.H) store_piece(to + h, r[i], a.H - h);
+constexpr int kMovePieces = 4;  // a lane and row
+
+// How rows are loaded and stored: as whole, aligned pieces of 16 bytes, past the caches where they
+// would not stay there anyway; as pieces at any element, the last of a row moved forward to its end;
+// element by element (rows shorter than a piece).
+enum class Move { kWhole, kOnce, kAnywhere, kElements };
+
+// Where a lane's piece begins that would begin at h, and how many of its elements are the piece's
+// before it.
+template <class X, Move MOVE>
+struct Place {
+  int h, skip;
+  bool in;
+  __device__ __forceinline__ Place(int at, int H) : h(at), skip(0), in(at < H) {
+    if (MOVE == Move::kAnywhere && at > H - Piece<X>::kN) {
+      h = H - Piece<X>::kN;
+      skip = at - h;
     }
-  };
-  for (int j = 0; j < a.k; ++j) {
-    const int p = a.places[(long long)t * a.k + j];
-    if ((unsigned)p < (unsigned)a.n) put(p);
   }
-  const int live = a.offsets[a.S];
-  if (live >= a.n || live < 0) return;
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i) r[i] = Piece<X>{};
-  for (int p = live + t; p < a.n; p += a.T) put(p);
+};
+
+template <Move MOVE, class X>
+__device__ __forceinline__ Piece<X> get(const X* row, int h, int H) {
+  using Loose = u32x4 __attribute__((aligned(sizeof(X))));
+  if constexpr (MOVE == Move::kElements) return load_piece(row + h, H - h);
+  if constexpr (MOVE == Move::kAnywhere)
+    return bits_as<Piece<X>>((u32x4) * reinterpret_cast<const Loose*>(row + h));
+  return bits_as<Piece<X>>(load16_of<MOVE == Move::kOnce>(row + h));
+}
+template <Move MOVE, class X>
+__device__ __forceinline__ void put(X* row, int h, int H, const Piece<X>& r) {
+  using Loose = u32x4 __attribute__((aligned(sizeof(X))));
+  const u32x4 v = bits_as<u32x4>(r);
+  if constexpr (MOVE == Move::kElements) {
+    store_piece(row + h, r, H - h);
+  } else if constexpr (MOVE == Move::kAnywhere) {
+    *reinterpret_cast<Loose*>(row + h) = v;
+  } else if constexpr (MOVE == Move::kOnce) {
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(row + h));
+  } else {
+    *reinterpret_cast<u32x4*>(row + h) = v;
+  }
 }
 
-// out[t] = sum_j weights[t, j] x[places[t, j]]: a wave takes 1 KB of a token's row.
-template <class X, class OUT = X>
-__global__ __launch_bounds__(kMoveWaves* kWave) void combine_k(MoveArgs a) {
+// Zeros in row p: from a wave's lanes, `from` on.
+template <class X, Move MOVE>
+__device__ __forceinline__ void clear_row(const MoveArgs& a, int p, int from) {
+#pragma unroll
+  for (int i = 0; i < kMovePieces; ++i) {
+    const Place<X, MOVE> at(from + i * kWave * Piece<X>::kN, a.H);
+    if (at.in) put<MOVE>(static_cast<X*>(a.out) + (long long)p * a.out_stride, at.h, a.H, Piece<X>{});
+  }
+}
+
+// out[places[t, j]] = x[t], and zeros in rows without a pair. A wave takes 4 KB of a token's row, reads
+// it once and writes it to its k places, and looks after the rows t k to t k + k - 1 if they have no
+// pair. Front to back over the rows, 134 MB of them took 38 us and not 28.
+template <class X, Move MOVE>
+__global__ __launch_bounds__(kMoveWaves* kWave) void dispatch_k(MoveArgs a) {
   constexpr int kN = Piece<X>::kN;
   const long long w = (long long)blockIdx.x * kMoveWaves + threadIdx.x / kWave;
-  const int t = __builtin_amdgcn_readfirstlane((int)(w / a.chunks));
+  const int t = __builtin_amdgcn_readfirstlane((int)(w / a.chunks)), lane = __lane_id();
   if (t >= a.T) return;
-  const int h = (int)(w - (long long)t * a.chunks) * (kWave * kN) + (int)__lane_id() * kN;
-  float sum[kN] = {};
-  for (int j = 0; j < a.k; ++j) {
-    const long long pair = (long long)t * a.k + j;
-    const int p = a.places[pair];
-    const float weight = a.weights ? a.weights[pair] : 1.f;
-    if ((unsigned)p >= (unsigned)a.n || weight == 0.f || h >= a.H) continue;
-    const Piece<X> r =
-        load_piece(static_cast<const X*>(a.x) + (long long)p * a.x_stride + h, a.H - h);
+  const int first = (int)(w - (long long)t * a.chunks) * (kMovePieces * kWave * kN) + lane * kN;
+  const X* const x = static_cast<const X*>(a.x) + t * a.x_stride;
+  const long long pair = (long long)t * a.k + min(lane, a.k - 1);
+  const int place = a.places[pair], row = a.rows[pair];
+  Piece<X> r[kMovePieces];
 #pragma unroll
-    for (int i = 0; i < kN; ++i) sum[i] = fmaf(weight, to_f32(r.v[i]), sum[i]);
+  for (int i = 0; i < kMovePieces; ++i) {
+    const Place<X, MOVE> at(first + i * kWave * kN, a.H);
+    if (at.in) r[i] = get<MOVE == Move::kOnce ? Move::kWhole : MOVE>(x, at.h, a.H);
   }
-  if (h >= a.H) return;
-  OUT* const to = static_cast<OUT*>(a.out) + t * a.out_stride + h;
-  struct {
+  for (unsigned long long left = ballot(lane < a.k && (unsigned)place < (unsigned)a.n); left;
+       left &= left - 1) {
+    const int p = __builtin_amdgcn_readlane(place, __builtin_ctzll(left));
+    X* const to = static_cast<X*>(a.out) + (long long)p * a.out_stride;
+#pragma unroll
+    for (int i = 0; i < kMovePieces; ++i) {
+      const Place<X, MOVE> at(first + i * kWave * kN, a.H);
+      if (at.in) put<MOVE>(to, at.h, a.H, r[i]);
+    }
+  }
+  for (unsigned long long left = ballot(lane < a.k && (unsigned)row >= (unsigned)a.n); left;
+       left &= left - 1)
+    clear_row<X, MOVE>(a, t * a.k + __builtin_ctzll(left), first);
+}
+
+// out[t] = sum_j weights[t, j] x[places[t, j]], in the order of j: a wave takes 1 KB of a token's
+// row. Lane j looks up pair j, so that the rows' loads wait for one load and not for one each.
+template <class X, Move MOVE, class OUT = X>
+__global__ __launch_bounds__(kMoveWaves* kWave) void combine_k(MoveArgs a) {
+  constexpr int kN = Piece<X>::kN, kAhead = 8;
+  const long long w = (long long)blockIdx.x * kMoveWaves + threadIdx.x / kWave;
+  const int t = __builtin_amdgcn_readfirstlane((int)(w / a.chunks)), lane = __lane_id();
+  if (t >= a.T) return;
+  const Place<X, MOVE> at((int)(w - (long long)t * a.chunks) * (kWave * kN) + lane * kN, a.H);
+  const long long pair = (long long)t * a.k + min(lane, a.k - 1);
+  const int place = a.places[pair];
+  const float weight = a.weights ? a.weights[pair] : 1.f;
+  unsigned long long left =
+      ballot(lane < a.k && (unsigned)place < (unsigned)a.n && weight != 0.f);
+  if (!at.in) return;  // lanes behind a row's end, whose places and weights are still read from them
+  float sum[kN] = {};
+  while (left) {
+    Piece<X> r[kAhead];
+    float f[kAhead];
+    int taken = 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (left == 0) break;
+      const int j = __builtin_ctzll(left);
+      left &= left - 1;
+      const int p = __builtin_amdgcn_readlane(place, j);
+      f[u] = bits_as<float>(__builtin_amdgcn_readlane(bits_as<int>(weight), j));
+      r[u] = get<MOVE>(static_cast<const X*>(a.x) + (long long)p * a.x_stride, at.h, a.H);
+      ++taken;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (u < taken)
+#pragma unroll
+        for (int i = 0; i < kN; ++i) sum[i] = fmaf(f[u], to_f32(r[u].v[i]), sum[i]);
+  }
+  OUT* const to = static_cast<OUT*>(a.out) + t * a.out_stride + at.h;
+  struct Results {
     OUT v[kN];
   } o;
 #pragma unroll
   for (int i = 0; i < kN; ++i) o.v[i] = from_f32<OUT>(sum[i]);
-  if (h + kN <= a.H) {
-    __builtin_memcpy(to, &o, sizeof o);
-  } else {
+  if constexpr (MOVE == Move::kElements) {
 #pragma unroll
     for (int i = 0; i < kN; ++i)
-      if (h + i < a.H) to[i] = o.v[i];
+      if (at.h + i < a.H) to[i] = o.v[i];
+  } else if constexpr (sizeof(OUT) == sizeof(X)) {
+    put<MOVE == Move::kOnce ? Move::kWhole : MOVE>(to - at.h, at.h, a.H, bits_as<Piece<OUT>>(o));
+  } else {
+    __builtin_memcpy(to, &o, sizeof o);  // Experts8's rows, of any place
   }
 }
 
@@ -324,47 +394,55 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// For every pair (t, j): out[p] = weights[t, j] x[t] (x is the gradient of combine's result) and
-// dweights[t, j] = <x[t], y[p]>, p its place. Rows behind the last place become zeros.
-template <class X>
+// For the pair (t, j) at place p: out[p] = weights[t, j] x[t] (x is the gradient of combine's result)
+// and dweights[t, j] = <x[t], y[p]>. A wave a pair, neighbours sharing x's row; it also clears the row
+// of its own number if that has no pair. 65536 pairs of 2048 bf16 values 100 us, of which 537 MB are
+// read or written once; by places and through the caches 117.
+template <class X, Move MOVE>
 __global__ __launch_bounds__(kMoveWaves* kWave) void combine_grad_k(MoveArgs a) {
-  constexpr int kN = Piece<X>::kN;
+  constexpr int kN = Piece<X>::kN, kStep = kMovePieces * kWave * kN;
   const int pair =
       __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kMoveWaves + threadIdx.x / kWave));
   if (pair >= a.n) return;
-  const int p = a.places[pair];
-  const bool live = (unsigned)p < (unsigned)a.n;
-  const float weight = a.weights ? a.weights[pair] : 1.f;
-  const X* const g = static_cast<const X*>(a.x) + (long long)(pair / a.k) * a.x_stride;
+  const int p = load_uniform(a.places + pair), row = load_uniform(a.rows + pair);
+  const float weight = a.weights ? load_uniform(a.weights + pair) : 1.f;
+  const int lane_at = (int)__lane_id() * kN;
   float dot = 0.f;
-  if (live) {
+  if ((unsigned)p < (unsigned)a.n) {
+    const X* const g = static_cast<const X*>(a.x) + (long long)(pair / a.k) * a.x_stride;
     const X* const y = static_cast<const X*>(a.y) + (long long)p * a.y_stride;
     X* const to = static_cast<X*>(a.out) + (long long)p * a.out_stride;
-    for (int h = (int)__lane_id() * kN; h < a.H; h += kWave * kN) {
-      const Piece<X> r = load_piece(g + h, a.H - h);
-      if (a.dweights) {
-        const Piece<X> v = load_piece(y + h, a.H - h);
+    for (int from = lane_at; from < a.H; from += kStep) {
+      Piece<X> r[kMovePieces], v[kMovePieces];
 #pragma unroll
-        for (int i = 0; i < kN; ++i) dot = fmaf(to_f32(r.v[i]), to_f32(v.v[i]), dot);
+      for (int i = 0; i < kMovePieces; ++i) {
+        const Place<X, MOVE> at(from + i * kWave * kN, a.H);
+        if (!at.in) continue;
+        if (a.dweights) v[i] = get<MOVE>(y, at.h, a.H);
+        r[i] = get<MOVE == Move::kOnce ? Move::kWhole : MOVE>(g, at.h, a.H);
       }
-      if (a.out) {
+#pragma unroll
+      for (int i = 0; i < kMovePieces; ++i) {
+        const Place<X, MOVE> at(from + i * kWave * kN, a.H);
+        if (!at.in) continue;
         Piece<X> o;
 #pragma unroll
-        for (int i = 0; i < kN; ++i) o.v[i] = from_f32<X>(weight * to_f32(r.v[i]));
-        store_piece(to + h, o, a.H - h);
+        for (int e = 0; e < kN; ++e) {
+          const float x = to_f32(r[i].v[e]);
+          if (a.dweights && (MOVE != Move::kAnywhere || e >= at.skip))
+            dot = fmaf(x, to_f32(v[i].v[e]), dot);
+          o.v[e] = from_f32<X>(weight * x);
+        }
+        if (a.out) put<MOVE>(to, at.h, a.H, o);
       }
     }
   }
   if (a.dweights) {
     dot = wave_sum(dot);
-    if (__lane_id() == 0) a.dweights[pair] = live ? dot : 0.f;
+    if (__lane_id() == 0) a.dweights[pair] = dot;
   }
-  const int behind = a.offsets[a.S];
-  if (a.out && behind >= 0 && pair < a.n - behind) {
-    X* const to = static_cast<X*>(a.out) + (long long)(behind + pair) * a.out_stride;
-    for (int h = (int)__lane_id() * kN; h < a.H; h += kWave * kN)
-      store_piece(to + h, Piece<X>{}, a.H - h);
-  }
+  if (a.out && (unsigned)row >= (unsigned)a.n)
+    for (int from = lane_at; from < a.H; from += kStep) clear_row<X, MOVE>(a, pair, from);
 }
 
 }  // namespace ec

@@ -75,13 +75,13 @@ SIGNATURES = {
     "expert_cache_sort_workspace": [_I, _I, _I, _P],
     # sort(ids, id_bytes, T, top_k, S, offsets, rows, places, workspace, stream)
     "expert_cache_sort": [_P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
-    # dispatch(x, type, x_stride, places, offsets, T, top_k, S, H, out, out_stride, stream)
-    "expert_cache_dispatch": [_P, _I, _L, _P, _P, _I, _I, _I, _I, _P, _L, _P],
+    # dispatch(x, type, x_stride, places, rows, T, top_k, H, out, out_stride, stream)
+    "expert_cache_dispatch": [_P, _I, _L, _P, _P, _I, _I, _I, _P, _L, _P],
     # combine(y, type, y_stride, weights, places, T, top_k, H, out, out_stride, stream)
     "expert_cache_combine": [_P, _I, _L, _P, _P, _I, _I, _I, _P, _L, _P],
-    # combine_grad(grad, type, grad_stride, y, y_stride, weights, places, offsets, T, top_k, S, H,
+    # combine_grad(grad, type, grad_stride, y, y_stride, weights, places, rows, T, top_k, H,
     #              dy, dy_stride, dweights, stream)
-    "expert_cache_combine_grad": ([_P, _I, _L, _P, _L, _P, _P, _P] + [_I] * 4
+    "expert_cache_combine_grad": ([_P, _I, _L, _P, _L, _P, _P, _P] + [_I] * 3
                                   + [_P, _L, _P, _P]),
     # quantize(x, type, x_stride, T, H, q, q_stride, scales, stream)
     "expert_cache_quantize": [_P, _I, _L, _I, _I, _P, _L, _P, _P],

@@ -469,8 +469,8 @@ def _dispatch(x, order):
     H, n = x.shape[1], order.T * order.k
     out = x.new_empty((n, H))
     _check(_on_device(order.device, _lib.lib().expert_cache_dispatch, x.data_ptr(), kind,
-                      max(H, x.stride(0)), order.places.data_ptr(), order.offsets.data_ptr(),
-                      order.T, order.k, order.S, H, out.data_ptr(), H), "expert_cache_dispatch")
+                      max(H, x.stride(0)), order.places.data_ptr(), order.rows.data_ptr(),
+                      order.T, order.k, H, out.data_ptr(), H), "expert_cache_dispatch")
     return out
 
 
@@ -546,11 +546,17 @@ def combine_grad(grad: torch.Tensor, y: torch.Tensor | None, weights: torch.Tens
                       max(H, grad.stride(0)), None if y is None else y.data_ptr(),
                       H if y is None else max(H, y.stride(0)),
                       None if weights is None else weights.data_ptr(), order.places.data_ptr(),
-                      order.offsets.data_ptr(), order.T, order.k, order.S, H,
+                      order.rows.data_ptr(), order.T, order.k, H,
                       None if dy is None else dy.data_ptr(), H,
                       None if dweights is None else dweights.data_ptr()),
            "expert_cache_combine_grad")
     return dy, dweights
+
+
+def _once() -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError("dispatch and combine are differentiable once: their gradients have none "
+                           "(create_graph)")
 
 
 class _Dispatch(torch.autograd.Function):
@@ -560,8 +566,8 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(x, order)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _once()
         return _combine(grad, None, ctx.order), None
 
 
@@ -573,8 +579,8 @@ class _Combine(torch.autograd.Function):
         return _combine(y, weights, order)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        _once()
         y, weights = ctx.saved_tensors
         need = ctx.needs_input_grad
         return *combine_grad(grad, y, weights, ctx.order, need_y=need[0],
