@@ -66,16 +66,17 @@ struct Quantizer {
   }
 };
 
-// A row a workgroup; what fits stays in registers between the maximum and the rounding.
-template <class X>
-__global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
+// A row for every kQuantizeThreads of a workgroup of GROUPS as many, all of which come here; what fits
+// stays in registers between the maximum and the rounding.
+template <int GROUPS, class X>
+__device__ __forceinline__ void quantize_row(const QuantizeArgs& a, int row) {
   constexpr int kN = Piece<X>::kN, kKept = 4, kStride = kQuantizeThreads * kN;
-  const int row = blockIdx.x;
-  if (a.live != nullptr && row >= *a.live) return;
-  const X* const x = static_cast<const X*>(a.x) + (long long)row * a.x_stride;
+  const int thread = threadIdx.x % kQuantizeThreads, group = threadIdx.x / kQuantizeThreads;
+  const bool in = row < a.rows;
+  const X* const x = static_cast<const X*>(a.x) + (in ? row : 0) * a.x_stride;
   Piece<X> kept[kKept];
   unsigned largest = 0;
-  const int first = threadIdx.x * kN;
+  const int first = thread * kN;
   for (int i = 0, h = first; h < a.H; ++i, h += kStride) {
     const Piece<X> r = load_piece(x + h, a.H - h);
 #pragma unroll
@@ -88,11 +89,13 @@ __global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
     }
   }
   largest = ~wave_min_u32(~largest);
-  __shared__ unsigned of_wave[kQuantizeThreads / kWave];
-  if (__lane_id() == 0) of_wave[threadIdx.x / kWave] = largest;
+  constexpr int kWaves = kQuantizeThreads / kWave;
+  __shared__ unsigned of_wave[GROUPS][kWaves];
+  if (__lane_id() == 0) of_wave[group][thread / kWave] = largest;
   lds_sync();
 #pragma unroll
-  for (int w = 0; w < kQuantizeThreads / kWave; ++w) largest = max(largest, of_wave[w]);
+  for (int w = 0; w < kWaves; ++w) largest = max(largest, of_wave[group][w]);
+  if (!in) return;
   const Quantizer<X> quantizer(largest);
   int8_t* const q = a.q + (long long)row * a.q_stride;
   const int padded = (a.H + 15) & ~15;
@@ -110,8 +113,27 @@ __global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
     for (int j = 0; j < kN; ++j) packed[j / 4] |= quantizer.of(to_f32(r.v[j])) << 8 * (j % 4);
     __builtin_memcpy(q + h, packed, kN);
   }
-  if (threadIdx.x == 0) a.scales[row] = quantizer.scale;
+  if (thread == 0) a.scales[row] = quantizer.scale;
 }
+
+template <class X>
+__global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
+  if (a.live != nullptr && (int)blockIdx.x >= *a.live) return;
+  quantize_row<1, X>(a, blockIdx.x);
+}
+
+// What a layer begins with, in one launch: the pairs sorted (up to kSortOne) or their keys counted, by
+// the first workgroups, and the tokens quantised by the others, four rows each.
+template <class X, bool MANY>
+__global__ __launch_bounds__(1024) void begin8_k(SortArgs s, int sorting, QuantizeArgs q) {
+  if ((int)blockIdx.x >= sorting)
+    quantize_row<4, X>(q, (blockIdx.x - sorting) * 4 + threadIdx.x / kQuantizeThreads);
+  else if constexpr (MANY)
+    sort_count(s);
+  else
+    sort_place<16, 4, false>(s);
+}
+
 
 constexpr int kDieUnits = 32;  // compute units of a die
 
@@ -201,7 +223,6 @@ __device__ __forceinline__ void landed() {
 template <int TM, int TN, int WM, int WN, int ST, Form FORM, class OUT>
 struct Product8 {
   static constexpr int kWaves = WM * WN;
-  static constexpr int kStage = (TM + TN) * kStepBytes;
   static constexpr int kMost = TM / WM / 16;                      // rounds
   static constexpr int kA = (TM / 8 + kWaves - 1) / kWaves;       // loads a wave and step
   static constexpr int kB = (TN / 8 + kWaves - 1) / kWaves;
@@ -209,11 +230,19 @@ struct Product8 {
   static constexpr bool kGrouped = FORM == Form::kGateUp || FORM == Form::kDown, kGated = FORM == Form::kGateUp;
   static constexpr int kOut = kGated ? kN / 2 : kN;               // of them with a result
   static constexpr int kScaleLoads = TN / kWave + (TM + kWave - 1) / kWave;  // 64 scales each
-  // behind the stages the scales of the tile's outputs and of its tokens
-  static constexpr int kLds = ST * kStage + kScaleLoads * 256;
+  // A stage holds a step of a tile of MI rounds. Tiles of fewer rounds take more stages, as many as
+  // there is room for: they have less to do while loads are under way.
+  static constexpr int stage_bytes(int mi) { return (mi * WM * 16 + TN) * kStepBytes; }
+  static constexpr int kRoom = TM + TN == 512 ? 155648 : ST * stage_bytes(kMost);
+  static constexpr int stages(int mi) {
+    const int n = kRoom / stage_bytes(mi);
+    return mi == kMost ? ST : n > 4 ? 4 : n;
+  }
+  // behind them the scales of the tile's outputs and of its tokens
+  static constexpr int kLds = kRoom + kScaleLoads * 256;
   static constexpr bool kCut = kMost >= 4;
   static_assert(kN * WN * 16 == TN && kMost * WM * 16 == TM && TN % 8 == 0 && kLds <= 163840);
-  static_assert(ST == 2 || ST == 4);
+  static_assert(ST >= 2 && ST * stage_bytes(kMost) <= kRoom);
   static_assert(TM % 32 == 0 && TN % kWave == 0);
 
   const Product8Args& a;
@@ -274,8 +303,9 @@ struct Product8 {
     return kGated ? a.pairs[m] / a.k : m;
   }
 
+  template <int MI>
   __device__ __forceinline__ void load(const Tile& t, int step) const {
-    char* const to = lds + step % ST * kStage;
+    char* const to = lds + step % stages(MI) * stage_bytes(MI);
     const int rows = t.rounds() * WM * 16;
     // the step's own offset is added behind the descriptor's check, so what is behind a row's end is
     // sent behind the array's
@@ -293,17 +323,18 @@ struct Product8 {
 #pragma unroll
     for (int i = 0; i < kB; ++i)
       if ((i + 1) * kWaves * 8 <= TN || (i * kWaves + wave) * 8 < TN)
-        load_to_lds(b_range, to + TM * kStepBytes + (i * kWaves + wave) * 1024,
+        load_to_lds(b_range, to + MI * WM * 16 * kStepBytes + (i * kWaves + wave) * 1024,
                     behind ? kFarOffset : b_at[i], step * kStepBytes);
   }
   // A tile's scales and its first steps.
+  template <int MI>
   __device__ __forceinline__ void load_first(const Tile& t) {
     if constexpr (kGated)
 #pragma unroll
       for (int i = 0; i < kA; ++i)
         a_at[i] = (unsigned)(token(t, (i * kWaves + wave) * 8 + (lane >> 3)) * a.a_stride) +
                   16 * chunk;
-    char* const to = lds + ST * kStage;
+    char* const to = lds + kRoom;
     const __amdgpu_buffer_rsrc_t w_scales = range_of(a.w_scale + (long long)t.slot * a.N, 4ll * a.N);
     const __amdgpu_buffer_rsrc_t a_scales = range_of(a.a_scale, 4ll * a.scale_rows);
 #pragma unroll
@@ -317,7 +348,7 @@ struct Product8 {
       }
     }
 #pragma unroll
-    for (int s = 0; s < ST; ++s) load(t, s);
+    for (int s = 0; s < stages(MI); ++s) load<MI>(t, s);
   }
 
   // The tile's product, MI rounds of it, and its results.
@@ -326,12 +357,14 @@ struct Product8 {
     struct Operands {
       i32x4 a[MI], b[kN];
     };
+    constexpr int kStages = stages(MI);
     i32x4 acc[MI][kN] = {};
     const auto read = [&](Operands& o, int step, int half) {
-      const char* const from = lds + step % ST * kStage + col * kStepBytes +
+      const char* const from = lds + step % kStages * stage_bytes(MI) + col * kStepBytes +
                                16 * ((half * 4 + quad) ^ (col & 7));
 #pragma unroll
-      for (int j = 0; j < kN; ++j) o.b[j] = *(const i32x4*)(from + (TM + b_row(j)) * kStepBytes);
+      for (int j = 0; j < kN; ++j)
+        o.b[j] = *(const i32x4*)(from + (MI * WM * 16 + b_row(j)) * kStepBytes);
 #pragma unroll
       for (int i = 0; i < MI; ++i) o.a[i] = *(const i32x4*)(from + a_row(i) * kStepBytes);
     };
@@ -347,23 +380,23 @@ struct Product8 {
     // behind the barrier there a later step can be loaded over it. Steps past the last load nothing,
     // but are counted.
     Operands even, odd;
-    load_first(t);
+    load_first<MI>(t);
     // at least so many loads a step: with as many left, all before them have landed
     constexpr int kLoads = MI * WM * 16 / 8 / kWaves + TN / 8 / kWaves;
-    landed<(ST - 1) * kLoads>();
+    landed<(kStages - 1) * kLoads>();
     read(even, 0, 0);
     for (int step = 0; step < steps; ++step) {
       read(odd, step, 1);
       multiply(even);
-      landed<(ST - 2) * kLoads>();
-      if (ST > 2 || step + ST < steps) load(t, step + ST);
+      landed<(kStages - 2) * kLoads>();
+      if (kStages > 2 || step + kStages < steps) load<MI>(t, step + kStages);
       read(even, step + 1, 0);
       multiply(odd);
     }
     landed<0>();  // LDS is the next workgroup's when this one ends
     products_done();
 
-    const char* const scales = lds + ST * kStage;
+    const char* const scales = lds + kRoom;
     f32x4 scale[kN];
     float row_scale[MI];
 #pragma unroll
@@ -477,9 +510,15 @@ __global__ __launch_bounds__(WM* WN* kWave) void product8_k(Product8Args a) {
     a.out = static_cast<OUT*>(a.out) + (long long)split * a.rows * a.out_stride;
   }
   P p(a, lds);
-  const int n_tile = __builtin_amdgcn_readfirstlane(tile / m_tiles);
-  const auto t = p.tile_of(tile - n_tile * m_tiles, n_tile, (at - whole) & ((1 << cut) - 1),
-                           part ? cut : 0);
+  // Where a column of tiles is less than a die takes at once, it takes several side by side, so that
+  // small tiles, the last of a column, come behind the large ones of all.
+  const int side = min(a.out_tiles, (kDieUnits + m_tiles - 1) / m_tiles);
+  const int group = __builtin_amdgcn_readfirstlane(tile / (side * m_tiles));
+  const int columns = min(side, a.out_tiles - group * side);
+  const int in_group = tile - group * side * m_tiles;
+  const int m_tile = __builtin_amdgcn_readfirstlane(in_group / columns);
+  const auto t = p.tile_of(m_tile, group * side + in_group - m_tile * columns,
+                           (at - whole) & ((1 << cut) - 1), part ? cut : 0);
   // a round more than a tile needs costs no more than one that it needs: variants for all of eight
   // would double the code for a sixteenth of a tile
   const int rounds = t.rounds();

@@ -52,10 +52,15 @@ void launch_place(const SortArgs& a, int blocks, hipStream_t stream) {
   hipLaunchKernelGGL((sort_place_k<W, R, MANY>), dim3(blocks), dim3(W * kWave), 0, stream, a);
 }
 
+// Pairs a workgroup: whole lots, so that none but the last is short.
+int sort_chunk(int n) {
+  const int blocks = sort_blocks(n);
+  return blocks > 1 ? ((n - 1) / blocks / kSortLot + 1) * kSortLot : n;
+}
+
 int launch_sort(SortArgs a, hipStream_t stream) {
-  const int blocks = sort_blocks(a.n);
-  // whole lots, so that none but the last is short
-  a.chunk = blocks > 1 ? ((a.n - 1) / blocks / kSortLot + 1) * kSortLot : a.n;
+  a.chunk = sort_chunk(a.n);
+  const int blocks = a.n <= kSortOne ? 1 : (a.n - 1) / a.chunk + 1;
   if (blocks > 1) {
     hipLaunchKernelGGL(sort_count_k, dim3(blocks), dim3(1024), 0, stream, a);
     launch_place<16, 1, true>(a, blocks, stream);
@@ -110,6 +115,20 @@ bool rows_bad(long rows, const void* x, long stride, int H) {
 template <class X>
 int launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(quantize_k<X>, dim3(a.rows), dim3(kQuantizeThreads), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <class X>
+int launch_begin(const SortArgs& s, const QuantizeArgs& q, hipStream_t stream) {
+  const bool many = s.n > kSortOne;
+  const int sorting = many ? (s.n - 1) / s.chunk + 1 : 1;
+  const dim3 grid(sorting + (q.rows + 3) / 4);
+  if (many) {
+    hipLaunchKernelGGL((begin8_k<X, true>), grid, dim3(1024), 0, stream, s, sorting, q);
+    launch_place<16, 1, true>(s, sorting, stream);
+  } else {
+    hipLaunchKernelGGL((begin8_k<X, false>), grid, dim3(1024), 0, stream, s, sorting, q);
+  }
   return (int)hipGetLastError();
 }
 
@@ -237,11 +256,11 @@ struct Moe8Plan {
   int tile_rows;
 };
 
-// Rows of the experts' tiles by the pairs a slot, us a call on MI355X: 33 tokens, 8 of 64, 2048 x 768 (4
-// a slot) 74 with 32 rows, 79 with 128; 128 of 128 (8) 144 and 136; 2048 tokens (128) 357, 291, 296
-// with 256; 8192 (512) 1142, 807, 735.
+// Rows of the experts' tiles by the pairs a slot, us a call on MI355X with 64, 128 and 256 rows: 33
+// tokens, 8 of 64 slots of 2048 x 768 (4 a slot) 70, 77, 86; 128 tokens, 8 of 128 (8) 133, 134, 142;
+// 1024 (64) 196, 201, 212; 2048 (128) 285, 263, 265; 1024, 2 of 8 of 4096 x 14336 (256) -, 677, 557.
 int moe8_rows(long pairs, long slots) {
-  return pairs >= 256 * slots ? 256 : pairs > 6 * slots ? 128 : 32;
+  return pairs >= 256 * slots ? 256 : pairs > 96 * slots ? 128 : 64;
 }
 
 Moe8Plan moe8_plan(const expert_cache_experts* e, long T, long k) {
@@ -281,8 +300,8 @@ bool moe8_bad(const expert_cache_experts* e, int T, int k) {
 
 template <Form FORM>
 int launch_grouped(Product8Args& a, const Moe8Plan& p, hipStream_t stream) {
-  if (p.tile_rows == 32)
-    return launch_product<32, 128, 1, 2, 4, FORM, float>(a, p.max_tiles, a.N, stream);
+  if (p.tile_rows == 64)
+    return launch_product<64, 128, 2, 2, 2, FORM, float>(a, p.max_tiles, a.N, stream);
   if (p.tile_rows == 128)
     return launch_product<128, 128, 2, 2, 2, FORM, float>(a, p.max_tiles, a.N, stream);
   return launch_product<256, 256, 2, 4, 2, FORM, float>(a, p.max_tiles, a.N, stream);
@@ -567,12 +586,12 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   s.tiles = reinterpret_cast<int2*>(at + p.tiles);
   s.n_tiles = ints(p.n_tiles);
   s.tile_rows = p.tile_rows;
-  int rc = launch_sort(s, stream);
-  if (rc) return rc;
-
+  s.chunk = sort_chunk(s.n);
+  // few tiles: their order decides when the last one ends; many share weights with their neighbours
+  s.large_first = p.tile_rows == 256 && n / 256 * (e->H / 256) < 4 * 256;
   QuantizeArgs z = {x, x_stride, T, e->H, nullptr, bytes(p.q), e->H, floats(p.q_scale)};
-  rc = e->type == EXPERT_CACHE_BF16 ? launch_quantize<Bf16>(z, stream)
-                                    : launch_quantize<F16>(z, stream);
+  int rc = e->type == EXPERT_CACHE_BF16 ? launch_begin<Bf16>(s, z, stream)
+                                        : launch_begin<F16>(s, z, stream);
   if (rc) return rc;
 
   Product8Args a = {};

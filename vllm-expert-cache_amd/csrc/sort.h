@@ -36,6 +36,7 @@ struct SortArgs {
   int2* tiles;         // of Experts8: slot and first row of every tile, and their number
   int* n_tiles;
   int tile_rows;
+  bool large_first;    // tiles of half their rows or fewer behind all others
 };
 
 __device__ __forceinline__ int sort_key(const SortArgs& a, int i) {
@@ -44,7 +45,8 @@ __device__ __forceinline__ int sort_key(const SortArgs& a, int i) {
   return id < 0 ? a.S : id;
 }
 
-__global__ __launch_bounds__(1024) void sort_count_k(SortArgs a) {
+// The keys of a workgroup's pairs counted.
+__device__ __forceinline__ void sort_count(const SortArgs& a) {
   __shared__ int count[kSortMaxSlots + 1];
   for (int e = threadIdx.x; e <= a.S; e += blockDim.x) count[e] = 0;
   lds_sync();
@@ -72,11 +74,12 @@ __device__ __forceinline__ int before_me(int v, int* word, int& all) {
 // first place, plus the key's pairs in earlier lots, in earlier waves, in this wave's earlier
 // groups of 64, and in lower lanes.
 template <int W, int R, bool MANY>
-__global__ __launch_bounds__(W* kWave) void sort_place_k(SortArgs a) {
+__device__ __forceinline__ void sort_place(const SortArgs& a) {
   constexpr int kThreads = W * kWave, kLot = kThreads * R, kKeys = kSortMaxSlots + 1;
   constexpr int kPer = (kSortMaxSlots + kThreads - 1) / kThreads;  // keys a thread
   __shared__ int start[kKeys], of_wave[W * kKeys], word[W];
   const int keys = a.S + 1, wave = threadIdx.x / kWave, lane = __lane_id();
+  const int blocks = MANY ? (a.n - 1) / a.chunk + 1 : 1;
   const int lo = blockIdx.x * a.chunk, hi = min(a.n, lo + a.chunk);
   const int bits = 32 - __builtin_clz(a.S);
   volatile int* const mine = of_wave + wave * keys;
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(W* kWave) void sort_place_k(SortArgs a) {
       if constexpr (MANY) {
         all[j] = 0;
 #pragma unroll 8
-        for (int b = 0; b < (int)gridDim.x; ++b) {
+        for (int b = 0; b < blocks; ++b) {
           const int c = a.counts[(long long)b * keys + e];
           first[j] += b < (int)blockIdx.x ? c : 0;
           all[j] += c;
@@ -154,20 +157,28 @@ __global__ __launch_bounds__(W* kWave) void sort_place_k(SortArgs a) {
     if (threadIdx.x * kPer + j < a.S) start[threadIdx.x * kPer + j] = ahead + first[j];
   if (last) start[a.S] = live + none;
   if (blockIdx.x == 0) {
-    int tiles = 0, n_tiles;
 #pragma unroll
     for (int j = 0, at = ahead; j < kPer; at += all[j++]) {
       if (threadIdx.x * kPer + j < a.S) a.offsets[threadIdx.x * kPer + j] = at;
-      if (a.tiles) tiles += (all[j] + a.tile_rows - 1) / a.tile_rows;
     }
     if (last) a.offsets[a.S] = live;
     if (a.tiles) {
-      int t = before_me<W>(tiles, word, n_tiles);
+      int large = 0, small = 0, n_large, n_small;
+      const auto is_small = [&](int rows) { return a.large_first && 2 * rows <= a.tile_rows; };
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int part = all[j] % a.tile_rows, apart = part != 0 && is_small(part);
+        large += (all[j] + a.tile_rows - 1) / a.tile_rows - apart;
+        small += apart;
+      }
+      large = before_me<W>(large, word, n_large);
+      small = n_large + before_me<W>(small, word, n_small);
 #pragma unroll
       for (int j = 0, at = ahead; j < kPer; at += all[j++])
         for (int row = 0; row < all[j]; row += a.tile_rows)
-          a.tiles[t++] = make_int2(threadIdx.x * kPer + j, at + row);
-      if (last) *a.n_tiles = n_tiles;
+          a.tiles[is_small(all[j] - row) ? small++ : large++] =
+              make_int2(threadIdx.x * kPer + j, at + row);
+      if (last) *a.n_tiles = n_large + n_small;
     }
   }
   for (int lot = lo;;) {
@@ -195,6 +206,13 @@ __global__ __launch_bounds__(W* kWave) void sort_place_k(SortArgs a) {
       if (threadIdx.x * kPer + j < a.S) own[j] = add_waves(threadIdx.x * kPer + j);
     if (last) own_none = add_waves(a.S);
   }
+}
+
+__global__ __launch_bounds__(1024) void sort_count_k(SortArgs a) { sort_count(a); }
+
+template <int W, int R, bool MANY>
+__global__ __launch_bounds__(W* kWave) void sort_place_k(SortArgs a) {
+  sort_place<W, R, MANY>(a);
 }
 
 // ---- rows ---------------------------------------------------------------------------------
