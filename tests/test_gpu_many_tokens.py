@@ -459,7 +459,7 @@ LINEARS = [(1, 1, 1), (1, 16, 16), (2, 128, 128), (3, 129, 17), (5, 1045, 1003),
            (128, 128, 128), (129, 640, 384), (200, 96, 1000), (256, 512, 256), (257, 16, 513),
            (300, 4112, 520), (513, 1040, 1045),
            # few tokens quantised beside the product, as many values as that takes and one row more
-           (4, 4096, 40), (8, 2048, 33), (9, 2048, 33), (1, 16384, 20), (1, 16400, 20), (48, 1000, 50),
+           (3, 4096, 24), (3, 5000, 24), (2, 8192, 20), (7, 2304, 18), (4, 4096, 40), (8, 2048, 33), (9, 2048, 33), (1, 16384, 20), (1, 16400, 20), (48, 1000, 50),
            # cut along the length: 6, 3 and 8 parts, of which the last is short or empty
            (70, 6200, 130), (130, 6160, 1029), (20, 8300, 77),
            # tiles of 128 and 256: filled, ragged, odd outputs, one step and several

@@ -134,7 +134,6 @@ __global__ __launch_bounds__(1024) void begin8_k(SortArgs s, int sorting, Quanti
     sort_place<16, 4, false>(s);
 }
 
-
 constexpr int kDieUnits = 32;  // compute units of a die
 
 // ---- tiles ----------------------------------------------------------------------------------
@@ -194,7 +193,6 @@ __device__ __forceinline__ void exchange_quads(unsigned& w0, unsigned& w1, unsig
   w3 = d[1];
 }
 
-
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t range_of(const void* p, long long bytes) {
   const unsigned n = bytes < (long long)kMaxRange ? (unsigned)bytes : kMaxRange;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n, 0x00027000);
@@ -227,7 +225,7 @@ struct Product8 {
   static constexpr int kA = (TM / 8 + kWaves - 1) / kWaves;       // loads a wave and step
   static constexpr int kB = (TN / 8 + kWaves - 1) / kWaves;
   static constexpr int kN = TN / WN / 16;                         // operands a wave
-  static constexpr bool kGrouped = FORM == Form::kGateUp || FORM == Form::kDown, kGated = FORM == Form::kGateUp;
+  static constexpr bool kGated = FORM == Form::kGateUp, kGrouped = kGated || FORM == Form::kDown;
   static constexpr int kOut = kGated ? kN / 2 : kN;               // of them with a result
   static constexpr int kScaleLoads = TN / kWave + (TM + kWave - 1) / kWave;  // 64 scales each
   // A stage holds a step of a tile of MI rounds. Tiles of fewer rounds take more stages, as many as
@@ -306,7 +304,8 @@ struct Product8 {
   template <int MI>
   __device__ __forceinline__ void load(const Tile& t, int step) const {
     char* const to = lds + step % stages(MI) * stage_bytes(MI);
-    const int rows = t.rounds() * WM * 16;
+    // all rows of MI rounds, though the tile may have fewer: a wave's loads are counted
+    constexpr int kRows = MI * WM * 16;
     // the step's own offset is added behind the descriptor's check, so what is behind a row's end is
     // sent behind the array's
     const bool behind = step * kStepBytes + 16 * chunk >= a.K;
@@ -314,7 +313,7 @@ struct Product8 {
     const __amdgpu_buffer_rsrc_t a_range = range_of(a.a + skipped, max(0ll, a.a_bytes - skipped));
 #pragma unroll
     for (int i = 0; i < kA; ++i)
-      if ((i * kWaves + wave) * 8 < rows)
+      if ((i + 1) * kWaves * 8 <= kRows || (i * kWaves + wave) * 8 < kRows)
         load_to_lds(a_range, to + (i * kWaves + wave) * 1024, behind ? kFarOffset : a_at[i],
                     step * kStepBytes);
     const long long ahead = t.n0 * a.w_stride;
@@ -617,8 +616,10 @@ __global__ __launch_bounds__(kFewWaves* kWave) void few8_k(Product8Args a, const
   const int pitch = a.K + 16;
   if constexpr (!kWhole) {
     const int share = few_row_waves(a.rows), in_row = wave % share;
-    for (int row = wave / share; row < a.rows; row += kFewWaves / share) {
-      const X* const t = x + row * x_stride;
+    // as often in every wave, also in those that have no row
+    for (int from = 0; from < a.rows; from += kFewWaves / share) {
+      const int row = from + wave / share;
+      const X* const t = x + min(row, a.rows - 1) * x_stride;
       Piece<X> kept[kFewPieces];
       unsigned largest = 0;
 #pragma unroll
@@ -632,11 +633,12 @@ __global__ __launch_bounds__(kFewWaves* kWave) void few8_k(Product8Args a, const
         for (int e = 0; e < 8; ++e)
           largest = max(largest, bits_as<unsigned>(to_f32(kept[p].v[e])) & 0x7FFFFFFFu);
       largest = ~wave_min_u32(~largest);
-      if (share > 1) {  // then there is one row a wave, and every wave is here
+      if (share > 1) {
         if (lane == 0) of_wave[wave] = largest;
         lds_sync();
         for (int v = 0; v < share; ++v) largest = max(largest, of_wave[wave - in_row + v]);
       }
+      if (row >= a.rows) continue;
       const Quantizer<X> quantizer(largest);
       if (lane == 0 && in_row == 0) token_scale[row] = quantizer.scale;
 #pragma unroll

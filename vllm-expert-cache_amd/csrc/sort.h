@@ -367,7 +367,8 @@ __global__ __launch_bounds__(kMoveWaves* kWave) void combine_k(MoveArgs a) {
   const float weight = a.weights ? a.weights[pair] : 1.f;
   unsigned long long left =
       ballot(lane < a.k && (unsigned)place < (unsigned)a.n && weight != 0.f);
-  if (!at.in) return;  // lanes behind a row's end, whose places and weights are still read from them
+  // lanes behind a row's end stay, since their places and weights are read, and load its first piece
+  const int h = at.in ? at.h : 0;
   float sum[kN] = {};
   while (left) {
     Piece<X> r[kAhead];
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(kMoveWaves* kWave) void combine_k(MoveArgs a) {
       left &= left - 1;
       const int p = __builtin_amdgcn_readlane(place, j);
       f[u] = bits_as<float>(__builtin_amdgcn_readlane(bits_as<int>(weight), j));
-      r[u] = get<MOVE>(static_cast<const X*>(a.x) + (long long)p * a.x_stride, at.h, a.H);
+      r[u] = get<MOVE>(static_cast<const X*>(a.x) + (long long)p * a.x_stride, h, a.H);
       ++taken;
     }
 #pragma unroll
@@ -389,6 +390,7 @@ __global__ __launch_bounds__(kMoveWaves* kWave) void combine_k(MoveArgs a) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) sum[i] = fmaf(f[u], to_f32(r[u].v[i]), sum[i]);
   }
+  if (!at.in) return;
   OUT* const to = static_cast<OUT*>(a.out) + t * a.out_stride + at.h;
   struct Results {
     OUT v[kN];
