@@ -68,26 +68,28 @@ struct Quantizer {
 
 // A row for every kQuantizeThreads of a workgroup of GROUPS as many, all of which come here; what fits
 // stays in registers between the maximum and the rounding.
-template <int GROUPS, class X>
+template <int GROUPS, int KEPT, class X>
 __device__ __forceinline__ void quantize_row(const QuantizeArgs& a, int row) {
-  constexpr int kN = Piece<X>::kN, kKept = 4, kStride = kQuantizeThreads * kN;
+  constexpr int kN = Piece<X>::kN, kKept = KEPT, kStride = kQuantizeThreads * kN;
   const int thread = threadIdx.x % kQuantizeThreads, group = threadIdx.x / kQuantizeThreads;
   const bool in = row < a.rows;
   const X* const x = static_cast<const X*>(a.x) + (in ? row : 0) * a.x_stride;
   Piece<X> kept[kKept];
   unsigned largest = 0;
   const int first = thread * kN;
-  for (int i = 0, h = first; h < a.H; ++i, h += kStride) {
-    const Piece<X> r = load_piece(x + h, a.H - h);
+  const auto look = [&](const Piece<X>& r) {
 #pragma unroll
     for (int j = 0; j < kN; ++j)
       largest = max(largest, bits_as<unsigned>(to_f32(r.v[j])) & 0x7FFFFFFFu);
-    if (i < kKept) {
+  };
 #pragma unroll
-      for (int m = 0; m < kKept; ++m)
-        if (m == i) kept[m] = r;
-    }
+  for (int i = 0; i < kKept; ++i) {
+    const int h = first + i * kStride;
+    kept[i] = h < a.H ? load_piece(x + h, a.H - h) : Piece<X>{};
   }
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) look(kept[i]);
+  for (int h = first + kKept * kStride; h < a.H; h += kStride) look(load_piece(x + h, a.H - h));
   largest = ~wave_min_u32(~largest);
   constexpr int kWaves = kQuantizeThreads / kWave;
   __shared__ unsigned of_wave[GROUPS][kWaves];
@@ -99,39 +101,36 @@ __device__ __forceinline__ void quantize_row(const QuantizeArgs& a, int row) {
   const Quantizer<X> quantizer(largest);
   int8_t* const q = a.q + (long long)row * a.q_stride;
   const int padded = (a.H + 15) & ~15;
-  for (int i = 0, h = first; h < padded; ++i, h += kStride) {
-    Piece<X> r{};
-    if (i < kKept) {
-#pragma unroll
-      for (int m = 0; m < kKept; ++m)
-        if (m == i && h < a.H) r = kept[m];
-    } else if (h < a.H) {
-      r = load_piece(x + h, a.H - h);
-    }
+  const auto write = [&](int h, const Piece<X>& r) {
     unsigned packed[kN / 4] = {};
 #pragma unroll
     for (int j = 0; j < kN; ++j) packed[j / 4] |= quantizer.of(to_f32(r.v[j])) << 8 * (j % 4);
     __builtin_memcpy(q + h, packed, kN);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (first + i * kStride < padded) write(first + i * kStride, kept[i]);
+  for (int h = first + kKept * kStride; h < padded; h += kStride)
+    write(h, h < a.H ? load_piece(x + h, a.H - h) : Piece<X>{});
   if (thread == 0) a.scales[row] = quantizer.scale;
 }
 
-template <class X>
+template <int KEPT, class X>
 __global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
   if (a.live != nullptr && (int)blockIdx.x >= *a.live) return;
-  quantize_row<1, X>(a, blockIdx.x);
+  quantize_row<1, KEPT, X>(a, blockIdx.x);
 }
 
-// What a layer begins with, in one launch: the pairs sorted (up to kSortOne) or their keys counted, by
+// What a layer begins with, in one launch: the pairs sorted (up to 1024 R) or their keys counted, by
 // the first workgroups, and the tokens quantised by the others, four rows each.
-template <class X, bool MANY>
+template <int R, class X, bool MANY>
 __global__ __launch_bounds__(1024) void begin8_k(SortArgs s, int sorting, QuantizeArgs q) {
   if ((int)blockIdx.x >= sorting)
-    quantize_row<4, X>(q, (blockIdx.x - sorting) * 4 + threadIdx.x / kQuantizeThreads);
+    quantize_row<4, 2, X>(q, (blockIdx.x - sorting) * 4 + threadIdx.x / kQuantizeThreads);
   else if constexpr (MANY)
     sort_count(s);
   else
-    sort_place<16, 4, false>(s);
+    sort_place<16, R, false>(s);
 }
 
 constexpr int kDieUnits = 32;  // compute units of a die

@@ -114,7 +114,15 @@ bool rows_bad(long rows, const void* x, long stride, int H) {
 
 template <class X>
 int launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL(quantize_k<X>, dim3(a.rows), dim3(kQuantizeThreads), 0, stream, a);
+  // as many pieces of 16 bytes a thread kept as the row has
+  const int pieces = (a.H * (int)sizeof(X) + 16 * kQuantizeThreads - 1) / (16 * kQuantizeThreads);
+  const dim3 grid(a.rows), block(kQuantizeThreads);
+  if (pieces <= 1)
+    hipLaunchKernelGGL((quantize_k<1, X>), grid, block, 0, stream, a);
+  else if (pieces <= 4)
+    hipLaunchKernelGGL((quantize_k<4, X>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((quantize_k<16, X>), grid, block, 0, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -124,10 +132,12 @@ int launch_begin(const SortArgs& s, const QuantizeArgs& q, hipStream_t stream) {
   const int sorting = many ? (s.n - 1) / s.chunk + 1 : 1;
   const dim3 grid(sorting + (q.rows + 3) / 4);
   if (many) {
-    hipLaunchKernelGGL((begin8_k<X, true>), grid, dim3(1024), 0, stream, s, sorting, q);
+    hipLaunchKernelGGL((begin8_k<1, X, true>), grid, dim3(1024), 0, stream, s, sorting, q);
     launch_place<16, 1, true>(s, sorting, stream);
+  } else if (s.n > 1024) {
+    hipLaunchKernelGGL((begin8_k<4, X, false>), grid, dim3(1024), 0, stream, s, sorting, q);
   } else {
-    hipLaunchKernelGGL((begin8_k<X, false>), grid, dim3(1024), 0, stream, s, sorting, q);
+    hipLaunchKernelGGL((begin8_k<1, X, false>), grid, dim3(1024), 0, stream, s, sorting, q);
   }
   return (int)hipGetLastError();
 }
