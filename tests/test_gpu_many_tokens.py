@@ -419,7 +419,8 @@ def _hard_rows(g, T, H, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("T,H", [(1, 1), (7, 16), (15, 1045), (29, 2048), (8, 8192), (8, 8200),
-                                 (9, 14336), (3, 40009), (600, 129)])
+                                 (9, 14336), (3, 40009), (600, 129), (1025, 129), (1026, 2049),
+                                 (1030, 4096), (1024, 4097)])
 def test_quantize(T, H, dtype):
     x = _hard_rows(_gen(T + H), T, H, dtype)
     q, scales = ops.quantize(x)

@@ -39,7 +39,7 @@ struct QuantizeArgs {
   float* scales;
 };
 
-constexpr int kQuantizeThreads = 256;
+constexpr int kQuantizeThreads = 256;  // of a workgroup
 
 // q = rint(127 x / m), m the row's largest magnitude. Rows below 2^-119 count as zeros; one with an
 // infinity or NaN gets a scale of NaN and zeros, so that whatever it is multiplied with shows it.
@@ -66,12 +66,12 @@ struct Quantizer {
   }
 };
 
-// A row for every kQuantizeThreads of a workgroup of GROUPS as many, all of which come here; what fits
-// stays in registers between the maximum and the rounding.
-template <int GROUPS, int KEPT, class X>
+// A row for every THREADS of a workgroup of GROUPS as many, all of which come here; KEPT pieces a thread
+// stay in registers between the maximum and the rounding.
+template <int THREADS, int GROUPS, int KEPT, class X>
 __device__ __forceinline__ void quantize_row(const QuantizeArgs& a, int row) {
-  constexpr int kN = Piece<X>::kN, kKept = KEPT, kStride = kQuantizeThreads * kN;
-  const int thread = threadIdx.x % kQuantizeThreads, group = threadIdx.x / kQuantizeThreads;
+  constexpr int kN = Piece<X>::kN, kKept = KEPT, kStride = THREADS * kN;
+  const int thread = threadIdx.x % THREADS, group = threadIdx.x / THREADS;
   const bool in = row < a.rows;
   const X* const x = static_cast<const X*>(a.x) + (in ? row : 0) * a.x_stride;
   Piece<X> kept[kKept];
@@ -91,12 +91,14 @@ __device__ __forceinline__ void quantize_row(const QuantizeArgs& a, int row) {
   for (int i = 0; i < kKept; ++i) look(kept[i]);
   for (int h = first + kKept * kStride; h < a.H; h += kStride) look(load_piece(x + h, a.H - h));
   largest = ~wave_min_u32(~largest);
-  constexpr int kWaves = kQuantizeThreads / kWave;
-  __shared__ unsigned of_wave[GROUPS][kWaves];
-  if (__lane_id() == 0) of_wave[group][thread / kWave] = largest;
-  lds_sync();
+  constexpr int kWaves = THREADS / kWave;
+  if constexpr (kWaves > 1) {
+    __shared__ unsigned of_wave[GROUPS][kWaves];
+    if (__lane_id() == 0) of_wave[group][thread / kWave] = largest;
+    lds_sync();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) largest = max(largest, of_wave[group][w]);
+    for (int w = 0; w < kWaves; ++w) largest = max(largest, of_wave[group][w]);
+  }
   if (!in) return;
   const Quantizer<X> quantizer(largest);
   int8_t* const q = a.q + (long long)row * a.q_stride;
@@ -115,10 +117,12 @@ __device__ __forceinline__ void quantize_row(const QuantizeArgs& a, int row) {
   if (thread == 0) a.scales[row] = quantizer.scale;
 }
 
-template <int KEPT, class X>
+template <int THREADS, int KEPT, class X>
 __global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
-  if (a.live != nullptr && (int)blockIdx.x >= *a.live) return;
-  quantize_row<1, KEPT, X>(a, blockIdx.x);
+  constexpr int kRows = kQuantizeThreads / THREADS;
+  if (a.live != nullptr) a.rows = min(a.rows, load_uniform(a.live));
+  if ((int)blockIdx.x * kRows >= a.rows) return;
+  quantize_row<THREADS, kRows, KEPT, X>(a, blockIdx.x * kRows + threadIdx.x / THREADS);
 }
 
 // What a layer begins with, in one launch: the pairs sorted (up to 1024 R) or their keys counted, by
@@ -126,7 +130,7 @@ __global__ __launch_bounds__(kQuantizeThreads) void quantize_k(QuantizeArgs a) {
 template <int R, class X, bool MANY>
 __global__ __launch_bounds__(1024) void begin8_k(SortArgs s, int sorting, QuantizeArgs q) {
   if ((int)blockIdx.x >= sorting)
-    quantize_row<4, 2, X>(q, (blockIdx.x - sorting) * 4 + threadIdx.x / kQuantizeThreads);
+    quantize_row<256, 4, 2, X>(q, (blockIdx.x - sorting) * 4 + threadIdx.x / 256);
   else if constexpr (MANY)
     sort_count(s);
   else

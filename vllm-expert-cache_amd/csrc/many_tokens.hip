@@ -114,15 +114,18 @@ bool rows_bad(long rows, const void* x, long stride, int H) {
 
 template <class X>
 int launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
-  // as many pieces of 16 bytes a thread kept as the row has
-  const int pieces = (a.H * (int)sizeof(X) + 16 * kQuantizeThreads - 1) / (16 * kQuantizeThreads);
-  const dim3 grid(a.rows), block(kQuantizeThreads);
-  if (pieces <= 1)
-    hipLaunchKernelGGL((quantize_k<1, X>), grid, block, 0, stream, a);
-  else if (pieces <= 4)
-    hipLaunchKernelGGL((quantize_k<4, X>), grid, block, 0, stream, a);
+  // A wave a row where rows are many and short, else a workgroup: 16384 rows of 768 floats 13.0 us, by
+  // workgroups 16.1; 4096 rows of 4096 bf16 16.5 and 14.0.
+  const long bytes = (long)a.H * sizeof(X);
+  const dim3 block(kQuantizeThreads), all(a.rows), quarter((a.rows + 3) / 4);
+  if (a.rows >= 1024 && bytes <= 4096)
+    hipLaunchKernelGGL((quantize_k<64, 4, X>), quarter, block, 0, stream, a);
+  else if (bytes <= 4096)
+    hipLaunchKernelGGL((quantize_k<256, 1, X>), all, block, 0, stream, a);
+  else if (bytes <= 16384)
+    hipLaunchKernelGGL((quantize_k<256, 4, X>), all, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((quantize_k<16, X>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((quantize_k<256, 16, X>), all, block, 0, stream, a);
   return (int)hipGetLastError();
 }
 

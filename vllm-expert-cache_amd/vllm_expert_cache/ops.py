@@ -456,15 +456,14 @@ def dispatch(x: torch.Tensor, order: Order) -> torch.Tensor:
     Differentiable in x, once: a token's gradient is the 32-bit sum of its rows', rounded to x's
     type. `combine(gradient, None, order)` is the same without autograd, for a call that is
     captured; one that autograd would record is refused then."""
-    if torch.is_grad_enabled() and x.requires_grad:
-        _movable(x, order.T, order, "x")
-        _recordable()
-        return _Dispatch.apply(x, order)
-    return _dispatch(x, order)
-
-
-def _dispatch(x, order):
     kind = _movable(x, order.T, order, "x")
+    if x.requires_grad and torch.is_grad_enabled():
+        _recordable()
+        return _Dispatch.apply(x, order, kind)
+    return _dispatch(x, order, kind)
+
+
+def _dispatch(x, order, kind):
     x = _pitched(x)
     H, n = x.shape[1], order.T * order.k
     out = x.new_empty((n, H))
@@ -482,12 +481,12 @@ def combine(y: torch.Tensor, weights: torch.Tensor | None, order: Order) -> torc
 
     Differentiable in y and weights, once (`combine_grad` is the same without autograd, for a call
     that is captured; one that autograd would record is refused then)."""
-    if torch.is_grad_enabled() and (y.requires_grad or
-                                    (weights is not None and weights.requires_grad)):
-        _combine_args(y, weights, order)
+    kind = _combine_args(y, weights, order)
+    if (y.requires_grad or (weights is not None and weights.requires_grad)) and \
+            torch.is_grad_enabled():
         _recordable()
-        return _Combine.apply(y, weights, order)
-    return _combine(y, weights, order)
+        return _Combine.apply(y, weights, order, kind)
+    return _combine(y, weights, order, kind)
 
 
 def _combine_args(y, weights, order) -> int:
@@ -499,8 +498,7 @@ def _combine_args(y, weights, order) -> int:
     return kind
 
 
-def _combine(y, weights, order):
-    kind = _combine_args(y, weights, order)
+def _combine(y, weights, order, kind):
     y = _pitched(y)
     if weights is not None and not weights.is_contiguous():
         weights = weights.contiguous()
@@ -520,13 +518,11 @@ def combine_grad(grad: torch.Tensor, y: torch.Tensor | None, weights: torch.Tens
     rounded to its type, and zero from order.offsets[S] on; dweights[t, j] is the 32-bit dot product
     of grad[t] and y[order.places[t, j]], 0 without a place. y may be None without need_weights."""
     kind = _movable(grad, order.T, order, "grad")
-    H, n = grad.shape[1], order.T * order.k
     need_weights = need_weights and weights is not None
     if y is not None:
         _combine_args(y, weights, order)
-        _need(y.shape[1] == H and y.dtype == grad.dtype,
+        _need(y.shape[1] == grad.shape[1] and y.dtype == grad.dtype,
               f"y {y.dtype} {list(y.shape)} does not go with grad {grad.dtype} {list(grad.shape)}")
-        y = _pitched(y)
     else:
         _need(not need_weights, "the gradient of weights needs y")
         _need(weights is None or (weights.dtype == torch.float32 and
@@ -535,11 +531,17 @@ def combine_grad(grad: torch.Tensor, y: torch.Tensor | None, weights: torch.Tens
               f"weights must be float32 {list(order.places.shape)} on {order.device}")
     if torch.is_grad_enabled():
         _no_gradient(grad, y, weights)
+    if not (need_y or need_weights):
+        return None, None
+    return _combine_grad(grad, y, weights, order, kind, need_y, need_weights)
+
+
+def _combine_grad(grad, y, weights, order, kind, need_y, need_weights):
+    H, n = grad.shape[1], order.T * order.k
     grad = _pitched(grad)
+    y = _pitched(y) if need_weights else None
     dy = grad.new_empty((n, H)) if need_y else None
     dweights = grad.new_empty((order.T, order.k), dtype=torch.float32) if need_weights else None
-    if dy is None and dweights is None:
-        return None, None
     if weights is not None and not weights.is_contiguous():
         weights = weights.contiguous()
     _check(_on_device(order.device, _lib.lib().expert_cache_combine_grad, grad.data_ptr(), kind,
@@ -559,32 +561,35 @@ def _once() -> None:
                            "(create_graph)")
 
 
+# Autograd hands a result's gradient over in its shape and type, so `backward` checks neither again.
+
 class _Dispatch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, order):
-        ctx.order = order
-        return _dispatch(x, order)
+    def forward(ctx, x, order, kind):
+        ctx.of = order, kind
+        return _dispatch(x, order, kind)
 
     @staticmethod
     def backward(ctx, grad):
         _once()
-        return _combine(grad, None, ctx.order), None
+        order, kind = ctx.of
+        return _combine(grad, None, order, kind), None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, weights, order):
-        ctx.order = order
+    def forward(ctx, y, weights, order, kind):
+        ctx.of = order, kind
         ctx.save_for_backward(y if ctx.needs_input_grad[1] else None, weights)
-        return _combine(y, weights, order)
+        return _combine(y, weights, order, kind)
 
     @staticmethod
     def backward(ctx, grad):
         _once()
         y, weights = ctx.saved_tensors
+        order, kind = ctx.of
         need = ctx.needs_input_grad
-        return *combine_grad(grad, y, weights, ctx.order, need_y=need[0],
-                             need_weights=need[1]), None
+        return *_combine_grad(grad, y, weights, order, kind, need[0], need[1]), None, None
 
 
 # ---- products in 8-bit integers ------------------------------------------------------------
