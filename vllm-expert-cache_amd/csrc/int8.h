@@ -156,9 +156,8 @@ struct Product8Args {
   int splits;            // of the length, with Form::kPart
   int out_tiles;         // tiles along N
   // Experts8: tiles of the sorted rows
-  const int2* tiles;
+  const int4* tiles;     // slot, first row, end
   const int* n_tiles;
-  const int* offsets;
   const int* pairs;      // the pair at every sorted row; its token is pair / k
   int k;
   void* out;
@@ -286,10 +285,10 @@ struct Product8 {
   __device__ __forceinline__ Tile tile_of(int m_tile, int n_tile, int part, int cut) const {
     Tile t = {0, m_tile * TM, a.rows, n_tile * (kGated ? TN / 2 : TN)};
     if constexpr (kGrouped) {
-      const u32x2 of = load_uniform(reinterpret_cast<const u32x2*>(a.tiles) + m_tile);
+      const u32x4 of = load_uniform(reinterpret_cast<const u32x4*>(a.tiles) + m_tile);
       t.slot = (int)of[0];
       t.m0 = (int)of[1];
-      t.m_end = load_uniform(a.offsets + of[0] + 1);
+      t.m_end = (int)of[2];
     }
     t.m_end = min(t.m_end, t.m0 + TM);
     if (cut) {

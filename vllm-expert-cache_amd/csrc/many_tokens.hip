@@ -291,7 +291,7 @@ Moe8Plan moe8_plan(const expert_cache_experts* e, long T, long k) {
   p.rows = take(4 * n);
   p.places = take(4 * n);
   p.counts = take(sort_bytes((int)n, e->S));
-  p.tiles = take(8 * p.max_tiles);
+  p.tiles = take(16 * p.max_tiles);
   p.n_tiles = take(4);
   p.q = take(T * e->H);
   p.q_scale = take(4 * T);
@@ -596,7 +596,7 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   s.rows = ints(p.rows);
   s.places = ints(p.places);
   s.counts = ints(p.counts);
-  s.tiles = reinterpret_cast<int2*>(at + p.tiles);
+  s.tiles = reinterpret_cast<int4*>(at + p.tiles);
   s.n_tiles = ints(p.n_tiles);
   s.tile_rows = p.tile_rows;
   s.chunk = sort_chunk(s.n);
@@ -621,7 +621,6 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   a.K = e->H;
   a.tiles = s.tiles;
   a.n_tiles = s.n_tiles;
-  a.offsets = s.offsets;
   a.pairs = s.rows;
   a.k = top_k;
   a.out = floats(p.h);

@@ -33,7 +33,7 @@ struct SortArgs {
   int* rows;
   int* places;
   int* counts;         // [blocks, S + 1]
-  int2* tiles;         // of Experts8: slot and first row of every tile, and their number
+  int4* tiles;         // of Experts8: slot, first row and end of every tile, and their number
   int* n_tiles;
   int tile_rows;
   bool large_first;    // tiles of half their rows or fewer behind all others
@@ -177,7 +177,7 @@ __device__ __forceinline__ void sort_place(const SortArgs& a) {
       for (int j = 0, at = ahead; j < kPer; at += all[j++])
         for (int row = 0; row < all[j]; row += a.tile_rows)
           a.tiles[is_small(all[j] - row) ? small++ : large++] =
-              make_int2(threadIdx.x * kPer + j, at + row);
+              make_int4(threadIdx.x * kPer + j, at + row, at + min(all[j], row + a.tile_rows), 0);
       if (last) *a.n_tiles = n_large + n_small;
     }
   }
