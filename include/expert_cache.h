@@ -347,9 +347,9 @@ int expert_cache_sort(const void* ids, int id_bytes, int T, int top_k, int S, in
  * places outside [0, T * top_k) are left out. x [T, H] and out [T * top_k, H] are of `type` (0-2),
  * rows x_stride and out_stride elements apart. The gradient of x is expert_cache_combine of out's
  * without weights.
- * Fails with -1 unless sizes are as for expert_cache_sort, 0 < H <= 2^20, T * H < 2^43,
- * strides are at least H (or there is one row), no array is null (unless T is 0), and out meets no
- * other.
+ * Fails with -1 unless sizes are as for expert_cache_sort, 0 < H <= 2^20, x's values are at most
+ * 2^35 bytes, strides are at least H (or there is one row), no array is null (unless T is 0), and
+ * out meets no other.
  */
 int expert_cache_dispatch(const void* x, int type, long x_stride, const int* places,
                           const int* rows, int T, int top_k, int H, void* out, long out_stride,
@@ -358,7 +358,8 @@ int expert_cache_dispatch(const void* x, int type, long x_stride, const int* pla
 /*
  * Back to the tokens: out[t] = sum_j weights[t, j] * y[places[t, j]], summed in 32 bits in the
  * order of j and rounded to `type`. y [T * top_k, H], out [T, H]; weights float[T, top_k], or null
- * for 1. A pair without a place or with a weight of 0 adds nothing. Fails with -1 as above.
+ * for 1. A pair without a place or with a weight of 0 adds nothing. Fails with -1 as above, with out's
+ * values in place of x's.
  */
 int expert_cache_combine(const void* y, int type, long y_stride, const float* weights,
                          const int* places, int T, int top_k, int H, void* out, long out_stride,
@@ -383,7 +384,7 @@ int expert_cache_combine_grad(const void* grad, int type, long grad_stride, cons
  * apart; q int8 with rows q_stride bytes apart, 16-byte aligned with q_stride a multiple of 16, and
  * zeros from H to the next multiple of 16. A row below 2^-119 throughout counts as zeros, scale 0;
  * one with an infinity or NaN becomes zeros with a scale of NaN.
- * Fails with -1 unless 0 <= T <= 2^24, 0 < H <= 2^20, strides hold a row (or there is one), no
+ * Fails with -1 unless 0 <= T <= 2^23, 0 < H <= 2^20, strides hold a row (or there is one), no
  * array is null (unless T is 0) and the results meet no other array.
  */
 int expert_cache_quantize(const void* x, int type, long x_stride, int T, int H, void* q,
@@ -410,9 +411,9 @@ int expert_cache_linear8_workspace(const expert_cache_linear* l, int type, int T
  * of type BF16 or F16 and quantised by the call as expert_cache_quantize does it (x_scales is not
  * read then), or INT8 with x_scales float[T], laid out like expert_cache_quantize's q (what is
  * behind H may be anything). out [T, O] is of out_type (0-2). `workspace` as for expert_cache_moe.
- * Fails with -1 unless 0 < H <= 131056, 0 < O <= 2^24, 0 <= T <= 2^24, strides hold a row (or there
- * is one) and those of 8-bit rows are at most 2^22, no array is null but as said (unless T is 0),
- * and out meets neither x nor x_scales.
+ * Fails with -1 unless 0 < H <= 131056, 0 < O <= 2^24, 0 <= T <= 2^23, T * O <= 2^38, strides hold a
+ * row (or there is one) and those of 8-bit rows are at most 2^22, no array is null but as said
+ * (unless T is 0), and out meets neither x nor x_scales.
  */
 int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, long x_stride,
                          const float* x_scales, int T, void* out, int out_type, long out_stride,
@@ -428,9 +429,10 @@ int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, 
  * Pairs are sorted by slot, so that a slot's weights serve all its pairs. The same call gives the
  * same bits, and a token's do not depend on the tokens beside it.
  * Fails with -1 unless the layer is as for expert_cache_moe with INT8 weights, S <= 1024, H and I
- * are multiples of 16 and at most 131056, 2 * I * H and T * H are at most 1.75 * 2^30, sizes are
- * otherwise as for expert_cache_sort, strides hold a row (or there is one), id_bytes is 4 or 8, no array is null
- * (unless T is 0), and out meets no other array.
+ * are multiples of 16 and at most 131056, 2 * I * H and T * H are at most 1.75 * 2^30, T * top_k is
+ * at most 2^23 and its product with H and with I 2^36, sizes are otherwise as for expert_cache_sort,
+ * strides hold a row (or there is one), id_bytes is 4 or 8, no array is null (unless T is 0), and out
+ * meets no other array.
  */
 int expert_cache_moe8_workspace(const expert_cache_experts* e, int T, int top_k, long* bytes);
 int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_stride,

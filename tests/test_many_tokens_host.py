@@ -177,6 +177,22 @@ def test_moe8_workspace_rejects(lib, over):
     assert _moe8(lib, bytes=True, **over) == -1
 
 
+# A launch has less than 2^32 threads: what would need more is refused before the first of a call.
+@pytest.mark.parametrize("entry,over", [
+    (_dispatch, dict(T=2 ** 24, k=1, H=1025, xs=1025, os=1025)),
+    (_dispatch, dict(T=2 ** 23, k=1, type=0, H=1025, xs=1025, os=1025)),
+    (_combine, dict(T=2 ** 24, k=1, H=1025, ys=1025, os=1025)),
+    (_combine_grad, dict(T=2 ** 24, k=1, H=1025, gs=1025, ys=1025, ds=1025)),
+    (_quantize, dict(T=2 ** 23 + 1)), (_linear, dict(T=2 ** 23 + 1)),
+    (_linear, dict(T=2 ** 23, O=2 ** 15 + 1, os=2 ** 16)), (_moe8, dict(T=2 ** 23 + 1, k=1)),
+    (_moe8, dict(T=2 ** 20 + 1, k=64, I=1024)), (_moe8, dict(T=2 ** 22, k=2, I=8208)),
+    (_moe8, dict(T=2 ** 17, k=64, H=8208, xs=8208, os=8208)),
+    (_moe8, dict(bytes=True, T=2 ** 22, k=2, I=8208)),
+    (_moe8, dict(bytes=True, T=2 ** 23 + 1, k=1))], ids=str)
+def test_calls_of_more_than_a_launch_holds_are_rejected(lib, entry, over):
+    assert entry(lib, **over) == -1
+
+
 def test_null_handles_are_rejected(lib):
     size = ctypes.c_long()
     at = ctypes.addressof(size)
@@ -280,6 +296,31 @@ def test_dispatch_arguments(order, x):
         x = x.detach().requires_grad_(wants and x.is_floating_point())
         with pytest.raises(ValueError):
             ops.dispatch(x, order)
+
+
+def test_more_rows_than_a_launch_moves_are_refused(anywhere):
+    order = ops.Order(torch.zeros(5, dtype=torch.int32), torch.zeros(2 ** 20, dtype=torch.int32),
+                      torch.zeros((2 ** 20, 1), dtype=torch.int32), 4)
+    for dtype, H in ((BF16, 16385), (F32, 8193)):
+        rows = torch.zeros(1, 1, dtype=dtype).expand(2 ** 20, H)
+        for call in (lambda: ops.dispatch(rows, order), lambda: ops.combine(rows, None, order),
+                     lambda: ops.combine_grad(rows, rows, None, order)):
+            with pytest.raises(ValueError, match="bytes"):
+                call()
+
+
+def test_more_tokens_than_a_launch_holds_are_refused(anywhere):
+    one = torch.zeros(1, 1, dtype=BF16)
+    with pytest.raises(ValueError, match="rows"):
+        ops.quantize(one.expand(2 ** 23 + 1, 1))
+    with pytest.raises(ValueError, match="tokens"):
+        _lin()(one.expand(2 ** 23 + 1, 32))
+    layer = ops.Experts8(*_w(I=1024), *_s(I=1024))
+    for T, k, of in ((2 ** 23 + 1, 1, layer), (2 ** 20, 64, layer),
+                     (2 ** 22, 2, ops.Experts8(*_w(I=8208), *_s(I=8208)))):
+        with pytest.raises(ValueError, match="pairs"):
+            of(one.expand(T, 32), torch.zeros(1, 1).expand(T, k),
+               torch.zeros(1, 1, dtype=torch.int32).expand(T, k))
 
 
 @pytest.mark.parametrize("y,w", [

@@ -19,7 +19,13 @@ namespace {
 
 constexpr int kMaxTopK = 64;
 constexpr int kMaxRow = 1 << 20;        // elements of a row that is moved
-constexpr long long kMaxGrid = 0x7FFFFFFFll;
+// A launch has less than 2^32 threads, and these keep every one's below that:
+constexpr long long kMaxMoved = 1ll << 35;   // bytes of the tokens' rows that are moved (a wave takes
+                                             // 1 KB of a row, and there are up to 2^24 tokens)
+constexpr int kMaxTokens8 = 1 << 23;         // rows that are quantised, at most a workgroup of 256 each
+constexpr long long kMaxValues8 = 1ll << 36; // hidden values and experts' outputs (tiles of 512
+                                             // threads for 2^15 of them, and one a slot)
+constexpr long long kMaxResults8 = 1ll << 38;
 
 long up(long v, long to) { return (v + to - 1) / to * to; }
 bool type_bad(int type) { return type < EXPERT_CACHE_F32 || type > EXPERT_CACHE_F16; }
@@ -106,6 +112,10 @@ int with_rows(int type, int H, long long moved, std::initializer_list<const void
   return (int)hipGetLastError();
 }
 
+bool moved_bad(long long T, int H, int type) {
+  return type_bad(type) || H <= 0 || H > kMaxRow || T * H * size_of(type) > kMaxMoved;
+}
+
 bool rows_bad(long rows, const void* x, long stride, int H) {
   return x == nullptr || (rows > 1 && stride < H);
 }
@@ -151,7 +161,6 @@ int launch_product(Product8Args& a, long long m_tiles, int outputs, hipStream_t 
   // every die's tiles, of which the last may be cut in parts: four of less than a quarter of its units
   const long long per = (m_tiles * a.out_tiles * (FORM == Form::kPart ? a.splits : 1) + 7) / 8;
   const long long blocks = 8 * (per + 3 * kDieUnits / 4);
-  if (blocks > kMaxGrid) return -1;
   hipLaunchKernelGGL((product8_k<TM, TN, WM, WN, ST, FORM, OUT>), dim3((unsigned)blocks),
                      dim3(WM * WN * kWave), 0, stream, a);
   return (int)hipGetLastError();
@@ -191,8 +200,6 @@ int launch_few(const Product8Args& a, const void* x, long x_stride, int H, hipSt
                      (long long)x_stride, H);
   return (int)hipGetLastError();
 }
-
-
 
 template <class OUT>
 int launch_dense(Product8Args& a, const DensePlan& plan, int* part, hipStream_t stream) {
@@ -260,7 +267,7 @@ bool linear_bad(const expert_cache_linear* l, int type, int T) {
   if (l->w_stride % 16 || l->w_stride < l->H || l->w_stride > (1 << 22)) return true;
   if (type != EXPERT_CACHE_BF16 && type != EXPERT_CACHE_F16 && type != EXPERT_CACHE_INT8)
     return true;
-  return T < 0 || T > (1 << 24) || l->O > (1 << 24);
+  return T < 0 || T > kMaxTokens8 || l->O > (1 << 24) || (long long)T * l->O > kMaxResults8;
 }
 
 struct Moe8Plan {
@@ -308,7 +315,9 @@ bool moe8_bad(const expert_cache_experts* e, int T, int k) {
   if (e->weights != EXPERT_CACHE_INT8 || e->H % 16 || e->I % 16) return true;
   if (e->H > kMaxLength8 || e->I > kMaxLength8) return true;
   if (2LL * e->I * e->H > (long long)kMaxRange) return true;
-  return pairs_bad(T, k) || (long long)T * e->H > (long long)kMaxRange;
+  if (pairs_bad(T, k) || (long long)T * e->H > (long long)kMaxRange) return true;
+  const long long n = (long long)T * k;
+  return n > kMaxTokens8 || n * (e->H > e->I ? e->H : e->I) > kMaxValues8;
 }
 
 template <Form FORM>
@@ -361,7 +370,7 @@ int expert_cache_sort(const void* ids, int id_bytes, int T, int top_k, int S, in
 int expert_cache_dispatch(const void* x, int type, long x_stride, const int* places,
                           const int* rows, int T, int top_k, int H, void* out, long out_stride,
                           hipStream_t stream) {
-  if (pairs_bad(T, top_k) || type_bad(type) || H <= 0 || H > kMaxRow) return -1;
+  if (pairs_bad(T, top_k) || moved_bad(T, H, type)) return -1;
   if (T == 0) return 0;
   const long long n = (long long)T * top_k;
   if (rows_bad(T, x, x_stride, H) || rows_bad(n, out, out_stride, H)) return -1;
@@ -384,7 +393,6 @@ int expert_cache_dispatch(const void* x, int type, long x_stride, const int* pla
   const int per = kMovePieces * 1024 / size_of(type);
   a.chunks = (H + per - 1) / per;
   const long long blocks = ((long long)T * a.chunks + kMoveWaves - 1) / kMoveWaves;
-  if (blocks > kMaxGrid) return -1;
   return with_rows(type, H, out_bytes, {x, out}, {T > 1 ? x_stride : 0, n > 1 ? out_stride : 0},
                    [&](auto v, auto move) {
                      hipLaunchKernelGGL((dispatch_k<decltype(v), move.value>),
@@ -396,7 +404,7 @@ int expert_cache_dispatch(const void* x, int type, long x_stride, const int* pla
 int expert_cache_combine(const void* y, int type, long y_stride, const float* weights,
                          const int* places, int T, int top_k, int H, void* out, long out_stride,
                          hipStream_t stream) {
-  if (pairs_bad(T, top_k) || type_bad(type) || H <= 0 || H > kMaxRow) return -1;
+  if (pairs_bad(T, top_k) || moved_bad(T, H, type)) return -1;
   if (T == 0) return 0;
   const long long n = (long long)T * top_k;
   if (rows_bad(n, y, y_stride, H) || rows_bad(T, out, out_stride, H) || places == nullptr)
@@ -420,7 +428,6 @@ int expert_cache_combine(const void* y, int type, long y_stride, const float* we
   const int per = 1024 / size_of(type);
   a.chunks = (H + per - 1) / per;
   const long long blocks = ((long long)T * a.chunks + kMoveWaves - 1) / kMoveWaves;
-  if (blocks > kMaxGrid) return -1;
   return with_rows(type, H, span(n, y_stride, H, size_of(type)), {y, out},
                    {n > 1 ? y_stride : 0, T > 1 ? out_stride : 0}, [&](auto v, auto move) {
                      hipLaunchKernelGGL((combine_k<decltype(v), move.value>),
@@ -433,7 +440,7 @@ int expert_cache_combine_grad(const void* grad, int type, long grad_stride, cons
                               long y_stride, const float* weights, const int* places,
                               const int* rows, int T, int top_k, int H, void* dy, long dy_stride,
                               float* dweights, hipStream_t stream) {
-  if (pairs_bad(T, top_k) || type_bad(type) || H <= 0 || H > kMaxRow) return -1;
+  if (pairs_bad(T, top_k) || moved_bad(T, H, type)) return -1;
   if (dy == nullptr && dweights == nullptr) return -1;
   if (T == 0) return 0;
   const long long n = (long long)T * top_k;
@@ -480,7 +487,7 @@ int expert_cache_combine_grad(const void* grad, int type, long grad_stride, cons
 int expert_cache_quantize(const void* x, int type, long x_stride, int T, int H, void* q,
                           long q_stride, float* scales, hipStream_t stream) {
   if (type != EXPERT_CACHE_BF16 && type != EXPERT_CACHE_F16) return -1;
-  if (T < 0 || T > (1 << 24) || H <= 0 || H > kMaxRow) return -1;
+  if (T < 0 || T > kMaxTokens8 || H <= 0 || H > kMaxRow) return -1;
   if (T == 0) return 0;
   const long padded = up(H, 16);
   if (rows_bad(T, x, x_stride, H) || rows_bad(T, q, q_stride, (int)padded)) return -1;

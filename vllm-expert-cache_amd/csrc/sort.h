@@ -6,7 +6,8 @@
 // bit of the key, so its rank among the wave's equal keys is a count of lower lanes and the wave's
 // own counter in LDS: no place depends on the order of atomics. Sums of the counters over lower keys
 // and earlier waves give the places. Up to 4096 pairs are one workgroup's, their keys and ranks in
-// registers; more take a launch before that which counts every workgroup's keys.
+// registers; more take a launch before that which counts every workgroup's keys. 8 pairs take 3.0 us of
+// kernel, 1551 5.0, 32768 of 128 slots 2.8 and 5.5: a chain of loads, barriers and ballots, not bytes.
 //
 // The rows move as they lie: `dispatch` reads a token's row once and writes it to its k places,
 // `combine` reads the k rows and sums them in 32 bits in the order of j, and `combine_grad` is a wave
@@ -354,7 +355,8 @@ __global__ __launch_bounds__(kMoveWaves* kWave) void dispatch_k(MoveArgs a) {
 }
 
 // out[t] = sum_j weights[t, j] x[places[t, j]], in the order of j: a wave takes 1 KB of a token's
-// row. Lane j looks up pair j, so that the rows' loads wait for one load and not for one each.
+// row. Lane j looks up pair j, so that the rows' loads wait for one load and not for one each, and
+// eight of them are under way. 8192 tokens of 8 rows of 2048 bf16 take 50 us, 6.0 TB/s.
 template <class X, Move MOVE, class OUT = X>
 __global__ __launch_bounds__(kMoveWaves* kWave) void combine_k(MoveArgs a) {
   constexpr int kN = Piece<X>::kN, kAhead = 8;

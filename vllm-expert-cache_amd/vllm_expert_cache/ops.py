@@ -52,8 +52,12 @@ MAX_OUTPUTS = 1 << 21  # of an adapter
 MAX_LENGTH = 1 << 24   # of a row of weights: H and I
 MAX_SORTED = 1 << 24   # pairs of one sort: tokens x top_k
 MAX_ROW = 1 << 20      # values of a row that is dispatched, combined or quantised
+MAX_MOVED = 1 << 35    # bytes of the tokens' rows that are dispatched or combined
+MAX_TOKENS8 = 1 << 23  # rows that are quantised: tokens of 8-bit products, Experts8's pairs
 MAX_LENGTH8 = 131056   # of a sum of 8-bit products, which 32 bits hold
 MAX_BYTES8 = 7 << 28   # of Experts8's quantised tokens, and of an expert's w13
+MAX_VALUES8 = 1 << 36  # of its hidden values, and of its pairs' outputs
+MAX_RESULTS8 = 1 << 38 # of a Linear8
 
 
 def _check(rc: int, name: str) -> None:
@@ -440,6 +444,8 @@ def _movable(t, rows: int, order: Order, what: str) -> int:
                          f"{order.device}, not {t.dtype} {list(t.shape)} on {t.device}")
     if not 0 < t.shape[1] <= MAX_ROW:
         raise ValueError(f"rows of {t.shape[1]} (1 to {MAX_ROW})")
+    if order.T * t.shape[1] * t.element_size() > MAX_MOVED:
+        raise ValueError(f"{order.T} tokens of {t.shape[1]} {t.dtype} values ({MAX_MOVED} bytes)")
     return kind
 
 
@@ -451,7 +457,8 @@ def _recordable() -> None:
 
 def dispatch(x: torch.Tensor, order: Order) -> torch.Tensor:
     """The tokens' rows in the slots' order, [T * k, H]: row p is x[order.rows[p] // k], and rows
-    from order.offsets[S] on are zeros. x [T, H] is float32, bfloat16 or float16; H up to 2^20.
+    from order.offsets[S] on are zeros. x [T, H] is float32, bfloat16 or float16; H up to 2^20, x up
+    to 2^35 bytes.
 
     Differentiable in x, once: a token's gradient is the 32-bit sum of its rows', rounded to x's
     type. `combine(gradient, None, order)` is the same without autograd, for a call that is
@@ -476,7 +483,7 @@ def _dispatch(x, order, kind):
 def combine(y: torch.Tensor, weights: torch.Tensor | None, order: Order) -> torch.Tensor:
     """Rows back to their tokens: [T, H], token t the sum over j of weights[t, j] times
     y[order.places[t, j]], in 32 bits and rounded to y's type. y [T * k, H] is float32, bfloat16 or
-    float16, weights float32 [T, k] or None (1). Pairs without a place or with a weight of 0 add
+    float16, the result up to 2^35 bytes, weights float32 [T, k] or None (1). Pairs without a place or with a weight of 0 add
     nothing (and an infinity in their rows does not show).
 
     Differentiable in y and weights, once (`combine_grad` is the same without autograd, for a call
@@ -597,15 +604,15 @@ class _Combine(torch.autograd.Function):
 def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows as 8-bit integers and what 1 stands for: (q int8 [T, H], scales float32 [T]), with m a
     row's largest magnitude scales = m / 127 and q = 127 x / m to the nearest, ties to even. x is
-    bfloat16 or float16 [T, H], H up to 2^20; q's rows lie in ones of a multiple of 16. A row below
+    bfloat16 or float16 [T, H], T up to 2^23 and H 2^20; q's rows lie in ones of a multiple of 16. A row below
     2^-119 throughout counts as zeros, and one with an infinity or NaN becomes zeros with a scale
     of NaN."""
     kind = _TOKENS.get(x.dtype)
     if kind is None or x.dim() != 2:
         raise ValueError(f"x must be bfloat16 or float16 [T, H], not {x.dtype} {list(x.shape)}")
     T, H = x.shape
-    if T > MAX_SORTED or not 0 < H <= MAX_ROW:
-        raise ValueError(f"{T} rows (at most {MAX_SORTED}) of {H} (1 to {MAX_ROW})")
+    if T > MAX_TOKENS8 or not 0 < H <= MAX_ROW:
+        raise ValueError(f"{T} rows (at most {MAX_TOKENS8}) of {H} (1 to {MAX_ROW})")
     device = _on_gpu(x)
     if torch.is_grad_enabled() and x.requires_grad:
         _no_gradient(x)
@@ -621,7 +628,7 @@ def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 class Linear8:
     """A projection in 8-bit integers: y = x w^T + bias, tokens quantised with a scale each.
 
-    w      int8 [O, H], H up to 131056        scale  float32 [O] or [O, 1], one a channel
+    w      int8 [O, H], H up to 131056, O 2^24        scale  float32 [O] or [O, 1], one a channel
     bias   float32, bfloat16 or float16 [O], or None
 
     Sums are exact; their product with both scales and the bias's sum are in 32 bits, and the result
@@ -668,8 +675,9 @@ class Linear8:
             raise ValueError(f"x must be bfloat16, float16 or int8 [T, {self.H}] on {self.device}, "
                              f"not {x.dtype} {list(x.shape)} on {x.device}")
         T = x.shape[0]
-        if T > MAX_SORTED:
-            raise ValueError(f"{T} tokens (at most {MAX_SORTED})")
+        if T > MAX_TOKENS8 or T * self.O > MAX_RESULTS8:
+            raise ValueError(f"{T} tokens (at most {MAX_TOKENS8}) of {self.O} results "
+                             f"({MAX_RESULTS8} in all)")
         if dtype is None:
             dtype = torch.bfloat16 if kind == 3 else x.dtype
         to = _LOGITS.get(dtype)
@@ -764,7 +772,7 @@ class Experts8:
                  out: torch.Tensor | None = None) -> torch.Tensor:
         """The layer's output [T, H] for tokens x [T, H] in bfloat16 or float16: the sum over their
         slots of the routing weight (float32 [T, top_k]) times the expert. slot_ids [T, top_k] are
-        int32 or int64; T x top_k is at most 2^24, T x H 1.75 * 2^30. A pair whose id is outside
+        int32 or int64; T x top_k is at most 2^23, T x H 1.75 * 2^30. A pair whose id is outside
         [0, S) or whose weight is 0 adds nothing; a token without any other pair gets zeros. `out`,
         if given, has contiguous rows and overlaps no other argument."""
         struct = self._structs.get(x.dtype)
@@ -778,9 +786,10 @@ class Experts8:
                              f"on {self.device}, not {topk_weights.dtype} "
                              f"{list(topk_weights.shape)} on {topk_weights.device}")
         k = shape[1]
-        if not 1 <= k <= MAX_TOP_K or T * k > MAX_SORTED or T * self.H > MAX_BYTES8:
+        if not 1 <= k <= MAX_TOP_K or T * k > MAX_TOKENS8 or T * self.H > MAX_BYTES8 or \
+                T * k * max(self.H, self.I) > MAX_VALUES8:
             raise ValueError(f"{T} tokens of {self.H} x top_k {k} (top_k at most {MAX_TOP_K}, "
-                             f"{MAX_SORTED} pairs, {MAX_BYTES8} values)")
+                             f"{MAX_TOKENS8} pairs, {MAX_BYTES8} values, {MAX_VALUES8} of the pairs')")
         if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or
                                         self._graded or out is not None):
             _no_gradient(x, topk_weights, out, *self._graded)
