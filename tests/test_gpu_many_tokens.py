@@ -10,11 +10,13 @@ side: `_moe8` finds those and allows each a step.
 """
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import gpu_util as gu
-from vllm_expert_cache import ops
+from vllm_expert_cache import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -529,6 +531,37 @@ def test_linear8_of_other_strides():
     lin(wide[:, :H], out=out[:, 2:2 + O])
     assert torch.equal(out[:, 2:2 + O], lin(wide[:, :H]))
     assert (out[:, :2] == 7).all() and (out[:, 2 + O:] == 7).all()
+
+
+# One row has no stride: in tiles (O from 8192 on) the rows that a tile has behind it touch nothing,
+# whatever stride is given. Long rows are cut along the length, with scales that end where they end.
+@pytest.mark.parametrize("H,O", [(1001, 8201), (6211, 8191 + 2), (70, 8192)])
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_linear8_of_one_row_of_any_stride(H, O, dtype):
+    g = _gen(23)
+    w = _whole(g, O, H)
+    lin = ops.Linear8(w, torch.rand(O, device=DEV, generator=g))
+    x, s = ops.quantize(_randn(g, 1, H).to(BF16))
+    if dtype == BF16:
+        x, s = _randn(g, 1, H).to(BF16), None
+        q, m = _quantized(x)
+        want, bound = _linear(q, m, lin, None)
+    else:
+        want = x.double() @ w.double().t() * s.double() * lin.scale.double()
+        bound = _gamma(3) * want.abs()
+    kind = 1 if dtype == BF16 else 3
+    h, size = _lib.lib(), ctypes.c_long()
+    assert h.expert_cache_linear8_workspace(lin._at, kind, 1, ctypes.addressof(size)) == 0
+    work = torch.empty(max(size.value, 16), dtype=torch.uint8, device=DEV)
+    for x_stride, out_stride in ((0, 0), (16, 4), (x.stride(0), O), (2 ** 22, 2 ** 20)):
+        out = torch.full((O + 64,), 7.0, device=DEV)
+        torch.cuda.synchronize()
+        assert h.expert_cache_linear8(lin._at, x.data_ptr(), kind, x_stride,
+                                      None if s is None else s.data_ptr(), 1, out.data_ptr(), 0,
+                                      out_stride, work.data_ptr(), None) == 0
+        torch.cuda.synchronize()
+        _close(out[None, :O], want, bound)
+        assert (out[O:] == 7).all()
 
 
 def test_linear8_shows_infinities_in_their_rows_alone():

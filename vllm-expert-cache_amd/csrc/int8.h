@@ -345,17 +345,20 @@ struct Product8 {
       for (int i = 0; i < kA; ++i)
         a_at[i] = (unsigned)(token(t, (i * kWaves + wave) * 8 + (lane >> 3)) * a.a_stride) +
                   16 * chunk;
-    char* const to = lds + kRoom;
-    const __amdgpu_buffer_rsrc_t w_scales = range_of(a.w_scale + (long long)t.slot * a.N, 4ll * a.N);
-    const __amdgpu_buffer_rsrc_t a_scales = range_of(a.a_scale, 4ll * a.scale_rows);
+    if constexpr (FORM != Form::kPart) {  // whose N goes to whole cells, behind the scales' end
+      char* const to = lds + kRoom;
+      const __amdgpu_buffer_rsrc_t w_scales =
+          range_of(a.w_scale + (long long)t.slot * a.N, 4ll * a.N);
+      const __amdgpu_buffer_rsrc_t a_scales = range_of(a.a_scale, 4ll * a.scale_rows);
 #pragma unroll
-    for (int i = 0; i < (kScaleLoads + kWaves - 1) / kWaves; ++i) {
-      const int part = i * kWaves + wave, r = part * kWave + lane;
-      if (part < TN / kWave) {
-        const int o = t.n0 + (kGated && r >= TN / 2 ? width + r - TN / 2 : r);
-        load_word_to_lds(w_scales, to + part * 256, 4 * o);
-      } else if (part < kScaleLoads) {
-        load_word_to_lds(a_scales, to + part * 256, 4 * token(t, r - TN));
+      for (int i = 0; i < (kScaleLoads + kWaves - 1) / kWaves; ++i) {
+        const int part = i * kWaves + wave, r = part * kWave + lane;
+        if (part < TN / kWave) {
+          const int o = t.n0 + (kGated && r >= TN / 2 ? width + r - TN / 2 : r);
+          load_word_to_lds(w_scales, to + part * 256, 4 * o);
+        } else if (part < kScaleLoads) {
+          load_word_to_lds(a_scales, to + part * 256, 4 * token(t, r - TN));
+        }
       }
     }
 #pragma unroll

@@ -528,6 +528,11 @@ int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, 
       (whole && ranges_meet(x_scales, 4LL * T, out, out_bytes)))
     return -1;
   Product8Args a = {};
+  // one row may come with any stride; a tile's rows behind it have to lie behind its end
+  if (T == 1) {
+    x_stride = whole ? K : l->H;
+    out_stride = l->O;
+  }
   a.a = static_cast<const int8_t*>(x);
   a.a_stride = x_stride;
   a.a_scale = x_scales;
