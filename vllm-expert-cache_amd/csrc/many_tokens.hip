@@ -245,6 +245,7 @@ struct Linear8Layout {
 Linear8Layout linear8_layout(const expert_cache_linear* l, int type, long T) {
   const long K = up(l->H, 16);
   Linear8Layout p = {};
+  if (T == 0) return p;  // no tiles that a plan could put beside each other
   if (type != EXPERT_CACHE_INT8) {
     p.scales = up(T * K, 256);
     p.part = p.scales + up(4 * T, 256);
