@@ -6,6 +6,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from vllm_expert_cache import _lib, ops
 
@@ -24,6 +25,7 @@ def no_kernels(monkeypatch):
     calls = []
     monkeypatch.setattr(ops, "_on_gpu", lambda *t: t[0].device)
     monkeypatch.setattr(ops, "_on_device", lambda device, call, *args: calls.append(args) or 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return calls
 
 
@@ -51,3 +53,82 @@ def test_a_layer_of_no_tokens(lib):
     for S, H, I in ((1, 16, 16), (1024, 131056, 16)):
         e = _lib.Experts(S, H, I, 1, 3, 16, 16, 16, 16)
         assert lib.expert_cache_moe8_workspace(ctypes.addressof(e), 0, 8, ctypes.addressof(size)) == 0
+
+
+# ---- forward-mode derivatives -------------------------------------------------------------
+
+def _order(T=3, k=2, S=4):
+    return ops.Order(torch.zeros(S + 1, dtype=torch.int32), torch.zeros(T * k, dtype=torch.int32),
+                     torch.zeros((T, k), dtype=torch.int32), S)
+
+
+def _tensors():
+    """Arguments of every operator; those that may be floating point can have a tangent."""
+    return dict(
+        x=torch.zeros(3, 32, dtype=BF16), y=torch.zeros(6, 32, dtype=BF16),
+        g=torch.zeros(3, 32, dtype=BF16), p=torch.zeros(3, 2),
+        i=torch.zeros(3, 2, dtype=torch.int32), i1=torch.zeros(3, dtype=torch.int32),
+        logits=torch.zeros(3, 16), gate=torch.zeros(16), w=torch.zeros(6, 32, dtype=I8),
+        s=torch.ones(6), b=torch.ones(6), b16=torch.ones(6, dtype=BF16),
+        q=torch.zeros(3, 32, dtype=I8), qs=torch.ones(3), out6=torch.zeros(3, 6, dtype=BF16),
+        out32=torch.zeros(3, 32, dtype=BF16), base=torch.zeros(3, 6, dtype=BF16),
+        w13=torch.zeros(2, 32, 32, dtype=I8), w2=torch.zeros(2, 32, 16, dtype=I8),
+        s13=torch.ones(2, 32), s2=torch.ones(2, 32), v13=torch.zeros(2, 32, 32, dtype=BF16),
+        v2=torch.zeros(2, 32, 16, dtype=BF16), down=torch.zeros(2, 8, 32, dtype=BF16),
+        up=torch.zeros(2, 6, 8, dtype=BF16), factors=torch.ones(2))
+
+
+# (call, the arguments that can have a tangent)
+CALLS = {
+    "route": (lambda t: ops.route(t["logits"], 2, bias=t["gate"]), ("logits", "gate")),
+    "dispatch": (lambda t: ops.dispatch(t["x"], _order()), ("x",)),
+    "combine": (lambda t: ops.combine(t["y"], t["p"], _order()), ("y", "p")),
+    "combine_grad": (lambda t: ops.combine_grad(t["g"], t["y"], t["p"], _order()), ("g", "y", "p")),
+    "quantize": (lambda t: ops.quantize(t["x"]), ("x",)),
+    "linear8": (lambda t: ops.Linear8(t["w"], t["s"], t["b"])(t["x"], out=t["out6"]),
+                ("x", "s", "b", "out6")),
+    "linear8 copied": (lambda t: ops.Linear8(t["w"], t["s"], t["b16"])(t["x"]), ("b16",)),
+    "linear8 whole": (lambda t: ops.Linear8(t["w"], t["s"])(t["q"], t["qs"]), ("qs", "s")),
+    "experts8": (lambda t: ops.Experts8(t["w13"], t["w2"], t["s13"], t["s2"])(
+        t["x"], t["p"], t["i"], out=t["out32"]), ("x", "p", "s13", "s2", "out32")),
+    "experts": (lambda t: ops.Experts(t["v13"], t["v2"])(t["x"], t["p"], t["i"], out=t["out32"]),
+                ("x", "p", "v13", "v2", "out32")),
+    "experts int8": (lambda t: ops.Experts(t["w13"], t["w2"], t["s13"], t["s2"])(
+        t["x"], t["p"], t["i"]), ("x", "s13", "s2")),
+    "adapters": (lambda t: ops.Adapters(t["down"], t["up"], t["factors"])(
+        t["x"], t["base"], t["i1"], out=t["out6"]),
+        ("x", "base", "down", "up", "factors", "out6")),
+}
+TANGENTS = [(op, name) for op, (_, names) in CALLS.items() for name in names]
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+@pytest.mark.parametrize("op,name", TANGENTS)
+def test_a_tangent_is_refused_and_not_dropped(no_kernels, op, name, no_grad):
+    call, t = CALLS[op][0], _tensors()
+    with forward_ad.dual_level(), torch.set_grad_enabled(not no_grad):
+        call(t)  # a level alone changes nothing
+        assert len(no_kernels) == 1
+        primal = t[name]
+        t[name] = forward_ad.make_dual(primal, torch.ones_like(primal))
+        with pytest.raises(ValueError, match="forward-mode"):
+            call(t)
+        assert len(no_kernels) == 1
+        t[name] = forward_ad.unpack_dual(t[name]).primal
+        call(t)
+    assert len(no_kernels) == 2
+
+
+@pytest.mark.parametrize("of", ["dispatch", "combine"])
+def test_a_tangent_of_a_gradient_is_refused(no_kernels, of):
+    """Forward over reverse: the backward pass is a call like any other."""
+    leaf = torch.zeros((3, 32) if of == "dispatch" else (6, 32), requires_grad=True)
+    weights = torch.zeros(3, 2, requires_grad=True)
+    out = ops.dispatch(leaf, _order()) if of == "dispatch" else ops.combine(leaf, weights, _order())
+    with forward_ad.dual_level():
+        grad = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(out, leaf, grad, retain_graph=True)
+        assert len(no_kernels) == 1
+        torch.autograd.grad(out, leaf, torch.ones_like(out))
+    assert len(no_kernels) == 2

@@ -23,7 +23,8 @@ tensors' device, allocate only their result and a workspace through torch, and r
 they can be captured.
 
 `dispatch` and `combine` have a backward pass. The others have none: with gradients enabled, a tensor
-that requires one (a handle's weights: when the handle is made) is refused.
+that requires one (a handle's weights: when the handle is made) is refused. None has a forward-mode
+derivative: a tensor with a tangent (torch.autograd.forward_ad) is refused everywhere.
 
 ValueError names an argument that an operator does not take; nothing has run then.
 """
@@ -32,6 +33,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -113,6 +115,16 @@ def _no_gradient(*tensors) -> None:
                              f"pass: detach it, or call under torch.no_grad()")
 
 
+def _no_tangent(*tensors) -> None:
+    """Refuses a tensor with a forward-mode derivative: the kernels would drop it, and the result
+    count as a constant. Only inside a level of `torch.autograd.forward_ad` has a tensor one, so calls
+    look for a level first; whether gradients are enabled makes no difference to it."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"a tensor {list(t.shape)} has a forward-mode derivative and there is "
+                             f"none of the result: pass forward_ad.unpack_dual(t).primal")
+
+
 def _graded(*weights) -> list:
     """A handle's weights that require a gradient: looked for once, since each look at a tensor
     is a tenth of a microsecond of a call."""
@@ -160,6 +172,8 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
         raise ValueError(f"bias must be contiguous float32 [{E}], not {bias.dtype} "
                          f"{list(bias.shape)}")
     device = _on_gpu(logits, bias)
+    if forward_ad._current_level >= 0:
+        _no_tangent(logits, bias)
     if torch.is_grad_enabled() and (logits.requires_grad or bias is not None):
         _no_gradient(logits, bias)
     step = logits.stride()
@@ -260,6 +274,8 @@ class Experts:
         if not 1 <= k <= MAX_TOP_K or T * k > MAX_PAIRS:
             raise ValueError(f"{T} tokens x top_k {k} (top_k at most {MAX_TOP_K}, {MAX_PAIRS} in "
                              f"all)")
+        if forward_ad._current_level >= 0:
+            _no_tangent(x, topk_weights, out, self.w13, self.w2, self.w13_scale, self.w2_scale)
         if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or
                                         self._graded or out is not None):
             _no_gradient(x, topk_weights, out, *self._graded)
@@ -343,6 +359,8 @@ class Adapters:
         if slot_ids.shape != (T,) or T > MAX_TOKENS:
             raise ValueError(f"slot_ids must be [{T}], not {list(slot_ids.shape)}, of at most "
                              f"{MAX_TOKENS} tokens")
+        if forward_ad._current_level >= 0:
+            _no_tangent(x, base, out, self.a, self.b, self.scales)
         if torch.is_grad_enabled() and (x.requires_grad or base.requires_grad or self._graded or
                                         out is not None):
             _no_gradient(x, base, out, *self._graded)
@@ -464,6 +482,8 @@ def dispatch(x: torch.Tensor, order: Order) -> torch.Tensor:
     type. `combine(gradient, None, order)` is the same without autograd, for a call that is
     captured; one that autograd would record is refused then."""
     kind = _movable(x, order.T, order, "x")
+    if forward_ad._current_level >= 0:
+        _no_tangent(x)
     if x.requires_grad and torch.is_grad_enabled():
         _recordable()
         return _Dispatch.apply(x, order, kind)
@@ -489,6 +509,8 @@ def combine(y: torch.Tensor, weights: torch.Tensor | None, order: Order) -> torc
     Differentiable in y and weights, once (`combine_grad` is the same without autograd, for a call
     that is captured; one that autograd would record is refused then)."""
     kind = _combine_args(y, weights, order)
+    if forward_ad._current_level >= 0:
+        _no_tangent(y, weights)
     if (y.requires_grad or (weights is not None and weights.requires_grad)) and \
             torch.is_grad_enabled():
         _recordable()
@@ -536,6 +558,8 @@ def combine_grad(grad: torch.Tensor, y: torch.Tensor | None, weights: torch.Tens
                                   weights.shape == order.places.shape and
                                   weights.device == order.device),
               f"weights must be float32 {list(order.places.shape)} on {order.device}")
+    if forward_ad._current_level >= 0:
+        _no_tangent(grad, y, weights)
     if torch.is_grad_enabled():
         _no_gradient(grad, y, weights)
     if not (need_y or need_weights):
@@ -562,10 +586,12 @@ def _combine_grad(grad, y, weights, order, kind, need_y, need_weights):
     return dy, dweights
 
 
-def _once() -> None:
+def _once(*tensors) -> None:
     if torch.is_grad_enabled():
         raise RuntimeError("dispatch and combine are differentiable once: their gradients have none "
                            "(create_graph)")
+    if forward_ad._current_level >= 0:
+        _no_tangent(*tensors)
 
 
 # Autograd hands a result's gradient over in its shape and type, so `backward` checks neither again.
@@ -578,7 +604,7 @@ class _Dispatch(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        _once()
+        _once(grad)
         order, kind = ctx.of
         return _combine(grad, None, order, kind), None, None
 
@@ -592,8 +618,8 @@ class _Combine(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        _once()
         y, weights = ctx.saved_tensors
+        _once(grad, y, weights)
         order, kind = ctx.of
         need = ctx.needs_input_grad
         return *_combine_grad(grad, y, weights, order, kind, need[0], need[1]), None, None
@@ -614,6 +640,8 @@ def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if T > MAX_TOKENS8 or not 0 < H <= MAX_ROW:
         raise ValueError(f"{T} rows (at most {MAX_TOKENS8}) of {H} (1 to {MAX_ROW})")
     device = _on_gpu(x)
+    if forward_ad._current_level >= 0:
+        _no_tangent(x)
     if torch.is_grad_enabled() and x.requires_grad:
         _no_gradient(x)
     x = _pitched(x)
@@ -647,6 +675,8 @@ class Linear8:
             _need(bias.dtype in _LOGITS and bias.shape == (O,),
                   f"bias must be float32, bfloat16 or float16 [{O}], not {bias.dtype} "
                   f"{list(bias.shape)}")
+        if forward_ad._current_level >= 0:
+            _no_tangent(bias)  # a copy of it may be kept
         self._graded = _graded(w, scale, bias)
         step = w.stride()
         if H % 16 or w.data_ptr() % 16 or step[1] != 1 or \
@@ -688,6 +718,8 @@ class Linear8:
                 x_scales.device != self.device)):
             raise ValueError(f"int8 tokens, and no others, have x_scales: float32 [{T}] on "
                              f"{self.device}")
+        if forward_ad._current_level >= 0:
+            _no_tangent(x, x_scales, out, self.scale, self.bias)
         if torch.is_grad_enabled() and (x.requires_grad or self._graded or out is not None or
                                         x_scales is not None):
             _no_gradient(x, x_scales, out, *self._graded)
@@ -790,6 +822,8 @@ class Experts8:
                 T * k * max(self.H, self.I) > MAX_VALUES8:
             raise ValueError(f"{T} tokens of {self.H} x top_k {k} (top_k at most {MAX_TOP_K}, "
                              f"{MAX_TOKENS8} pairs, {MAX_BYTES8} values, {MAX_VALUES8} of the pairs')")
+        if forward_ad._current_level >= 0:
+            _no_tangent(x, topk_weights, out, self.w13, self.w2, self.w13_scale, self.w2_scale)
         if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or
                                         self._graded or out is not None):
             _no_gradient(x, topk_weights, out, *self._graded)
