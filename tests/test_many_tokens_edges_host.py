@@ -132,3 +132,47 @@ def test_a_tangent_of_a_gradient_is_refused(no_kernels, of):
         assert len(no_kernels) == 1
         torch.autograd.grad(out, leaf, torch.ones_like(out))
     assert len(no_kernels) == 2
+
+
+# ---- traces -------------------------------------------------------------------------------
+
+TRACED = {name: call for name, (call, _) in CALLS.items()}
+TRACED["sort"] = lambda t: ops.sort(t["i"], 4)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+@pytest.mark.parametrize("op", TRACED)
+@pytest.mark.parametrize("how", ["trace", "make_fx"])
+def test_a_trace_is_refused(monkeypatch, op, how):
+    """It would hold the allocation of the result and nothing that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    class Library:
+        launches = []
+
+        def __getattr__(self, name):
+            if name.endswith("_workspace"):
+                return lambda *args: 0
+            return lambda *args: self.launches.append(name) or 0
+
+    library, t = Library(), _tensors()
+    monkeypatch.setattr(ops._lib, "lib", lambda: library)
+    monkeypatch.setattr(ops, "_on_gpu", lambda *t: t[0].device)
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(ops, "_workspace", lambda *args: 16)
+
+    def of(x):
+        out = TRACED[op](t)
+        return out.places if op == "sort" else out[0] if isinstance(out, tuple) else out
+
+    of(t["x"])
+    assert len(library.launches) == 1
+    with pytest.raises(ValueError, match="trace"):
+        if how == "trace":
+            torch.jit.trace(of, t["x"], check_trace=False)
+        else:
+            make_fx(of)(t["x"])
+    assert len(library.launches) == 1
+    of(t["x"])
+    assert len(library.launches) == 2

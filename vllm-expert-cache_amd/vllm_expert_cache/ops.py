@@ -24,7 +24,8 @@ they can be captured.
 
 `dispatch` and `combine` have a backward pass. The others have none: with gradients enabled, a tensor
 that requires one (a handle's weights: when the handle is made) is refused. None has a forward-mode
-derivative: a tensor with a tangent (torch.autograd.forward_ad) is refused everywhere.
+derivative: a tensor with a tangent (torch.autograd.forward_ad) is refused everywhere. They are no
+registered torch operators, and a call that torch.jit.trace or make_fx would record is refused.
 
 ValueError names an argument that an operator does not take; nothing has run then.
 """
@@ -73,8 +74,18 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# Whether torch.jit.trace runs, and whether a graph of torch's own operators is recorded from real
+# tensors (make_fx). Neither sees a kernel launch, only the result's allocation.
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_mode = getattr(torch._C, "_get_dispatch_mode", lambda key: None)
+_PROXY = getattr(getattr(torch._C, "_TorchDispatchModeKey", None), "PROXY", None)
+
+
 def _on_device(device: torch.device, call, *args):
     """call(*args, stream) on the current stream of `device`, with that device current."""
+    if _tracing() or _mode(_PROXY) is not None:
+        raise ValueError("a trace would keep the result's memory without what fills it: leave the "
+                         "call outside what is traced")
     index = device.index
     if index == torch.cuda.current_device():
         return call(*args, _raw_stream(index))
