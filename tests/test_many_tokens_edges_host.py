@@ -176,3 +176,30 @@ def test_a_trace_is_refused(monkeypatch, op, how):
     assert len(library.launches) == 1
     of(t["x"])
     assert len(library.launches) == 2
+
+
+# ---- results that meet what the call reads ------------------------------------------------
+
+S, H, I, T, K = 4, 32, 16, 2, 2
+LAYER = dict(w13=(0x10000, S * 2 * I * H), w2=(0x20000, S * H * I), s13=(0x30000, 4 * S * 2 * I),
+             s2=(0x40000, 4 * S * H), x=(0x50000, 2 * T * H), probs=(0x60000, 4 * T * K),
+             ids=(0x70000, 4 * T * K), work=(0x80000, None))
+
+
+def _workspace_of(lib):
+    size = ctypes.c_long()
+    e = _lib.Experts(S, H, I, 1, 3, 16, 16, 16, 16)
+    assert lib.expert_cache_moe8_workspace(ctypes.addressof(e), T, K, ctypes.addressof(size)) == 0
+    return size.value
+
+
+@pytest.mark.parametrize("name", LAYER)
+def test_a_layers_result_over_what_it_reads_is_refused(lib, name):
+    """Its first byte on the array's last, and its last on the array's first: -1, before any launch."""
+    at = {n: first for n, (first, _) in LAYER.items()}
+    first, size = LAYER[name]
+    size = _workspace_of(lib) if size is None else size
+    e = _lib.Experts(S, H, I, 1, 3, at["w13"], at["w2"], at["s13"], at["s2"])
+    for out in (first + size - 1, first - 2 * T * H + 1):
+        assert lib.expert_cache_moe8(ctypes.addressof(e), at["x"], H, at["probs"], at["ids"], 4, T, K,
+                                     out, H, at["work"], None) == -1

@@ -589,11 +589,13 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   if (topk_weights == nullptr || ids == nullptr) return -1;
   if (workspace == nullptr || !aligned16(workspace)) return -1;
   const long long out_bytes = span(T, out_stride, e->H, 2), n = (long long)T * top_k;
-  if (ranges_meet(x, span(T, x_stride, e->H, 2), out, out_bytes) ||
-      ranges_meet(ids, n * id_bytes, out, out_bytes) ||
-      ranges_meet(topk_weights, 4 * n, out, out_bytes))
-    return -1;
+  const long long slot = (long long)e->I * e->H;
   const Moe8Plan p = moe8_plan(e, T, top_k);
+  const void* const in[] = {x, ids, topk_weights, e->w13, e->w2, e->s13, e->s2, workspace};
+  const long long in_bytes[] = {span(T, x_stride, e->H, 2), n * id_bytes, 4 * n, 2 * e->S * slot,
+                                e->S * slot, 8LL * e->S * e->I, 4LL * e->S * e->H, p.bytes};
+  for (int i = 0; i < 8; ++i)
+    if (ranges_meet(in[i], in_bytes[i], out, out_bytes)) return -1;
   char* const at = static_cast<char*>(workspace);
   const auto ints = [&](long offset) { return reinterpret_cast<int*>(at + offset); };
   const auto floats = [&](long offset) { return reinterpret_cast<float*>(at + offset); };
