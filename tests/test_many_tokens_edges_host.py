@@ -203,3 +203,23 @@ def test_a_layers_result_over_what_it_reads_is_refused(lib, name):
     for out in (first + size - 1, first - 2 * T * H + 1):
         assert lib.expert_cache_moe8(ctypes.addressof(e), at["x"], H, at["probs"], at["ids"], 4, T, K,
                                      out, H, at["work"], None) == -1
+
+
+# ---- a caller's `out` ---------------------------------------------------------------------
+
+INTO = {"linear8": "out6", "experts8": "out32", "experts": "out32", "adapters": "out6"}
+
+
+@pytest.mark.parametrize("op", INTO)
+def test_a_write_into_out_is_counted(no_kernels, op):
+    """A backward pass that saved `out` before finds that it was written since."""
+    t = _tensors()
+    out, factor = t[INTO[op]], torch.ones((), dtype=BF16, requires_grad=True)
+    product = out * factor
+    CALLS[op][0](t)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():  # where nothing is counted
+        t[INTO[op]] = torch.empty_like(out)
+        CALLS[op][0](t)
+    assert len(no_kernels) == 2

@@ -294,7 +294,8 @@ class Experts:
         if not topk_weights.is_contiguous():
             topk_weights = topk_weights.contiguous()
         x = _rows(x)
-        if out is None:
+        given = out is not None
+        if not given:
             out = x.new_empty((T, self.H))
         else:
             _out(out, x.dtype, (T, self.H), self.device)
@@ -306,6 +307,8 @@ class Experts:
         _check(_on_device(self.device, h.expert_cache_moe, at, x.data_ptr(), x.stride(0),
                           topk_weights.data_ptr(), ids.data_ptr(), nbytes, T, k, out.data_ptr(),
                           out.stride(0), work.data_ptr()), "expert_cache_moe")
+        if given:
+            _written(out)
         return out
 
 
@@ -319,6 +322,13 @@ def _out(out, dtype, shape, device) -> None:
     _need(out.dtype == dtype and tuple(out.shape) == shape and out.device == device and
           out.stride(1) == 1 and (shape[0] < 2 or out.stride(0) >= shape[1]),
           f"out must be {dtype} {list(shape)} on {device} with contiguous rows")
+
+
+def _written(out) -> None:
+    """Counts the write into a caller's `out`, as torch does for its own operators: a backward pass
+    that saved what it held is refused then, and doesn't go on with what it holds now."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
 
 
 class Adapters:
@@ -377,7 +387,8 @@ class Adapters:
             _no_gradient(x, base, out, *self._graded)
         ids, nbytes = _ids(slot_ids, device)
         x = _rows(x)
-        if out is None:
+        given = out is not None
+        if not given:
             out = x.new_empty((T, self.O))
         else:
             _out(out, dtype, (T, self.O), device)
@@ -391,6 +402,8 @@ class Adapters:
         _check(_on_device(device, h.expert_cache_adapt, self._at, x.data_ptr(), x.stride(0),
                           ids.data_ptr(), nbytes, T, base.data_ptr(), base.stride(0),
                           out.data_ptr(), out.stride(0), work.data_ptr()), "expert_cache_adapt")
+        if given:
+            _written(out)
         return out
 
 
@@ -740,7 +753,8 @@ class Linear8:
                 x_scales = x_scales.contiguous()
         else:
             x = _pitched(x)
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((T, self.O), dtype=dtype, device=self.device)
         else:
             _out(out, dtype, (T, self.O), self.device)
@@ -756,6 +770,8 @@ class Linear8:
                           max(x.stride(0), self.H), None if kind != 3 else x_scales.data_ptr(), T,
                           out.data_ptr(), to, max(out.stride(0), self.O), work.data_ptr()),
                "expert_cache_linear8")
+        if given:
+            _written(out)
         return out
 
     def _whole(self, x: torch.Tensor) -> torch.Tensor:
@@ -842,7 +858,8 @@ class Experts8:
         if not topk_weights.is_contiguous():
             topk_weights = topk_weights.contiguous()
         x = _pitched(x)
-        if out is None:
+        given = out is not None
+        if not given:
             out = x.new_empty((T, self.H))
         else:
             _out(out, x.dtype, (T, self.H), self.device)
@@ -857,4 +874,6 @@ class Experts8:
                           max(x.stride(0), self.H), topk_weights.data_ptr(), ids.data_ptr(), nbytes,
                           T, k, out.data_ptr(), max(out.stride(0), self.H), work.data_ptr()),
                "expert_cache_moe8")
+        if given:
+            _written(out)
         return out
