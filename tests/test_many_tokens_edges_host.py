@@ -223,3 +223,20 @@ def test_a_write_into_out_is_counted(no_kernels, op):
         t[INTO[op]] = torch.empty_like(out)
         CALLS[op][0](t)
     assert len(no_kernels) == 2
+
+
+# ---- workspaces ---------------------------------------------------------------------------
+
+# tokens, outputs, length and parts of it: as many as have room beside each other (256 tiles of 64 x
+# 64), as leave each eight steps of 128, and eight at most
+@pytest.mark.parametrize("T,O,H,parts", [(70, 130, 6200, 6), (130, 1029, 6160, 5), (20, 77, 8300, 8),
+                                         (64, 4096, 14336, 4), (1, 8192, 6017, 2), (1, 8192, 6016, 1),
+                                         (1, 8193, 8192, 1), (1, 10, 131056, 1)])
+def test_workspaces_hold_the_parts_of_a_length(lib, T, O, H, parts):
+    K = -(-H // 16) * 16
+    l, size = _lib.Linear(O, H, K, 16, 16, None), ctypes.c_long()
+    sums = 4 * parts * T * -(-O // 4) * 4 if parts > 1 else 0
+    assert lib.expert_cache_linear8_workspace(ctypes.addressof(l), 3, T, ctypes.addressof(size)) == 0
+    assert size.value == sums
+    assert lib.expert_cache_linear8_workspace(ctypes.addressof(l), 1, T, ctypes.addressof(size)) == 0
+    assert size.value >= T * K + 4 * T + sums
