@@ -511,7 +511,9 @@ __global__ __launch_bounds__(WM* WN* kWave) void product8_k(Product8Args a) {
   const bool part = at >= whole;
   int tile = from + (part ? whole + ((at - whole) >> cut) : at);
   if constexpr (FORM == Form::kPart) {
-    // neighbours have the same part of the length; whole steps, as many each but for the last
+    // neighbours have the same part of the length; whole steps, as many each but for the last, which has
+    // one at least with eight steps or more a part and at most eight parts (the bound below zero guards
+    // what dense_plan doesn't ask for)
     const int split = __builtin_amdgcn_readfirstlane(tile / (m_tiles * a.out_tiles));
     tile -= split * m_tiles * a.out_tiles;
     const int steps = (a.K + kStepBytes - 1) / kStepBytes;
