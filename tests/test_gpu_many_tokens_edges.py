@@ -1,6 +1,6 @@
 """The operators for many tokens (vllm_expert_cache/ops.py) on the GPU where their plans change: one row
-through parts of a length, long products in every tile, slots that just fill a small tile, tiles in
-their own order. Against the formulas in 64 bits and the tolerances of `test_gpu_many_tokens.py`."""
+through parts of a length, long products in every tile, slots that just fill a small tile, many
+tiles. Against the formulas in 64 bits and the tolerances of `test_gpu_many_tokens.py`."""
 from __future__ import annotations
 
 import ctypes
@@ -117,10 +117,9 @@ def test_experts8_of_every_fill_of_small_tiles():
     assert torch.equal(got, e(x, probs, ids))
 
 
-def test_experts8_of_tiles_in_their_own_order():
-    """So many tiles of 256 rows that short ones aren't put behind the others."""
+def test_experts8_of_many_tiles_of_256_rows():
     T, k, S, H, I = 33000, 2, 8, 1024, 48
-    assert T * k >= 256 * S and T * k // 256 * (H // 256) >= 1024
+    assert T * k >= 256 * S
     e = many._experts(92, S, H, I)
     x, probs, ids = many._tokens(93, T, k, S, H, BF16, torch.int32)
     got = e(x, probs, ids)

@@ -615,8 +615,6 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   s.n_tiles = ints(p.n_tiles);
   s.tile_rows = p.tile_rows;
   s.chunk = sort_chunk(s.n);
-  // few tiles: their order decides when the last one ends; many share weights with their neighbours
-  s.large_first = p.tile_rows == 256 && n / 256 * (e->H / 256) < 4 * 256;
   QuantizeArgs z = {x, x_stride, T, e->H, nullptr, bytes(p.q), e->H, floats(p.q_scale)};
   int rc = e->type == EXPERT_CACHE_BF16 ? launch_begin<Bf16>(s, z, stream)
                                         : launch_begin<F16>(s, z, stream);
@@ -680,6 +678,8 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   const auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kMoveWaves * kWave), 0, stream, m);
   };
+  // outputs that the launch before has written: 6000 tokens, 8 of 64 slots of 2048 x 768 (393 MB), 472 us
+  // a layer past the caches and 491 through them; 4096, 4 of 16 of 2048 x 4096 (134 MB), 592 and 596
   const bool once = 4 * n * e->H >= kOnceBytes;
   if (e->type == EXPERT_CACHE_BF16)
     once ? launch(combine_k<float, Move::kOnce, Bf16>) : launch(combine_k<float, Move::kWhole, Bf16>);

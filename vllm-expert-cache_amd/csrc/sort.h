@@ -22,6 +22,8 @@ constexpr int kSortMaxSlots = 1024;
 constexpr int kSortMaxPairs = 1 << 24;
 constexpr int kSortOne = 4096;      // pairs that one workgroup sorts
 constexpr int kSortLot = 1024;      // pairs that a workgroup of many takes at a time
+// Workgroups at most, since each reads the counts of all: 2^20 pairs of 128 slots take 26 us, with up to
+// 128 of them 27 and with 512 35; 2^24 pairs 164, 294 and 134.
 constexpr int kSortMaxBlocks = 256;
 constexpr int kMoveWaves = 4;       // waves of a workgroup that moves rows
 
@@ -37,7 +39,6 @@ struct SortArgs {
   int4* tiles;         // of Experts8: slot, first row and end of every tile, and their number
   int* n_tiles;
   int tile_rows;
-  bool large_first;    // tiles of half their rows or fewer behind all others
 };
 
 __device__ __forceinline__ int sort_key(const SortArgs& a, int i) {
@@ -164,22 +165,18 @@ __device__ __forceinline__ void sort_place(const SortArgs& a) {
     }
     if (last) a.offsets[a.S] = live;
     if (a.tiles) {
-      int large = 0, small = 0, n_large, n_small;
-      const auto is_small = [&](int rows) { return a.large_first && 2 * rows <= a.tile_rows; };
+      // slot by slot; tiles of half their rows or fewer behind all others were 1 % slower (2048 tokens, 2
+      // of 8 slots of 4096 x 14336, 900 us and 891; 4096, 4 of 16 of 2048 x 4096, 592 and 582)
+      int tile = 0, tiles;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int part = all[j] % a.tile_rows, apart = part != 0 && is_small(part);
-        large += (all[j] + a.tile_rows - 1) / a.tile_rows - apart;
-        small += apart;
-      }
-      large = before_me<W>(large, word, n_large);
-      small = n_large + before_me<W>(small, word, n_small);
+      for (int j = 0; j < kPer; ++j) tile += (all[j] + a.tile_rows - 1) / a.tile_rows;
+      tile = before_me<W>(tile, word, tiles);
 #pragma unroll
       for (int j = 0, at = ahead; j < kPer; at += all[j++])
         for (int row = 0; row < all[j]; row += a.tile_rows)
-          a.tiles[is_small(all[j] - row) ? small++ : large++] =
+          a.tiles[tile++] =
               make_int4(threadIdx.x * kPer + j, at + row, at + min(all[j], row + a.tile_rows), 0);
-      if (last) *a.n_tiles = n_large + n_small;
+      if (last) *a.n_tiles = tiles;
     }
   }
   for (int lot = lo;;) {
