@@ -424,15 +424,16 @@ int expert_cache_linear8(const expert_cache_linear* l, const void* x, int type, 
  * weights (with their scales, as for expert_cache_moe; the formula and what ids and weights mean
  * are also its):
  *   both projections' inputs are quantised row by row as by expert_cache_quantize, the hidden
- *   values from 32 bits; their products are exact, the rest is in 32 bits, and out [T, H] is
- *   rounded to the layer's type. A token with an infinity or NaN gets NaN.
+ *   values from 32 bits; their products are exact, the rest is in 32 bits (the exponential of the
+ *   gate g to (2 |g| + 4) 2^-24 of itself), and out [T, H] is rounded to the layer's type. A token
+ *   with an infinity or NaN gets NaN.
  * Pairs are sorted by slot, so that a slot's weights serve all its pairs. The same call gives the
  * same bits, and a token's do not depend on the tokens beside it.
  * Fails with -1 unless the layer is as for expert_cache_moe with INT8 weights, S <= 1024, H and I
  * are multiples of 16 and at most 131056, 2 * I * H and T * H are at most 1.75 * 2^30, T * top_k is
  * at most 2^23 and its product with H and with I 2^36, sizes are otherwise as for expert_cache_sort,
  * strides hold a row (or there is one), id_bytes is 4 or 8, no array is null (unless T is 0), and out
- * meets no other array.
+ * meets no other array: x, ids, topk_weights, the weights, their scales or the workspace.
  */
 int expert_cache_moe8_workspace(const expert_cache_experts* e, int T, int top_k, long* bytes);
 int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_stride,

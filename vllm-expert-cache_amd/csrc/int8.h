@@ -14,14 +14,15 @@
 // a 16-row operand read from all banks. Loads past an array's end are the buffer descriptor's to
 // answer with zeros: rows behind the last, and what is behind a row's end in the last step.
 //
-// What bounds them. 4096 x 4096 x 14336 (256 tiles of 256 x 256) takes 174 us, 2.8 POP/s; a step of
-// such a tile is 2048 clocks of matrix instructions and as many of LDS (192 KB of operands and 64 KB of
-// loads at 128 bytes a clock) and takes 2700, at the 1.9 GHz to which the card goes under such loads.
-// Each tile has about 10 us besides: its first loads, and 128 KB of results, which all compute units
-// store at the same time. So 4096 x 14336 x 4096 takes 219 to 230 us, 2.1 POP/s. A workgroup for several
-// tiles that loads the next one's first steps before it stores was no faster (247 us for four tiles
-// each of 4096 x 16384 x 4096, where a workgroup for each takes 229), and steps of 64 bytes and stores
-// past the caches weren't either.
+// What bounds them (sizes as tokens, length x outputs). 4096 of 14336 x 4096, a tile of 256 x 256 for
+// every compute unit, takes 174 to 195 us by the card's clock, 2.5 to 2.8 POP/s; a step of such a tile
+// is 2048 clocks of matrix instructions and as many of LDS (192 KB of operands and 64 KB of loads at
+// 128 bytes a clock) and takes 2700, at the 1.9 GHz to which the card goes under such loads. Each tile
+// has about 10 us besides: its first loads, and 128 KB of results, which all compute units store at the
+// same time. So 4096 of 4096 x 14336 takes 215 to 230 us, 2.1 POP/s. A workgroup for several tiles that
+// loads the next one's first steps before it stores was no faster (247 us for four tiles each of 4096
+// of 4096 x 16384, where a workgroup for each takes 229), and steps of 64 bytes and stores past the
+// caches weren't either.
 #pragma once
 #include "mfma.h"
 #include "sort.h"
@@ -229,7 +230,12 @@ __device__ __forceinline__ void landed() {
 // most TM / 16 / WM) gives every wave less to do. A gate-up tile's weights are TN / 2 rows of the gate
 // and the same of the up projection, so that a lane holds both of a hidden value. Hidden values and an
 // expert's outputs go on in 32 bits: rounding hidden values to bf16 before they are quantised would
-// move about one in forty to the neighbouring whole number (2^-9 of a value, of up to 127 steps).
+// move about one in forty to the neighbouring whole number (2^-9 of a value, of up to 127 steps). SiLU's
+// exponential is the instruction's, off by up to (2 |gate| + 4) 2^-24 of itself: a hidden value that is
+// nearer than 32-bit arithmetic to half way between two whole numbers may go to either, which moves
+// results of 2048 tokens by 1.0e-4 to 1.6e-4 of their size from another 32-bit form's, both 0.0017 off
+// the formula in 64 bits by their rounding to bf16. The library's own exponential takes 1 to 2 % longer:
+// 2048 tokens, 2 of 8 slots of 4096 x 14336, 917 us and 903.
 template <int TM, int TN, int WM, int WN, int ST, Form FORM, class OUT>
 struct Product8 {
   static constexpr int kWaves = WM * WN;
@@ -500,7 +506,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void product8_k(Product8Args a) {
   // Consecutive workgroups go to the eight dies in turn: each die gets a run of tiles, so that
   // its second-level cache holds what they share. Of its last tiles, fewer than it has compute units,
   // each is cut in two or four where that many parts fit beside each other: 4096 tokens of 4096 x 14336
-  // (3.5 tiles a compute unit) 223 us, uncut 240; 2048 tokens, 8 of 128 slots of 2048 x 768, 269 and 273.
+  // (3.5 tiles a compute unit) 223 us, uncut 240; 2048, 8 of 128 slots of 2048 x 768, 269 and 273.
   const int m_tiles = P::kGrouped ? load_uniform(a.n_tiles) : (a.rows + TM - 1) / TM;
   const int splits = FORM == Form::kPart ? a.splits : 1;
   const int n = m_tiles * a.out_tiles * splits, per = (n + 7) / 8, from = (blockIdx.x & 7) * per;
@@ -513,8 +519,9 @@ __global__ __launch_bounds__(WM* WN* kWave) void product8_k(Product8Args a) {
   int tile = from + (part ? whole + ((at - whole) >> cut) : at);
   if constexpr (FORM == Form::kPart) {
     // neighbours have the same part of the length; whole steps, as many each but for the last, which has
-    // one at least with eight steps or more a part and at most eight parts (the bound below zero guards
-    // what dense_plan doesn't ask for)
+    // one at least, since dense_plan makes at most eight parts of eight steps or more. The bound at zero
+    // below is never met; without it this compiler waits a state too few at the loop's end for sums that
+    // it moves there, as the test of the built code shows.
     const int split = __builtin_amdgcn_readfirstlane(tile / (m_tiles * a.out_tiles));
     tile -= split * m_tiles * a.out_tiles;
     const int steps = (a.K + kStepBytes - 1) / kStepBytes;

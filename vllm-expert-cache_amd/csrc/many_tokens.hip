@@ -678,8 +678,9 @@ int expert_cache_moe8(const expert_cache_experts* e, const void* x, long x_strid
   const auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kMoveWaves * kWave), 0, stream, m);
   };
-  // outputs that the launch before has written: 6000 tokens, 8 of 64 slots of 2048 x 768 (393 MB), 472 us
-  // a layer past the caches and 491 through them; 4096, 4 of 16 of 2048 x 4096 (134 MB), 592 and 596
+  // The launch before has written these rows: 6000 tokens, 8 of 64 slots of 2048 x 768 (393 MB), take
+  // 472 us a layer past the caches and 491 through them; 4096, 4 of 16 of 2048 x 4096 (134 MB), 592 and
+  // 596.
   const bool once = 4 * n * e->H >= kOnceBytes;
   if (e->type == EXPERT_CACHE_BF16)
     once ? launch(combine_k<float, Move::kOnce, Bf16>) : launch(combine_k<float, Move::kWhole, Bf16>);

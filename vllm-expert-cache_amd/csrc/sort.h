@@ -165,8 +165,8 @@ __device__ __forceinline__ void sort_place(const SortArgs& a) {
     }
     if (last) a.offsets[a.S] = live;
     if (a.tiles) {
-      // slot by slot; tiles of half their rows or fewer behind all others were 1 % slower (2048 tokens, 2
-      // of 8 slots of 4096 x 14336, 900 us and 891; 4096, 4 of 16 of 2048 x 4096, 592 and 582)
+      // Slot by slot: with tiles of half their rows or fewer behind all others 2048 tokens, 2 of 8 slots
+      // of 4096 x 14336, took 900 us and not 891, and 4096, 4 of 16 of 2048 x 4096, 592 and not 582.
       int tile = 0, tiles;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) tile += (all[j] + a.tile_rows - 1) / a.tile_rows;

@@ -527,8 +527,8 @@ def _dispatch(x, order, kind):
 def combine(y: torch.Tensor, weights: torch.Tensor | None, order: Order) -> torch.Tensor:
     """Rows back to their tokens: [T, H], token t the sum over j of weights[t, j] times
     y[order.places[t, j]], in 32 bits and rounded to y's type. y [T * k, H] is float32, bfloat16 or
-    float16, the result up to 2^35 bytes, weights float32 [T, k] or None (1). Pairs without a place or with a weight of 0 add
-    nothing (and an infinity in their rows does not show).
+    float16, the result up to 2^35 bytes, weights float32 [T, k] or None (1). Pairs without a place or
+    with a weight of 0 add nothing (and an infinity in their rows does not show).
 
     Differentiable in y and weights, once (`combine_grad` is the same without autograd, for a call
     that is captured; one that autograd would record is refused then)."""
@@ -654,9 +654,9 @@ class _Combine(torch.autograd.Function):
 def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows as 8-bit integers and what 1 stands for: (q int8 [T, H], scales float32 [T]), with m a
     row's largest magnitude scales = m / 127 and q = 127 x / m to the nearest, ties to even. x is
-    bfloat16 or float16 [T, H], T up to 2^23 and H 2^20; q's rows lie in ones of a multiple of 16. A row below
-    2^-119 throughout counts as zeros, and one with an infinity or NaN becomes zeros with a scale
-    of NaN."""
+    bfloat16 or float16 [T, H], T up to 2^23 and H 2^20; q's rows lie in ones of a multiple of 16. A
+    row below 2^-119 throughout counts as zeros, and one with an infinity or NaN becomes zeros with a
+    scale of NaN."""
     kind = _TOKENS.get(x.dtype)
     if kind is None or x.dim() != 2:
         raise ValueError(f"x must be bfloat16 or float16 [T, H], not {x.dtype} {list(x.shape)}")
@@ -795,9 +795,11 @@ class Experts8:
     H and I are multiples of 16, S up to 1024.
 
     Tokens and hidden values are quantised row by row (`quantize`; hidden values from 32 bits), so
-    results differ from `Experts`' by the rounding of those. Sums are exact, the rest is in 32 bits,
-    the result is rounded to the tokens' type. The same call gives the same bits, and a token's are
-    the same among any others. A token with an infinity or NaN gets NaN."""
+    results differ from `Experts`' by the rounding of those. Sums are exact, the rest is in 32 bits
+    (the exponential of a gate value g to (2 |g| + 4) 2^-24 of itself, so a hidden value that near to
+    half way between two whole numbers may go to either), the result is rounded to the tokens' type.
+    The same call gives the same bits, and a token's are the same among any others. A token with an
+    infinity or NaN gets NaN."""
 
     def __init__(self, w13: torch.Tensor, w2: torch.Tensor, w13_scale: torch.Tensor,
                  w2_scale: torch.Tensor):
